@@ -65,8 +65,15 @@ class ServeStats(C.Structure):
                 ("active_seq_steps", C.c_longlong)]
 
 
+class KVView(C.Structure):
+    """hyc_kv_view: a paged KV cache in device memory."""
+    _fields_ = [("kv", C.c_void_p), ("pages", C.c_void_p), ("layers", C.c_int), ("npages", C.c_int),
+                ("kv_heads", C.c_int), ("hdim", C.c_int), ("slots", C.c_int), ("page_max", C.c_int)]
+
+
 # Every symbol include/hymt2_cuda.h declares, with its ctypes signature.
 P, I, F, Z = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+LL, KV = C.c_longlong, C.POINTER(KVView)
 SIGNATURES = {
     "hy_cuda_create": (P, [C.c_char_p, C.c_char_p, Z]),
     "hy_cuda_probe": (I, [C.c_char_p, I]),
@@ -116,6 +123,11 @@ SIGNATURES = {
     "hyc_trace": (I, [P, I]),
     "hyc_trace_read": (I, [P, P, I]),
     "hyc_attention_decode_noalloc": (I, [P, I, I, I, I, P, F, P, P, P, P, P, P, P, P, C.c_char_p, I]),
+    "hyc_tree_attention_ws": (Z, [KV, I, I]),
+    "hyc_tree_attention": (I, [P, KV, I, I, I, P, P, P, P, LL, I, F, P, LL, P, P, Z, C.c_char_p, I]),
+    "hyc_tree_commit": (I, [P, KV, I, P, P, P, P, P, P, P, P, P, P, C.c_char_p, I]),
+    "hyc_cache_weights": (I, [P, KV, I, I, P, P, P, P, LL, LL, I, P, LL, F, P, I, C.c_char_p, I]),
+    "hyc_cache_evict": (I, [P, KV, KV, P, P, I, I, I, I, P, P, P, C.c_char_p, I]),
     "hyc_attention_test": (I, [P, I, I, I, I, I, I, F, P, P, P, P, P, P, P, P]),
 }
 

@@ -19,8 +19,8 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
               "-Xcompiler", "-Wall"]
 CSRC = os.path.join(_paths.PKG, "csrc")
-SOURCES = ["hy_backend.cu"]
-HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith(".cuh"))  # every header the sources include
+SOURCES = ["hy_backend.cu", "hy_kvops.cu"]
+HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith((".cuh", ".h")))  # every header the sources include
 
 
 def _nvcc() -> str:
@@ -64,9 +64,12 @@ def build_backend(force: bool = False, trace: bool = False) -> None:
     objs = []
     for src in SOURCES:
         obj = os.path.join(objdir, src.replace(".cu", ".o"))
+        objs.append(obj)
+        own = [d for d in deps if not d.endswith(".cu") or os.path.basename(d) == src]
+        if not force and not _stale(obj, own):
+            continue
         _run([_nvcc(), *ARCH, *NVCC_FLAGS, *(["-DHYK_TRACE"] if trace else []), "-c", os.path.join(CSRC, src),
               "-o", obj])
-        objs.append(obj)
     tmp = so + ".tmp"
     _run([_nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", tmp, *objs, "-lrt", "-ldl", "-lpthread"])
     os.replace(tmp, so)

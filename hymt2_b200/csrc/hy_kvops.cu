@@ -1,0 +1,641 @@
+// hy_kvops.cu — operators on a paged bf16 KV cache: attention of drafted token
+// trees, acceptance of a drafted path, attention weights accumulated per
+// cached row, and eviction by them (include/hymt2_cuda.h states each).
+//
+// No counterpart in the reference: it decodes one token per step
+// (src/model.c:943-954) over a cache that only grows (:804-808).  The cache
+// is the batch engine's, [layer][page][K | V][16][kvdim]; row r of a slot is
+// row r % 16 of page pages[slot][r / 16].
+#include <cuda_runtime.h>
+
+#include <cstdio>
+#include <cstring>
+
+#include "../../include/hymt2_cuda.h"
+#include "hy_common.cuh"
+#include "hy_pages.h"
+
+using namespace hyk;
+
+namespace {
+
+constexpr int kTreeMax = 64;  // nodes of one tree
+
+struct KvView {
+    uint16_t *kv;
+    const int *pages;
+    int layers, npages, kvh, hd, slots, page_max, kvd;
+    long long page_stride, layer_stride;  // elements
+
+    // Page of row r of a slot, -1 when there is none.
+    __device__ __forceinline__ int page(int slot, int r) const {
+        if (r < 0 || (r >> kPageShift) >= page_max) return -1;
+        const int p = __ldg(pages + (size_t)slot * page_max + (r >> kPageShift));
+        return p < 0 || p >= npages ? -1 : p;
+    }
+    // Element offset of K row r in page p of a layer (V: + kPageRows * kvd).
+    __device__ __forceinline__ long long row(int layer, int p, int r) const {
+        return layer * layer_stride + (long long)p * page_stride + (long long)(r & (kPageRows - 1)) * kvd;
+    }
+};
+
+int op_fail(char *err, int cap, int code, const char *msg) {
+    if (err && cap > 0) snprintf(err, (size_t)cap, "%s", msg);
+    return code;
+}
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// The checked view; false with a message when the geometry is not served.
+bool make_view(const hyc_kv_view *v, KvView &o, const char **why) {
+    *why = nullptr;
+    if (!v || !v->kv || !v->pages) *why = "null cache view";
+    else if (v->layers < 1 || v->npages < 1 || v->kv_heads < 1 || v->slots < 1 || v->page_max < 1)
+        *why = "empty cache view";
+    else if (v->hdim != 64 && v->hdim != 128) *why = "hdim must be 64 or 128";
+    else if (!aligned16(v->kv)) *why = "the cache must be 16-byte aligned";
+    else if (v->page_max > (1 << 26) || v->slots > 65535 || v->kv_heads > 65535) *why = "cache view too large";
+    if (*why) return false;
+    o.kv = v->kv;
+    o.pages = v->pages;
+    o.layers = v->layers;
+    o.npages = v->npages;
+    o.kvh = v->kv_heads;
+    o.hd = v->hdim;
+    o.slots = v->slots;
+    o.page_max = v->page_max;
+    o.kvd = v->kv_heads * v->hdim;
+    o.page_stride = 2LL * kPageRows * o.kvd;
+    o.layer_stride = o.npages * o.page_stride;
+    return true;
+}
+
+bool group_ok(int heads, int kvh, int &G) {
+    if (heads < 1 || heads % kvh) return false;
+    G = heads / kvh;
+    return G == 1 || G == 2 || G == 4 || G == 8;
+}
+
+// ---------------------------------------------------------------- tree attention
+
+struct TreeArgs {
+    KvView v;
+    int layer, heads, G, max_nodes;
+    const int *len, *off, *parent;
+    const void *q;
+    long long q_ld;
+    float scale;
+    void *out;
+    long long out_ld;
+    float *lse;
+};
+
+template <typename T>
+__device__ __forceinline__ float ld_elem(const T *p);
+template <>
+__device__ __forceinline__ float ld_elem<float>(const float *p) { return *p; }
+template <>
+__device__ __forceinline__ float ld_elem<__nv_bfloat16>(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void st_elem(float *p, float v) { *p = v; }
+__device__ __forceinline__ void st_elem(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+
+// Slot s's cached rows and nodes, bounded by its page table and max_nodes.
+__device__ __forceinline__ void tree_span(const KvView &v, const int *len, const int *off, int max_nodes, int s, int &L,
+                                          int &t0, int &n) {
+    const int cap = v.page_max * kPageRows;
+    L = min(max(__ldg(len + s), 0), cap);
+    t0 = __ldg(off + s);
+    n = min(max(__ldg(off + s + 1) - t0, 0), max_nodes);
+}
+
+constexpr int kTreeWarps = 8;
+
+// grid (slots, kv heads, max_nodes): one node and KV head per CTA, its keys
+// round robin over the warps, a lane owning hd / 32 dims of every head.
+template <typename T, int HD, int G>
+__global__ void __launch_bounds__(kTreeWarps * 32) tree_attn_plain(const __grid_constant__ TreeArgs a) {
+    constexpr int D = HD / 32;
+    __shared__ float s_m[kTreeWarps][G], s_l[kTreeWarps][G], s_o[kTreeWarps][G][HD];
+    __shared__ unsigned long long s_mask;
+    const int s = blockIdx.x, kvh = blockIdx.y, node = blockIdx.z, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int L, t0, n;
+    tree_span(a.v, a.len, a.off, a.max_nodes, s, L, t0, n);
+    if (node >= n) return;
+    const int t = t0 + node;
+    if (threadIdx.x == 0) {  // the node and its ancestors
+        unsigned long long m = 0;
+        int p = a.parent[t], i = node;
+        if (p != -2) {
+            m = 1ull << node;
+            while (p >= 0 && p < i) {
+                i = p;
+                p = a.parent[t0 + i];
+                if (p == -2) break;
+                m |= 1ull << i;
+            }
+        }
+        s_mask = m;
+    }
+    __syncthreads();
+    const unsigned long long mask = s_mask;
+    float q[G][D], o[G][D], m[G], l[G];
+    const T *qr = (const T *)a.q + (long long)t * a.q_ld + (long long)kvh * G * HD;
+#pragma unroll
+    for (int h = 0; h < G; h++) {
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+#pragma unroll
+        for (int d = 0; d < D; d++) {
+            q[h][d] = ld_elem<T>(qr + h * HD + lane * D + d);
+            o[h][d] = 0.f;
+        }
+    }
+    const int end = mask ? L + n : 0;
+    for (int r = w; r < end; r += kTreeWarps) {
+        if (r >= L && !((mask >> (r - L)) & 1)) continue;
+        if ((r >> kPageShift) >= a.v.page_max) break;
+        const int pg = a.v.page(s, r);
+        float k[D], v[D];
+#pragma unroll
+        for (int d = 0; d < D; d++) k[d] = v[d] = 0.f;
+        if (pg >= 0) {
+            const uint16_t *kr = a.v.kv + a.v.row(a.layer, pg, r) + kvh * HD + lane * D;
+#pragma unroll
+            for (int d = 0; d < D; d++) {
+                k[d] = bf16_bits_to_f32(kr[d]);
+                v[d] = bf16_bits_to_f32(kr[kPageRows * a.v.kvd + d]);
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < G; h++) {
+            float x = 0.f;
+#pragma unroll
+            for (int d = 0; d < D; d++) x = fmaf(q[h][d], k[d], x);
+            x = warp_sum(x) * a.scale;
+            const float mn = fmaxf(m[h], x);
+            const float c = m[h] == -INFINITY ? 0.f : expf(m[h] - mn), p = mn == -INFINITY ? 0.f : expf(x - mn);
+            m[h] = mn;
+            l[h] = l[h] * c + p;
+#pragma unroll
+            for (int d = 0; d < D; d++) o[h][d] = fmaf(p, v[d], o[h][d] * c);
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < G; h++) {
+        if (lane == 0) {
+            s_m[w][h] = m[h];
+            s_l[w][h] = l[h];
+        }
+#pragma unroll
+        for (int d = 0; d < D; d++) s_o[w][h][lane * D + d] = o[h][d];
+    }
+    __syncthreads();
+    for (int h = w; h < G; h += kTreeWarps) {
+        float M = -INFINITY, S = 0.f, O[D];
+#pragma unroll
+        for (int d = 0; d < D; d++) O[d] = 0.f;
+        for (int x = 0; x < kTreeWarps; x++) M = fmaxf(M, s_m[x][h]);
+        for (int x = 0; x < kTreeWarps; x++) {
+            const float f = s_m[x][h] == -INFINITY ? 0.f : expf(s_m[x][h] - M);
+            S = fmaf(s_l[x][h], f, S);
+#pragma unroll
+            for (int d = 0; d < D; d++) O[d] = fmaf(s_o[x][h][lane * D + d], f, O[d]);
+        }
+        T *dst = (T *)a.out + (long long)t * a.out_ld + (long long)(kvh * G + h) * HD + lane * D;
+#pragma unroll
+        for (int d = 0; d < D; d++) st_elem(dst + d, S > 0.f ? O[d] / S : 0.f);
+        if (a.lse && lane == 0) a.lse[(long long)t * a.heads + kvh * G + h] = S > 0.f ? M + logf(S) : -INFINITY;
+    }
+}
+
+// ---------------------------------------------------------------- tree commit
+
+struct CommitArgs {
+    KvView v;
+    int max_nodes;
+    const int *len, *off, *parent, *tokens, *next, *forced;
+    int *len_out, *naccept, *path, *bonus;
+};
+
+// grid (layers, slots).  Warp 0 walks the tree (the next node is the lowest
+// one whose parent and token match: two ballots per accepted node); then
+// thread c owns 16 bytes of a K or V row and moves the path's rows in order.
+// Row j of the path comes from row path[j] >= j, so a row is read before
+// anything is written over it.  CTAs of layer 0 write the outcome.
+__global__ void __launch_bounds__(128) tree_commit(const __grid_constant__ CommitArgs a) {
+    __shared__ int s_path[kTreeMax], s_n, s_last;
+    const int layer = blockIdx.x, s = blockIdx.y, lane = threadIdx.x & 31;
+    int L, t0, n;
+    tree_span(a.v, a.len, a.off, a.max_nodes, s, L, t0, n);
+    if (threadIdx.x < 32) {
+        int par[2], tok[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int i = lane + 32 * h;
+            par[h] = i < n ? a.parent[t0 + i] : -3;
+            tok[h] = i < n ? a.tokens[t0 + i] : 0;
+        }
+        int cnt = 0, cur = 0;
+        if (n > 0 && a.forced && a.forced[s]) {
+            for (int i = lane; i < n; i += 32) s_path[i] = i;
+            cnt = n;
+            cur = n - 1;
+        } else if (n > 0) {
+            for (;;) {
+                if (lane == 0) s_path[cnt] = cur;
+                cnt++;
+                const int want = a.next[t0 + cur];
+                const unsigned lo = __ballot_sync(0xffffffffu, par[0] == cur && lane > cur && tok[0] == want);
+                const unsigned hi = __ballot_sync(0xffffffffu, par[1] == cur && lane + 32 > cur && tok[1] == want);
+                if (!lo && !hi) break;
+                cur = lo ? __ffs(lo) - 1 : 31 + __ffs(hi);
+            }
+        }
+        if (lane == 0) {
+            s_n = cnt;
+            s_last = cur;
+        }
+    }
+    __syncthreads();
+    const int cnt = s_n;
+    if (layer == 0) {
+        for (int i = threadIdx.x; i < a.max_nodes; i += blockDim.x)
+            a.path[(size_t)s * a.max_nodes + i] = i < cnt ? t0 + s_path[i] : -1;
+        if (threadIdx.x == 0) {
+            a.len_out[s] = L + cnt;
+            a.naccept[s] = cnt;
+            a.bonus[s] = n > 0 ? a.next[t0 + s_last] : -1;
+        }
+    }
+    const int chunks = a.v.kvd / 8;  // of a row
+    for (int c = threadIdx.x; c < 2 * chunks; c += blockDim.x) {
+        uint16_t *base = a.v.kv + (c >= chunks ? (long long)kPageRows * a.v.kvd + (c - chunks) * 8 : (long long)c * 8);
+        for (int j = 0; j < cnt; j++) {
+            const int i = s_path[j];
+            if (i == j) continue;
+            const int sp = a.v.page(s, L + i), dp = a.v.page(s, L + j);
+            if (dp < 0) continue;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (sp >= 0) x = *(const uint4 *)(base + a.v.row(layer, sp, L + i));
+            *(uint4 *)(base + a.v.row(layer, dp, L + j)) = x;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- accumulated weights
+
+struct WeightArgs {
+    KvView v;
+    int heads, G, max_q;
+    const int *len, *nq, *sel;
+    const void *q;
+    long long q_ld, q_layer;
+    const float *lse;
+    long long lse_layer;
+    float scale;
+    float *acc;
+    int acc_rows;
+};
+
+constexpr int kWRows = 128;
+
+// grid (row blocks, slots * kv heads, layers): a thread per cached row, the
+// queries one after the other.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kWRows) cache_weights_plain(const __grid_constant__ WeightArgs a) {
+    __shared__ float sq[HD];
+    const int s = blockIdx.y / a.v.kvh, kvh = blockIdx.y % a.v.kvh, layer = blockIdx.z, r = blockIdx.x * kWRows + threadIdx.x;
+    const int cap = min(a.v.page_max * kPageRows, a.acc_rows);
+    const int L = min(max(a.len[s], 0), cap), n = min(max(a.nq[s], 0), a.max_q), end = min(L + n, cap);
+    if ((int)(blockIdx.x * kWRows) >= end) return;
+    const int pg = r < end ? a.v.page(s, r) : -1;
+    const uint16_t *kr = a.v.kv + a.v.row(layer, max(pg, 0), r) + kvh * HD;
+    float sum = 0.f;
+    for (int j = 0; j < n; j++) {
+        const int t = a.sel[(size_t)s * a.max_q + j];
+        if (t < 0) continue;
+        for (int g = 0; g < a.G; g++) {
+            __syncthreads();
+            for (int d = threadIdx.x; d < HD; d += blockDim.x)
+                sq[d] = ld_elem<T>((const T *)a.q + layer * a.q_layer + t * a.q_ld + (kvh * a.G + g) * HD + d);
+            __syncthreads();
+            if (r < end && r <= L + j) {
+                float x = 0.f;
+                if (pg >= 0)
+                    for (int d = 0; d < HD; d++) x = fmaf(sq[d], bf16_bits_to_f32(kr[d]), x);
+                const float e = a.lse[layer * a.lse_layer + (long long)t * a.heads + kvh * a.G + g];
+                sum += e == -INFINITY ? 0.f : expf(x * a.scale - e);
+            }
+        }
+    }
+    if (r < end) {
+        float *p = a.acc + (((size_t)layer * a.v.slots + s) * a.v.kvh + kvh) * a.acc_rows + r;
+        *p = r < L ? *p + sum : sum;
+    }
+}
+
+// ---------------------------------------------------------------- eviction
+
+struct EvictArgs {
+    KvView v, d;
+    const int *len;
+    const float *acc;
+    int acc_rows, budget, sinks, recent;
+    int *len_out, *kept;
+    float *acc_out;
+};
+
+constexpr int kSelThreads = 512;
+
+// Order-preserving key of an accumulated weight: NaN as -inf, -0 as 0.
+__device__ __forceinline__ uint32_t weight_key(float v) {
+    if (v != v) v = -INFINITY;
+    const uint32_t u = __float_as_uint(v + 0.f);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+// grid (layers * slots * kv heads): the kept rows of one cache column, in
+// order.  A radix select over the candidates' 32-bit keys (8 bits a pass)
+// finds the lightest kept key T and how many rows equal to T stay; one ordered
+// pass then writes the rows that are forced, above T, or among those.
+__global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constant__ EvictArgs a) {
+    __shared__ unsigned hist[256], wsum[2][kSelThreads / 32];
+    __shared__ unsigned s_prefix, s_need;
+    const int idx = blockIdx.x, kvh = idx % a.v.kvh, s = (idx / a.v.kvh) % a.v.slots, layer = idx / (a.v.kvh * a.v.slots);
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n = min(min(max(a.len[s], 0), a.acc_rows), a.v.page_max * kPageRows);
+    const float *acc = a.acc + (size_t)idx * a.acc_rows;
+    int *kept = a.kept + (size_t)idx * a.budget;
+    float *acc_out = a.acc_out + (size_t)idx * a.budget;
+    if (layer == 0 && kvh == 0 && threadIdx.x == 0) a.len_out[s] = min(n, a.budget);
+    for (int j = threadIdx.x + min(n, a.budget); j < a.budget; j += kSelThreads) {
+        kept[j] = -1;
+        acc_out[j] = 0.f;
+    }
+    if (n <= a.budget) {
+        for (int j = threadIdx.x; j < n; j += kSelThreads) {
+            kept[j] = j;
+            acc_out[j] = acc[j];
+        }
+        return;
+    }
+    const int c0 = a.sinks, c1 = n - a.recent, want = a.budget - a.sinks - a.recent;  // want < c1 - c0
+    if (threadIdx.x == 0) {
+        s_prefix = 0;
+        s_need = want;
+    }
+    for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
+        for (int i = threadIdx.x; i < 256; i += kSelThreads) hist[i] = 0;
+        __syncthreads();
+        const unsigned prefix = s_prefix, hmask = shift == 24 ? 0u : ~0u << (shift + 8);
+        for (int r = c0 + threadIdx.x; r < c1; r += kSelThreads) {
+            const uint32_t k = weight_key(acc[r]);
+            if ((k & hmask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
+        }
+        __syncthreads();
+        if (w == 0) {
+            // lane l: bins 255 - 8 l .. 248 - 8 l, counted from the heaviest
+            unsigned c[8], t = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) t += c[i] = hist[255 - 8 * lane - i];
+            unsigned incl = t;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += y;
+            }
+            const unsigned need = s_need;
+            unsigned before = incl - t;
+            if (before < need && need <= incl) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (before < need && need <= before + c[i]) {
+                        s_prefix = prefix | ((unsigned)(255 - 8 * lane - i) << shift);
+                        s_need = need - before;
+                        before = 0xffffffffu;
+                        break;
+                    }
+                    before += c[i];
+                }
+            }
+        }
+        __syncthreads();
+    }
+    __syncthreads();
+    const unsigned T = s_prefix, need = want > 0 ? s_need : 0;
+    unsigned base = 0, ties = 0;  // kept and tied rows so far
+    for (int r0 = 0; r0 < n; r0 += kSelThreads) {
+        const int r = r0 + threadIdx.x;
+        const float v = r < n ? acc[r] : 0.f;
+        const bool cand = r >= c0 && r < c1;
+        const uint32_t k = weight_key(v);
+        const bool sure = r < n && (!cand || (want > 0 && k > T)), tie = cand && want > 0 && k == T;
+        const unsigned bs = __ballot_sync(0xffffffffu, sure), bt = __ballot_sync(0xffffffffu, tie);
+        if (lane == 0) {
+            wsum[0][w] = __popc(bs);
+            wsum[1][w] = __popc(bt);
+        }
+        __syncthreads();
+        unsigned ps = 0, pt = 0, as = 0, at = 0;
+        for (int i = 0; i < kSelThreads / 32; i++) {
+            if (i < w) {
+                ps += wsum[0][i];
+                pt += wsum[1][i];
+            }
+            as += wsum[0][i];
+            at += wsum[1][i];
+        }
+        const unsigned below = (1u << lane) - 1;
+        const unsigned tr = ties + pt + __popc(bt & below);               // this row's rank among the ties
+        const unsigned sr = base + ps + __popc(bs & below) + min(tr, need) - min(ties, need);
+        if (sure || (tie && tr < need)) {
+            kept[sr] = r;
+            acc_out[sr] = v;
+        }
+        base += as + min(ties + at, need) - min(ties, need);
+        ties += at;
+        __syncthreads();
+    }
+}
+
+// grid (layers * slots * kv heads, row blocks): a warp copies K (lanes 0-15)
+// and V (lanes 16-31) of one kept row, 16 bytes a lane (hd 64: 8).
+constexpr int kGatherRows = 64;
+__global__ void __launch_bounds__(256) evict_gather(const __grid_constant__ EvictArgs a) {
+    const int idx = blockIdx.x, kvh = idx % a.v.kvh, s = (idx / a.v.kvh) % a.v.slots, layer = idx / (a.v.kvh * a.v.slots);
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n = min(min(min(max(a.len[s], 0), a.acc_rows), a.v.page_max * kPageRows), a.budget);
+    const int per = a.v.hd / 16;  // elements a lane moves: 8 or 4
+    const long long col = (lane >> 4) * (long long)kPageRows * a.v.kvd + kvh * a.v.hd + (lane & 15) * per;
+    for (int j = blockIdx.y * kGatherRows + w; j < min(n, (int)(blockIdx.y + 1) * kGatherRows); j += 8) {
+        const int r = a.kept[(size_t)idx * a.budget + j];
+        const int sp = a.v.page(s, r), dp = a.d.page(s, j);
+        if (dp < 0) continue;
+        const uint16_t *src = a.v.kv + a.v.row(layer, max(sp, 0), r) + col;
+        uint16_t *dst = a.d.kv + a.d.row(layer, dp, j) + col;
+        if (per == 8) *(uint4 *)dst = sp < 0 ? make_uint4(0, 0, 0, 0) : *(const uint4 *)src;
+        else *(uint2 *)dst = sp < 0 ? make_uint2(0, 0) : *(const uint2 *)src;
+    }
+}
+
+template <typename K, typename A>
+cudaError_t go(K kern, dim3 grid, dim3 block, size_t smem, void *stream, const A &a) {
+    kern<<<grid, block, smem, (cudaStream_t)stream>>>(a);
+    return cudaGetLastError();
+}
+
+int done(cudaError_t e, char *err, int cap) {
+    if (e != cudaSuccess) return op_fail(err, cap, -3, cudaGetErrorString(e));
+    if (err && cap > 0) err[0] = 0;
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+HYC_API size_t hyc_tree_attention_ws(const hyc_kv_view *cache, int heads, int max_nodes) {
+    (void)cache;
+    (void)heads;
+    (void)max_nodes;
+    return 16;
+}
+
+HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer, int heads, int max_nodes,
+                               const int *d_len, const int *d_off, const int *d_parent, const void *d_q,
+                               long long q_ld, int q_bf16, float scale, void *d_out, long long out_ld, float *d_lse,
+                               void *d_ws, size_t ws_bytes, char *err, int err_cap) {
+    TreeArgs a;
+    const char *why;
+    if (!make_view(cache, a.v, &why)) return op_fail(err, err_cap, -1, why);
+    if (!group_ok(heads, a.v.kvh, a.G)) return op_fail(err, err_cap, -1, "heads / kv_heads must be 1, 2, 4 or 8");
+    if (layer < 0 || layer >= a.v.layers) return op_fail(err, err_cap, -1, "no such layer");
+    if (max_nodes < 1 || max_nodes > kTreeMax) return op_fail(err, err_cap, -1, "max_nodes must be 1 .. 64");
+    if (!d_len || !d_off || !d_parent || !d_q || !d_out || !d_ws) return op_fail(err, err_cap, -1, "null argument");
+    const int el = q_bf16 ? 2 : 4;
+    if (!aligned16(d_q) || !aligned16(d_out) || !aligned16(d_ws) || (q_ld * el) % 16 || (out_ld * el) % 16 ||
+        q_ld < (long long)heads * a.v.hd || out_ld < (long long)heads * a.v.hd)
+        return op_fail(err, err_cap, -1, "q, out and the scratch must be 16-byte aligned with rows of heads * hdim or more");
+    if (ws_bytes < hyc_tree_attention_ws(cache, heads, max_nodes)) return op_fail(err, err_cap, -1, "scratch too small");
+    a.layer = layer;
+    a.heads = heads;
+    a.max_nodes = max_nodes;
+    a.len = d_len;
+    a.off = d_off;
+    a.parent = d_parent;
+    a.q = d_q;
+    a.q_ld = q_ld;
+    a.scale = scale;
+    a.out = d_out;
+    a.out_ld = out_ld;
+    a.lse = d_lse;
+    const dim3 grid(a.v.slots, a.v.kvh, max_nodes), block(kTreeWarps * 32);
+    cudaError_t e = cudaErrorInvalidValue;
+#define HY_TREE(HD_, G_)                                                                             \
+    if (a.v.hd == HD_ && a.G == G_)                                                                  \
+        e = q_bf16 ? go(tree_attn_plain<__nv_bfloat16, HD_, G_>, grid, block, 0, stream, a)          \
+                   : go(tree_attn_plain<float, HD_, G_>, grid, block, 0, stream, a);
+    HY_TREE(64, 1) HY_TREE(64, 2) HY_TREE(64, 4) HY_TREE(64, 8)
+    HY_TREE(128, 1) HY_TREE(128, 2) HY_TREE(128, 4) HY_TREE(128, 8)
+#undef HY_TREE
+    return done(e, err, err_cap);
+}
+
+HYC_API int hyc_tree_commit(void *stream, const hyc_kv_view *cache, int max_nodes, const int *d_len,
+                            const int *d_off, const int *d_parent, const int *d_tokens, const int *d_next,
+                            const int *d_forced, int *d_len_out, int *d_naccept, int *d_path, int *d_bonus,
+                            char *err, int err_cap) {
+    CommitArgs a;
+    const char *why;
+    if (!make_view(cache, a.v, &why)) return op_fail(err, err_cap, -1, why);
+    if (max_nodes < 1 || max_nodes > kTreeMax) return op_fail(err, err_cap, -1, "max_nodes must be 1 .. 64");
+    if (!d_len || !d_off || !d_parent || !d_tokens || !d_next || !d_len_out || !d_naccept || !d_path || !d_bonus)
+        return op_fail(err, err_cap, -1, "null argument");
+    if (d_len_out == d_len) return op_fail(err, err_cap, -1, "d_len_out must not be d_len");
+    a.max_nodes = max_nodes;
+    a.len = d_len;
+    a.off = d_off;
+    a.parent = d_parent;
+    a.tokens = d_tokens;
+    a.next = d_next;
+    a.forced = d_forced;
+    a.len_out = d_len_out;
+    a.naccept = d_naccept;
+    a.path = d_path;
+    a.bonus = d_bonus;
+    return done(go(tree_commit, dim3(a.v.layers, a.v.slots), dim3(128), 0, stream, a), err, err_cap);
+}
+
+HYC_API int hyc_cache_weights(void *stream, const hyc_kv_view *cache, int heads, int max_q, const int *d_len,
+                              const int *d_nq, const int *d_sel, const void *d_q, long long q_ld, long long q_layer,
+                              int q_bf16, const float *d_lse, long long lse_layer, float scale, float *d_acc,
+                              int acc_rows, char *err, int err_cap) {
+    WeightArgs a;
+    const char *why;
+    if (!make_view(cache, a.v, &why)) return op_fail(err, err_cap, -1, why);
+    if (!group_ok(heads, a.v.kvh, a.G)) return op_fail(err, err_cap, -1, "heads / kv_heads must be 1, 2, 4 or 8");
+    if (max_q < 1 || max_q > kTreeMax) return op_fail(err, err_cap, -1, "max_q must be 1 .. 64");
+    if (!d_len || !d_nq || !d_sel || !d_q || !d_lse || !d_acc || acc_rows < 1)
+        return op_fail(err, err_cap, -1, "null argument");
+    const int el = q_bf16 ? 2 : 4;
+    if (!aligned16(d_q) || (q_ld * el) % 16 || (q_layer * el) % 16 || q_ld < (long long)heads * a.v.hd)
+        return op_fail(err, err_cap, -1, "q must be 16-byte aligned with rows of heads * hdim or more");
+    a.heads = heads;
+    a.max_q = max_q;
+    a.len = d_len;
+    a.nq = d_nq;
+    a.sel = d_sel;
+    a.q = d_q;
+    a.q_ld = q_ld;
+    a.q_layer = q_layer;
+    a.lse = d_lse;
+    a.lse_layer = lse_layer;
+    a.scale = scale;
+    a.acc = d_acc;
+    a.acc_rows = acc_rows;
+    const int rows = a.v.page_max * kPageRows < acc_rows ? a.v.page_max * kPageRows : acc_rows;
+    if (a.v.slots * (long long)a.v.kvh > 65535 || a.v.layers > 65535) return op_fail(err, err_cap, -1, "cache view too large");
+    const dim3 grid((rows + kWRows - 1) / kWRows, a.v.slots * a.v.kvh, a.v.layers), block(kWRows);
+    cudaError_t e;
+    if (a.v.hd == 64)
+        e = q_bf16 ? go(cache_weights_plain<__nv_bfloat16, 64>, grid, block, 0, stream, a)
+                   : go(cache_weights_plain<float, 64>, grid, block, 0, stream, a);
+    else
+        e = q_bf16 ? go(cache_weights_plain<__nv_bfloat16, 128>, grid, block, 0, stream, a)
+                   : go(cache_weights_plain<float, 128>, grid, block, 0, stream, a);
+    return done(e, err, err_cap);
+}
+
+HYC_API int hyc_cache_evict(void *stream, const hyc_kv_view *cache, const hyc_kv_view *dst, const int *d_len,
+                            const float *d_acc, int acc_rows, int budget, int sinks, int recent, int *d_len_out,
+                            int *d_kept, float *d_acc_out, char *err, int err_cap) {
+    EvictArgs a;
+    const char *why;
+    if (!make_view(cache, a.v, &why) || !make_view(dst, a.d, &why)) return op_fail(err, err_cap, -1, why);
+    if (a.v.layers != a.d.layers || a.v.slots != a.d.slots || a.v.kvh != a.d.kvh || a.v.hd != a.d.hd)
+        return op_fail(err, err_cap, -1, "the two caches must have the same layers, slots and heads");
+    if (!d_len || !d_acc || !d_len_out || !d_kept || !d_acc_out) return op_fail(err, err_cap, -1, "null argument");
+    if (d_len_out == d_len) return op_fail(err, err_cap, -1, "d_len_out must not be d_len");
+    if (budget < 1 || sinks < 0 || recent < 0 || (long long)sinks + recent > budget)
+        return op_fail(err, err_cap, -1, "budget must hold at least sinks + recent rows");
+    if ((long long)a.d.page_max * kPageRows < budget)
+        return op_fail(err, err_cap, -1, "the destination's page table does not hold budget rows");
+    if (acc_rows < 1) return op_fail(err, err_cap, -1, "acc_rows must be positive");
+    a.len = d_len;
+    a.acc = d_acc;
+    a.acc_rows = acc_rows;
+    a.budget = budget;
+    a.sinks = sinks;
+    a.recent = recent;
+    a.len_out = d_len_out;
+    a.kept = d_kept;
+    a.acc_out = d_acc_out;
+    const long long cols = (long long)a.v.layers * a.v.slots * a.v.kvh;
+    if (cols > 0x7fffffff || budget > (1 << 21)) return op_fail(err, err_cap, -1, "cache or budget too large");
+    cudaError_t e = go(evict_select, dim3((unsigned)cols), dim3(kSelThreads), 0, stream, a);
+    if (e == cudaSuccess)
+        e = go(evict_gather, dim3((unsigned)cols, (budget + kGatherRows - 1) / kGatherRows), dim3(256), 0, stream, a);
+    return done(e, err, err_cap);
+}
+
+}  // extern "C"

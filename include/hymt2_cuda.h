@@ -327,6 +327,93 @@ HYC_API int hyc_attention_decode_noalloc(void *stream, int heads, int kv_heads, 
                                          const float *d_q_norm, const float *d_k_norm, const float *d_rope_cos,
                                          const float *d_rope_sin, float *d_ao, char *err, int err_cap);
 
+/* ---- operators on a paged KV cache ------------------------------------ */
+
+/* Speculative decoding over, and a bound on, a paged bf16 cache: attention
+ * of a drafted token tree, acceptance of its path, attention weights
+ * accumulated per cached row, and eviction by them.  No counterpart in the
+ * reference (one token per step, src/model.c:943-954; its cache only grows,
+ * :804-808).  All work is enqueued on `stream` (a cudaStream_t of the current
+ * device); arrays named d_* are device memory, nothing is allocated and
+ * nothing synchronises, so the calls can be captured.  They return 0, -1
+ * (bad argument) or -3 (CUDA error); `err` (optional) receives a message.
+ *
+ * A view of a cache: pages of 16 rows, [layers][npages][K | V][16][kv_heads *
+ * hdim] bf16 from kv (16-byte aligned), row r of a slot being row r % 16 of
+ * page pages[slot][r / 16].  hdim 64 or 128.  A page number outside [0,
+ * npages) reads as rows of zeros and is never written.
+ *
+ * Drafted trees: slot s holds d_len[s] cached rows and drafts the nodes
+ * d_off[s] .. d_off[s + 1] - 1 (d_off[0] = 0, at most max_nodes <= 64 a slot,
+ * none is fine), whose K and V stand in rows d_len[s] + i.  d_parent[t] is
+ * the node's parent within its tree, below the node itself (-1, or any number
+ * that is not below it: none; -2: a padding node, which sees nothing and is
+ * nobody's ancestor).  Rows past a slot's page table do not exist. */
+typedef struct hyc_kv_view {
+    uint16_t *kv;
+    const int *pages; /* device [slots][page_max] */
+    int layers, npages, kv_heads, hdim, slots, page_max;
+} hyc_kv_view;
+
+/* Attention of every node over its slot's cached rows, its ancestors and
+ * itself, in one layer: x_r = scale * q . k_r, out = sum softmax(x)_r v_r,
+ * lse = log sum exp(x_r).  d_q is [tokens][heads][hdim] with q_ld elements
+ * from token to token (a multiple of 16 bytes), fp32 (q_bf16 = 0) or bf16;
+ * d_out likewise with out_ld and the same type; d_lse (optional) is [tokens]
+ * [heads] fp32.  A node that sees no row gets zeros and -inf.  heads /
+ * kv_heads in {1, 2, 4, 8}.  d_ws is scratch of at least
+ * hyc_tree_attention_ws bytes, 16-byte aligned, used by this call alone until
+ * it has run; its contents need no preparation.  K or V of rows that a node
+ * does not see never reach its output, whatever they hold. */
+HYC_API size_t hyc_tree_attention_ws(const hyc_kv_view *cache, int heads, int max_nodes);
+HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer, int heads, int max_nodes,
+                               const int *d_len, const int *d_off, const int *d_parent, const void *d_q,
+                               long long q_ld, int q_bf16, float scale, void *d_out, long long out_ld, float *d_lse,
+                               void *d_ws, size_t ws_bytes, char *err, int err_cap);
+
+/* Greedy acceptance: the path starts at node 0 (the token the sequence ends
+ * with) and goes on to the first child whose token is d_next[t], the token
+ * chosen after node t, until no child matches.  Slots with d_forced[s] != 0
+ * (d_forced may be NULL) take all their nodes in order: a given continuation.
+ * The path's rows move up to rows d_len[s], d_len[s] + 1, ... in every layer
+ * of the view.  Writes d_naccept[s] (0 for a slot without nodes), d_path[s]
+ * [max_nodes] (token numbers, -1 behind the path), d_bonus[s] = d_next of the
+ * path's last node (-1 without nodes) and d_len_out[s] = d_len[s] +
+ * d_naccept[s]; d_len_out must not be d_len. */
+HYC_API int hyc_tree_commit(void *stream, const hyc_kv_view *cache, int max_nodes, const int *d_len,
+                            const int *d_off, const int *d_parent, const int *d_tokens, const int *d_next,
+                            const int *d_forced, int *d_len_out, int *d_naccept, int *d_path, int *d_bonus,
+                            char *err, int err_cap);
+
+/* Accumulated attention weights: for layer l, KV head h and row r of slot s,
+ *   d_acc[l][s][h][r] += sum over the slot's queries j and the head's group
+ *                        of exp(scale * q . k_r - lse),   r <= d_len[s] + j;
+ * rows d_len[s] .. d_len[s] + n - 1, the queries' own, start from zero.
+ * Query j < n = d_nq[s] (at most max_q <= 64) is token d_sel[s * max_q + j]
+ * of d_q, fp32 or bf16, q_ld elements from token to token and q_layer from
+ * layer to layer, and of d_lse [layers][lse_layer elements] as [tokens]
+ * [heads].  A negative d_sel is left out.  d_acc holds acc_rows rows per (l,
+ * s, h), rows from acc_rows on are not accumulated.  The order of the sums
+ * is fixed: the same inputs give the same bits. */
+HYC_API int hyc_cache_weights(void *stream, const hyc_kv_view *cache, int heads, int max_q, const int *d_len,
+                              const int *d_nq, const int *d_sel, const void *d_q, long long q_ld, long long q_layer,
+                              int q_bf16, const float *d_lse, long long lse_layer, float scale, float *d_acc,
+                              int acc_rows, char *err, int err_cap);
+
+/* Eviction: for every layer and KV head of slot s with n = d_len[s] rows,
+ * keeps all rows when n <= budget, else the first `sinks`, the last `recent`
+ * and the heaviest of the others by d_acc [layers][slots][kv_heads][acc_rows]
+ * (ties: the lowest row; NaN counts as -inf), budget in all, and copies them
+ * in order to rows 0, 1, ... of `dst`, another cache of the same layers,
+ * slots and heads with room for budget rows a slot.  d_kept [layers][slots]
+ * [kv_heads][budget] receives the kept rows (-1 behind them), d_acc_out,
+ * shaped alike, their weights (0 behind them), d_len_out[s] = min(n, budget).
+ * Pages of `dst` must not be pages of `cache` that a slot still reads, and no
+ * page may serve two slots of `dst`.  acc_rows must cover every d_len. */
+HYC_API int hyc_cache_evict(void *stream, const hyc_kv_view *cache, const hyc_kv_view *dst, const int *d_len,
+                            const float *d_acc, int acc_rows, int budget, int sinks, int recent, int *d_len_out,
+                            int *d_kept, float *d_acc_out, char *err, int err_cap);
+
 #ifdef __cplusplus
 }
 #endif
