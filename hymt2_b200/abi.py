@@ -123,6 +123,7 @@ SIGNATURES = {
     "hyc_trace": (I, [P, I]),
     "hyc_trace_read": (I, [P, P, I]),
     "hyc_attention_decode_noalloc": (I, [P, I, I, I, I, P, F, P, P, P, P, P, P, P, P, C.c_char_p, I]),
+    "hyc_kvops_timeouts": (I, []),
     "hyc_tree_attention_ws": (Z, [KV, I, I]),
     "hyc_tree_attention": (I, [P, KV, I, I, I, P, P, P, P, LL, I, F, P, LL, P, P, Z, C.c_char_p, I]),
     "hyc_tree_commit": (I, [P, KV, I, P, P, P, P, P, P, P, P, P, P, C.c_char_p, I]),

@@ -6,38 +6,20 @@
 // (src/model.c:943-954) over a cache that only grows (:804-808).  The cache
 // is the batch engine's, [layer][page][K | V][16][kvdim]; row r of a slot is
 // row r % 16 of page pages[slot][r / 16].
+#undef HYK_TRACE  // the measurement build's timelines belong to the decode kernels
+#include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <mutex>
 
 #include "../../include/hymt2_cuda.h"
-#include "hy_common.cuh"
-#include "hy_pages.h"
-
-using namespace hyk;
+#include "hy_kvtree.cuh"
+#include "hy_kvview.cuh"
 
 namespace {
-
-constexpr int kTreeMax = 64;  // nodes of one tree
-
-struct KvView {
-    uint16_t *kv;
-    const int *pages;
-    int layers, npages, kvh, hd, slots, page_max, kvd;
-    long long page_stride, layer_stride;  // elements
-
-    // Page of row r of a slot, -1 when there is none.
-    __device__ __forceinline__ int page(int slot, int r) const {
-        if (r < 0 || (r >> kPageShift) >= page_max) return -1;
-        const int p = __ldg(pages + (size_t)slot * page_max + (r >> kPageShift));
-        return p < 0 || p >= npages ? -1 : p;
-    }
-    // Element offset of K row r in page p of a layer (V: + kPageRows * kvd).
-    __device__ __forceinline__ long long row(int layer, int p, int r) const {
-        return layer * layer_stride + (long long)p * page_stride + (long long)(r & (kPageRows - 1)) * kvd;
-    }
-};
 
 int op_fail(char *err, int cap, int code, const char *msg) {
     if (err && cap > 0) snprintf(err, (size_t)cap, "%s", msg);
@@ -54,7 +36,10 @@ bool make_view(const hyc_kv_view *v, KvView &o, const char **why) {
         *why = "empty cache view";
     else if (v->hdim != 64 && v->hdim != 128) *why = "hdim must be 64 or 128";
     else if (!aligned16(v->kv)) *why = "the cache must be 16-byte aligned";
-    else if (v->page_max > (1 << 26) || v->slots > 65535 || v->kv_heads > 65535) *why = "cache view too large";
+    else if (v->page_max > (1 << 26) || v->kv_heads > 65535 || v->layers > 65535) *why = "cache view too large";
+    else if ((long long)v->layers * v->npages * 2 * kPageRows > 0x7fffffffLL ||
+             (long long)v->slots * v->kv_heads * (v->page_max / 4 + 1) > 0x7fffffffLL)
+        *why = "cache view too large";
     if (*why) return false;
     o.kv = v->kv;
     o.pages = v->pages;
@@ -76,136 +61,59 @@ bool group_ok(int heads, int kvh, int &G) {
     return G == 1 || G == 2 || G == 4 || G == 8;
 }
 
-// ---------------------------------------------------------------- tree attention
-
-struct TreeArgs {
-    KvView v;
-    int layer, heads, G, max_nodes;
-    const int *len, *off, *parent;
-    const void *q;
-    long long q_ld;
-    float scale;
-    void *out;
-    long long out_ld;
-    float *lse;
-};
-
 template <typename T>
 __device__ __forceinline__ float ld_elem(const T *p);
 template <>
 __device__ __forceinline__ float ld_elem<float>(const float *p) { return *p; }
 template <>
 __device__ __forceinline__ float ld_elem<__nv_bfloat16>(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void st_elem(float *p, float v) { *p = v; }
-__device__ __forceinline__ void st_elem(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
 
-// Slot s's cached rows and nodes, bounded by its page table and max_nodes.
-__device__ __forceinline__ void tree_span(const KvView &v, const int *len, const int *off, int max_nodes, int s, int &L,
-                                          int &t0, int &n) {
-    const int cap = v.page_max * kPageRows;
-    L = min(max(__ldg(len + s), 0), cap);
-    t0 = __ldg(off + s);
-    n = min(max(__ldg(off + s + 1) - t0, 0), max_nodes);
+// ---------------------------------------------------------------- tensor maps and kernel attributes
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The whole pool as rows of kvd elements, read in boxes of 64 elements x one
+// page's 16 rows, 128-byte swizzled.
+bool page_map(const KvView &v, CUtensorMap *map) {
+    static EncodeTiled encode = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult st;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &st) == cudaSuccess &&
+            st == cudaDriverEntryPointSuccess)
+            encode = (EncodeTiled)f;
+    });
+    if (!encode) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)v.kvd, (cuuint64_t)v.layers * v.npages * 2 * kPageRows}, strides[1] = {(cuuint64_t)v.kvd * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)kPageRows}, el[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, v.kv, dims, strides, box, el, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr int kTreeWarps = 8;
-
-// grid (slots, kv heads, max_nodes): one node and KV head per CTA, its keys
-// round robin over the warps, a lane owning hd / 32 dims of every head.
-template <typename T, int HD, int G>
-__global__ void __launch_bounds__(kTreeWarps * 32) tree_attn_plain(const __grid_constant__ TreeArgs a) {
-    constexpr int D = HD / 32;
-    __shared__ float s_m[kTreeWarps][G], s_l[kTreeWarps][G], s_o[kTreeWarps][G][HD];
-    __shared__ unsigned long long s_mask;
-    const int s = blockIdx.x, kvh = blockIdx.y, node = blockIdx.z, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int L, t0, n;
-    tree_span(a.v, a.len, a.off, a.max_nodes, s, L, t0, n);
-    if (node >= n) return;
-    const int t = t0 + node;
-    if (threadIdx.x == 0) {  // the node and its ancestors
-        unsigned long long m = 0;
-        int p = a.parent[t], i = node;
-        if (p != -2) {
-            m = 1ull << node;
-            while (p >= 0 && p < i) {
-                i = p;
-                p = a.parent[t0 + i];
-                if (p == -2) break;
-                m |= 1ull << i;
-            }
-        }
-        s_mask = m;
-    }
-    __syncthreads();
-    const unsigned long long mask = s_mask;
-    float q[G][D], o[G][D], m[G], l[G];
-    const T *qr = (const T *)a.q + (long long)t * a.q_ld + (long long)kvh * G * HD;
-#pragma unroll
-    for (int h = 0; h < G; h++) {
-        m[h] = -INFINITY;
-        l[h] = 0.f;
-#pragma unroll
-        for (int d = 0; d < D; d++) {
-            q[h][d] = ld_elem<T>(qr + h * HD + lane * D + d);
-            o[h][d] = 0.f;
-        }
-    }
-    const int end = mask ? L + n : 0;
-    for (int r = w; r < end; r += kTreeWarps) {
-        if (r >= L && !((mask >> (r - L)) & 1)) continue;
-        if ((r >> kPageShift) >= a.v.page_max) break;
-        const int pg = a.v.page(s, r);
-        float k[D], v[D];
-#pragma unroll
-        for (int d = 0; d < D; d++) k[d] = v[d] = 0.f;
-        if (pg >= 0) {
-            const uint16_t *kr = a.v.kv + a.v.row(a.layer, pg, r) + kvh * HD + lane * D;
-#pragma unroll
-            for (int d = 0; d < D; d++) {
-                k[d] = bf16_bits_to_f32(kr[d]);
-                v[d] = bf16_bits_to_f32(kr[kPageRows * a.v.kvd + d]);
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < G; h++) {
-            float x = 0.f;
-#pragma unroll
-            for (int d = 0; d < D; d++) x = fmaf(q[h][d], k[d], x);
-            x = warp_sum(x) * a.scale;
-            const float mn = fmaxf(m[h], x);
-            const float c = m[h] == -INFINITY ? 0.f : expf(m[h] - mn), p = mn == -INFINITY ? 0.f : expf(x - mn);
-            m[h] = mn;
-            l[h] = l[h] * c + p;
-#pragma unroll
-            for (int d = 0; d < D; d++) o[h][d] = fmaf(p, v[d], o[h][d] * c);
-        }
-    }
-#pragma unroll
-    for (int h = 0; h < G; h++) {
-        if (lane == 0) {
-            s_m[w][h] = m[h];
-            s_l[w][h] = l[h];
-        }
-#pragma unroll
-        for (int d = 0; d < D; d++) s_o[w][h][lane * D + d] = o[h][d];
-    }
-    __syncthreads();
-    for (int h = w; h < G; h += kTreeWarps) {
-        float M = -INFINITY, S = 0.f, O[D];
-#pragma unroll
-        for (int d = 0; d < D; d++) O[d] = 0.f;
-        for (int x = 0; x < kTreeWarps; x++) M = fmaxf(M, s_m[x][h]);
-        for (int x = 0; x < kTreeWarps; x++) {
-            const float f = s_m[x][h] == -INFINITY ? 0.f : expf(s_m[x][h] - M);
-            S = fmaf(s_l[x][h], f, S);
-#pragma unroll
-            for (int d = 0; d < D; d++) O[d] = fmaf(s_o[x][h][lane * D + d], f, O[d]);
-        }
-        T *dst = (T *)a.out + (long long)t * a.out_ld + (long long)(kvh * G + h) * HD + lane * D;
-#pragma unroll
-        for (int d = 0; d < D; d++) st_elem(dst + d, S > 0.f ? O[d] / S : 0.f);
-        if (a.lse && lane == 0) a.lse[(long long)t * a.heads + kvh * G + h] = S > 0.f ? M + logf(S) : -INFINITY;
-    }
+// SMs of the current device, with the kernels' shared-memory limits raised on
+// its first use; 0 when there is no usable device.
+int device_sms() {
+    constexpr int kMax = 128;
+    static std::mutex mu;
+    static int sms[kMax];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMax) return 0;
+    std::lock_guard<std::mutex> lock(mu);
+    if (sms[dev]) return sms[dev];
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) return 0;
+    const auto raise = [](const void *k, size_t b) {
+        return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)b) == cudaSuccess;
+    };
+    if (!raise((const void *)tree_attn_tc<float, 64>, tt_smem<float, 64>()) ||
+        !raise((const void *)tree_attn_tc<float, 128>, tt_smem<float, 128>()) ||
+        !raise((const void *)tree_attn_tc<__nv_bfloat16, 64>, tt_smem<__nv_bfloat16, 64>()) ||
+        !raise((const void *)tree_attn_tc<__nv_bfloat16, 128>, tt_smem<__nv_bfloat16, 128>()))
+        return 0;
+    return sms[dev] = n;
 }
 
 // ---------------------------------------------------------------- tree commit
@@ -217,14 +125,14 @@ struct CommitArgs {
     int *len_out, *naccept, *path, *bonus;
 };
 
-// grid (layers, slots).  Warp 0 walks the tree (the next node is the lowest
+// grid (slots, layers).  Warp 0 walks the tree (the next node is the lowest
 // one whose parent and token match: two ballots per accepted node); then
 // thread c owns 16 bytes of a K or V row and moves the path's rows in order.
 // Row j of the path comes from row path[j] >= j, so a row is read before
 // anything is written over it.  CTAs of layer 0 write the outcome.
 __global__ void __launch_bounds__(128) tree_commit(const __grid_constant__ CommitArgs a) {
     __shared__ int s_path[kTreeMax], s_n, s_last;
-    const int layer = blockIdx.x, s = blockIdx.y, lane = threadIdx.x & 31;
+    const int s = blockIdx.x, layer = blockIdx.y, lane = threadIdx.x & 31;
     int L, t0, n;
     tree_span(a.v, a.len, a.off, a.max_nodes, s, L, t0, n);
     if (threadIdx.x < 32) {
@@ -478,10 +386,36 @@ __global__ void __launch_bounds__(256) evict_gather(const __grid_constant__ Evic
     }
 }
 
-template <typename K, typename A>
-cudaError_t go(K kern, dim3 grid, dim3 block, size_t smem, void *stream, const A &a) {
-    kern<<<grid, block, smem, (cudaStream_t)stream>>>(a);
-    return cudaGetLastError();
+template <typename... KArgs, typename... Args>
+cudaError_t go(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, void *stream, bool pdl, Args &&...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+// Scratch of one tree attention: the columns' table, then two pieces a range
+// and row block (a range's first and last column may be split).
+struct TreeWs {
+    int ranges, row_blocks;
+    size_t ml, o, bytes;
+};
+TreeWs tree_ws(const KvView &v, int G, int max_nodes, int sms) {
+    TreeWs w;
+    w.row_blocks = (max_nodes * G + 127) / 128;
+    w.ranges = sms / w.row_blocks > 1 ? sms / w.row_blocks : 1;
+    const size_t pieces = (size_t)2 * w.ranges * w.row_blocks;
+    w.ml = ((size_t)v.slots * v.kvh * sizeof(int2) + 255) & ~(size_t)255;
+    w.o = w.ml + pieces * 128 * sizeof(float2);
+    w.bytes = w.o + pieces * 128 * v.hd * sizeof(float);
+    return w;
 }
 
 int done(cudaError_t e, char *err, int cap) {
@@ -494,11 +428,18 @@ int done(cudaError_t e, char *err, int cap) {
 
 extern "C" {
 
+HYC_API int hyc_kvops_timeouts(void) {
+    unsigned n = 0;
+    return cudaMemcpyFromSymbol(&n, g_kv_timeouts, sizeof n) == cudaSuccess ? (int)n : -1;
+}
+
 HYC_API size_t hyc_tree_attention_ws(const hyc_kv_view *cache, int heads, int max_nodes) {
-    (void)cache;
-    (void)heads;
-    (void)max_nodes;
-    return 16;
+    KvView v;
+    const char *why;
+    int G;
+    if (!make_view(cache, v, &why) || !group_ok(heads, v.kvh, G) || max_nodes < 1 || max_nodes > kTreeMax) return 0;
+    const int sms = device_sms();
+    return tree_ws(v, G, max_nodes, sms > 0 ? sms : 148).bytes;
 }
 
 HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer, int heads, int max_nodes,
@@ -516,7 +457,6 @@ HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer
     if (!aligned16(d_q) || !aligned16(d_out) || !aligned16(d_ws) || (q_ld * el) % 16 || (out_ld * el) % 16 ||
         q_ld < (long long)heads * a.v.hd || out_ld < (long long)heads * a.v.hd)
         return op_fail(err, err_cap, -1, "q, out and the scratch must be 16-byte aligned with rows of heads * hdim or more");
-    if (ws_bytes < hyc_tree_attention_ws(cache, heads, max_nodes)) return op_fail(err, err_cap, -1, "scratch too small");
     a.layer = layer;
     a.heads = heads;
     a.max_nodes = max_nodes;
@@ -529,14 +469,30 @@ HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer
     a.out = d_out;
     a.out_ld = out_ld;
     a.lse = d_lse;
-    const dim3 grid(a.v.slots, a.v.kvh, max_nodes), block(kTreeWarps * 32);
+    const int sms = device_sms();
+    if (sms < 1) return op_fail(err, err_cap, -3, "no usable CUDA device");
+    const TreeWs ws = tree_ws(a.v, a.G, max_nodes, sms);
+    if (ws_bytes < ws.bytes) return op_fail(err, err_cap, -1, "scratch too small");
+    a.cols = (int2 *)d_ws;
+    a.part_ml = (float2 *)((char *)d_ws + ws.ml);
+    a.part_o = (float *)((char *)d_ws + ws.o);
+    a.ranges = ws.ranges;
+    a.row_blocks = ws.row_blocks;
+    a.min_tiles = 1;
+    CUtensorMap map;
+    if (!page_map(a.v, &map)) return op_fail(err, err_cap, -3, "cuTensorMapEncodeTiled failed");
+    const dim3 grid(ws.ranges * ws.row_blocks), mgrid(a.v.slots * a.v.kvh, (max_nodes * a.G + kMergeRows - 1) / kMergeRows);
     cudaError_t e = cudaErrorInvalidValue;
-#define HY_TREE(HD_, G_)                                                                             \
-    if (a.v.hd == HD_ && a.G == G_)                                                                  \
-        e = q_bf16 ? go(tree_attn_plain<__nv_bfloat16, HD_, G_>, grid, block, 0, stream, a)          \
-                   : go(tree_attn_plain<float, HD_, G_>, grid, block, 0, stream, a);
-    HY_TREE(64, 1) HY_TREE(64, 2) HY_TREE(64, 4) HY_TREE(64, 8)
-    HY_TREE(128, 1) HY_TREE(128, 2) HY_TREE(128, 4) HY_TREE(128, 8)
+#define HY_TREE(T_, HD_)                                                                                       \
+    {                                                                                                          \
+        e = go(tree_attn_tc<T_, HD_>, grid, dim3(kTtThreads), tt_smem<T_, HD_>(), stream, false, a, map);       \
+        if (e == cudaSuccess) e = go(tree_merge<T_, HD_, kTtK>, mgrid, dim3(256), 0, stream, true, a);          \
+    }
+    if (q_bf16) {
+        if (a.v.hd == 64) HY_TREE(__nv_bfloat16, 64) else HY_TREE(__nv_bfloat16, 128)
+    } else {
+        if (a.v.hd == 64) HY_TREE(float, 64) else HY_TREE(float, 128)
+    }
 #undef HY_TREE
     return done(e, err, err_cap);
 }
@@ -563,7 +519,7 @@ HYC_API int hyc_tree_commit(void *stream, const hyc_kv_view *cache, int max_node
     a.naccept = d_naccept;
     a.path = d_path;
     a.bonus = d_bonus;
-    return done(go(tree_commit, dim3(a.v.layers, a.v.slots), dim3(128), 0, stream, a), err, err_cap);
+    return done(go(tree_commit, dim3(a.v.slots, a.v.layers), dim3(128), 0, stream, false, a), err, err_cap);
 }
 
 HYC_API int hyc_cache_weights(void *stream, const hyc_kv_view *cache, int heads, int max_q, const int *d_len,
@@ -598,11 +554,11 @@ HYC_API int hyc_cache_weights(void *stream, const hyc_kv_view *cache, int heads,
     const dim3 grid((rows + kWRows - 1) / kWRows, a.v.slots * a.v.kvh, a.v.layers), block(kWRows);
     cudaError_t e;
     if (a.v.hd == 64)
-        e = q_bf16 ? go(cache_weights_plain<__nv_bfloat16, 64>, grid, block, 0, stream, a)
-                   : go(cache_weights_plain<float, 64>, grid, block, 0, stream, a);
+        e = q_bf16 ? go(cache_weights_plain<__nv_bfloat16, 64>, grid, block, 0, stream, false, a)
+                   : go(cache_weights_plain<float, 64>, grid, block, 0, stream, false, a);
     else
-        e = q_bf16 ? go(cache_weights_plain<__nv_bfloat16, 128>, grid, block, 0, stream, a)
-                   : go(cache_weights_plain<float, 128>, grid, block, 0, stream, a);
+        e = q_bf16 ? go(cache_weights_plain<__nv_bfloat16, 128>, grid, block, 0, stream, false, a)
+                   : go(cache_weights_plain<float, 128>, grid, block, 0, stream, false, a);
     return done(e, err, err_cap);
 }
 
@@ -632,9 +588,9 @@ HYC_API int hyc_cache_evict(void *stream, const hyc_kv_view *cache, const hyc_kv
     a.acc_out = d_acc_out;
     const long long cols = (long long)a.v.layers * a.v.slots * a.v.kvh;
     if (cols > 0x7fffffff || budget > (1 << 21)) return op_fail(err, err_cap, -1, "cache or budget too large");
-    cudaError_t e = go(evict_select, dim3((unsigned)cols), dim3(kSelThreads), 0, stream, a);
+    cudaError_t e = go(evict_select, dim3((unsigned)cols), dim3(kSelThreads), 0, stream, false, a);
     if (e == cudaSuccess)
-        e = go(evict_gather, dim3((unsigned)cols, (budget + kGatherRows - 1) / kGatherRows), dim3(256), 0, stream, a);
+        e = go(evict_gather, dim3((unsigned)cols, (budget + kGatherRows - 1) / kGatherRows), dim3(256), 0, stream, false, a);
     return done(e, err, err_cap);
 }
 

@@ -343,6 +343,11 @@ HYC_API int hyc_attention_decode_noalloc(void *stream, int heads, int kv_heads, 
  * page pages[slot][r / 16].  hdim 64 or 128.  A page number outside [0,
  * npages) reads as rows of zeros and is never written.
  *
+ * Kernels that wait inside (for copies and tensor-core products) do so for at
+ * most 2 s a wait and then end with wrong outputs; hyc_kvops_timeouts returns
+ * how many waits have given up on the current device since the library was
+ * loaded (0 unless something is broken; it synchronises), -1 on an error.
+ *
  * Drafted trees: slot s holds d_len[s] cached rows and drafts the nodes
  * d_off[s] .. d_off[s + 1] - 1 (d_off[0] = 0, at most max_nodes <= 64 a slot,
  * none is fine), whose K and V stand in rows d_len[s] + i.  d_parent[t] is
@@ -365,6 +370,7 @@ typedef struct hyc_kv_view {
  * hyc_tree_attention_ws bytes, 16-byte aligned, used by this call alone until
  * it has run; its contents need no preparation.  K or V of rows that a node
  * does not see never reach its output, whatever they hold. */
+HYC_API int hyc_kvops_timeouts(void);
 HYC_API size_t hyc_tree_attention_ws(const hyc_kv_view *cache, int heads, int max_nodes);
 HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer, int heads, int max_nodes,
                                const int *d_len, const int *d_off, const int *d_parent, const void *d_q,
