@@ -18,6 +18,7 @@
 #include "../../include/hymt2_cuda.h"
 #include "hy_kvtree.cuh"
 #include "hy_kvview.cuh"
+#include "hy_kvweights.cuh"
 
 namespace {
 
@@ -38,7 +39,7 @@ bool make_view(const hyc_kv_view *v, KvView &o, const char **why) {
     else if (!aligned16(v->kv)) *why = "the cache must be 16-byte aligned";
     else if (v->page_max > (1 << 26) || v->kv_heads > 65535 || v->layers > 65535) *why = "cache view too large";
     else if ((long long)v->layers * v->npages * 2 * kPageRows > 0x7fffffffLL ||
-             (long long)v->slots * v->kv_heads * (v->page_max / 4 + 1) > 0x7fffffffLL)
+             (double)v->layers * v->slots * v->kv_heads * (v->page_max / 8 + 1) > 2147483647.0)
         *why = "cache view too large";
     if (*why) return false;
     o.kv = v->kv;
@@ -60,13 +61,6 @@ bool group_ok(int heads, int kvh, int &G) {
     G = heads / kvh;
     return G == 1 || G == 2 || G == 4 || G == 8;
 }
-
-template <typename T>
-__device__ __forceinline__ float ld_elem(const T *p);
-template <>
-__device__ __forceinline__ float ld_elem<float>(const float *p) { return *p; }
-template <>
-__device__ __forceinline__ float ld_elem<__nv_bfloat16>(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
 
 // ---------------------------------------------------------------- tensor maps and kernel attributes
 
@@ -111,7 +105,11 @@ int device_sms() {
     if (!raise((const void *)tree_attn_tc<float, 64>, tt_smem<float, 64>()) ||
         !raise((const void *)tree_attn_tc<float, 128>, tt_smem<float, 128>()) ||
         !raise((const void *)tree_attn_tc<__nv_bfloat16, 64>, tt_smem<__nv_bfloat16, 64>()) ||
-        !raise((const void *)tree_attn_tc<__nv_bfloat16, 128>, tt_smem<__nv_bfloat16, 128>()))
+        !raise((const void *)tree_attn_tc<__nv_bfloat16, 128>, tt_smem<__nv_bfloat16, 128>()) ||
+        !raise((const void *)cache_weights_tc<float, 64>, kWtSmem + 1024) ||
+        !raise((const void *)cache_weights_tc<float, 128>, kWtSmem + 1024) ||
+        !raise((const void *)cache_weights_tc<__nv_bfloat16, 64>, kWtSmem + 1024) ||
+        !raise((const void *)cache_weights_tc<__nv_bfloat16, 128>, kWtSmem + 1024))
         return 0;
     return sms[dev] = n;
 }
@@ -187,58 +185,6 @@ __global__ void __launch_bounds__(128) tree_commit(const __grid_constant__ Commi
             if (sp >= 0) x = *(const uint4 *)(base + a.v.row(layer, sp, L + i));
             *(uint4 *)(base + a.v.row(layer, dp, L + j)) = x;
         }
-    }
-}
-
-// ---------------------------------------------------------------- accumulated weights
-
-struct WeightArgs {
-    KvView v;
-    int heads, G, max_q;
-    const int *len, *nq, *sel;
-    const void *q;
-    long long q_ld, q_layer;
-    const float *lse;
-    long long lse_layer;
-    float scale;
-    float *acc;
-    int acc_rows;
-};
-
-constexpr int kWRows = 128;
-
-// grid (row blocks, slots * kv heads, layers): a thread per cached row, the
-// queries one after the other.
-template <typename T, int HD>
-__global__ void __launch_bounds__(kWRows) cache_weights_plain(const __grid_constant__ WeightArgs a) {
-    __shared__ float sq[HD];
-    const int s = blockIdx.y / a.v.kvh, kvh = blockIdx.y % a.v.kvh, layer = blockIdx.z, r = blockIdx.x * kWRows + threadIdx.x;
-    const int cap = min(a.v.page_max * kPageRows, a.acc_rows);
-    const int L = min(max(a.len[s], 0), cap), n = min(max(a.nq[s], 0), a.max_q), end = min(L + n, cap);
-    if ((int)(blockIdx.x * kWRows) >= end) return;
-    const int pg = r < end ? a.v.page(s, r) : -1;
-    const uint16_t *kr = a.v.kv + a.v.row(layer, max(pg, 0), r) + kvh * HD;
-    float sum = 0.f;
-    for (int j = 0; j < n; j++) {
-        const int t = a.sel[(size_t)s * a.max_q + j];
-        if (t < 0) continue;
-        for (int g = 0; g < a.G; g++) {
-            __syncthreads();
-            for (int d = threadIdx.x; d < HD; d += blockDim.x)
-                sq[d] = ld_elem<T>((const T *)a.q + layer * a.q_layer + t * a.q_ld + (kvh * a.G + g) * HD + d);
-            __syncthreads();
-            if (r < end && r <= L + j) {
-                float x = 0.f;
-                if (pg >= 0)
-                    for (int d = 0; d < HD; d++) x = fmaf(sq[d], bf16_bits_to_f32(kr[d]), x);
-                const float e = a.lse[layer * a.lse_layer + (long long)t * a.heads + kvh * a.G + g];
-                sum += e == -INFINITY ? 0.f : expf(x * a.scale - e);
-            }
-        }
-    }
-    if (r < end) {
-        float *p = a.acc + (((size_t)layer * a.v.slots + s) * a.v.kvh + kvh) * a.acc_rows + r;
-        *p = r < L ? *p + sum : sum;
     }
 }
 
@@ -549,16 +495,25 @@ HYC_API int hyc_cache_weights(void *stream, const hyc_kv_view *cache, int heads,
     a.scale = scale;
     a.acc = d_acc;
     a.acc_rows = acc_rows;
-    const int rows = a.v.page_max * kPageRows < acc_rows ? a.v.page_max * kPageRows : acc_rows;
-    if (a.v.slots * (long long)a.v.kvh > 65535 || a.v.layers > 65535) return op_fail(err, err_cap, -1, "cache view too large");
-    const dim3 grid((rows + kWRows - 1) / kWRows, a.v.slots * a.v.kvh, a.v.layers), block(kWRows);
+    const int sms = device_sms();
+    if (sms < 1) return op_fail(err, err_cap, -3, "no usable CUDA device");
+    CUtensorMap map;
+    if (!page_map(a.v, &map)) return op_fail(err, err_cap, -3, "cuTensorMapEncodeTiled failed");
+    // a second Q buffer where it leaves K four stages or more
+    a.block = max_q * a.G < 128 ? (max_q * a.G + 15) & ~15 : 128;
+    const int qbytes = (q_bf16 ? 1 : 3) * a.block * a.v.hd * 2, stage = 128 * a.v.hd * 2;
+    a.qbufs = (kWtSmem - 2 * qbytes) / stage >= 4 ? 2 : 1;
+    a.stages = (kWtSmem - a.qbufs * qbytes) / stage;
+    if (a.stages > 8) a.stages = 8;
+    const size_t smem = (size_t)a.qbufs * qbytes + (size_t)a.stages * stage + 1024;
+    const dim3 grid(sms), block(kWtThreads);
     cudaError_t e;
     if (a.v.hd == 64)
-        e = q_bf16 ? go(cache_weights_plain<__nv_bfloat16, 64>, grid, block, 0, stream, false, a)
-                   : go(cache_weights_plain<float, 64>, grid, block, 0, stream, false, a);
+        e = q_bf16 ? go(cache_weights_tc<__nv_bfloat16, 64>, grid, block, smem, stream, false, a, map)
+                   : go(cache_weights_tc<float, 64>, grid, block, smem, stream, false, a, map);
     else
-        e = q_bf16 ? go(cache_weights_plain<__nv_bfloat16, 128>, grid, block, 0, stream, false, a)
-                   : go(cache_weights_plain<float, 128>, grid, block, 0, stream, false, a);
+        e = q_bf16 ? go(cache_weights_tc<__nv_bfloat16, 128>, grid, block, smem, stream, false, a, map)
+                   : go(cache_weights_tc<float, 128>, grid, block, smem, stream, false, a, map);
     return done(e, err, err_cap);
 }
 
