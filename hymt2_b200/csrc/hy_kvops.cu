@@ -495,6 +495,7 @@ HYC_API int hyc_cache_weights(void *stream, const hyc_kv_view *cache, int heads,
     a.scale = scale;
     a.acc = d_acc;
     a.acc_rows = acc_rows;
+    a.lg = a.G == 1 ? 0 : a.G == 2 ? 1 : a.G == 4 ? 2 : 3;
     const int sms = device_sms();
     if (sms < 1) return op_fail(err, err_cap, -3, "no usable CUDA device");
     CUtensorMap map;

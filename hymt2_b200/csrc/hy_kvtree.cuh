@@ -209,7 +209,7 @@ __device__ __noinline__ void tree_add_bad(const TreeArgs &a, int slot, int kvh, 
 //   warp 4     streams K and V pages by TMA into a ring of stages, 128-byte
 //              swizzled: K rows are the K-major B operand of Q . K^T, V rows
 //              the MN-major B operand of P . V, so nothing is transposed
-//   warp 5     one thread issues S = Q . K^T (two S tiles, so that the next
+//   warp 5     issues S = Q . K^T (two S tiles, so that the next
 //              one runs while this one's softmax does) and O += P . V
 //   warps 0-3  one row a thread: S from tensor memory, running maximum and
 //              sum, P back over S as the A operand in tensor memory
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
     __shared__ int s_stop;
     uint8_t *sq = (uint8_t *)(((uintptr_t)dsm + 1023) & ~(uintptr_t)1023);
     uint8_t *ring = sq + tt_qbytes<T, HD>();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rb = blockIdx.x % a.row_blocks, range = blockIdx.x / a.row_blocks;
     const int NB = 128 / a.G, node0 = rb * NB;  // nodes of a row block
     pdl_trigger();
@@ -283,12 +283,12 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
     pdl_wait();
     tree_plan<kTtK>(a, range, s_scan, s_start);
     um_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     TreeWalk<kTtK> w = tree_walk<kTtK>(s_start, range);
     const int cap = a.v.page_max * kPageRows;
     if (warp == 4) {
-        // lane j of 0 .. 7 copies page j of a tile, K then V; a page that does
-        // not exist is read past the end of the map, which fills zeros
+        // eight pages a tile, K then V; a page that does not exist is read past
+        // the end of the map, which fills zeros
         const int y0 = a.layer * a.v.npages * 2 * kPageRows, yend = a.v.layers * a.v.npages * 2 * kPageRows;
         int pos = 0;
         while (w.next(a, node0)) {
@@ -301,25 +301,30 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                     const int st = pos % NST, use = pos / NST;
                     if (use > 0) mb_wait(&empty[st], (use - 1) & 1, &s_stop);
                     if (__any_sync(0xffffffffu, *(volatile int *)&s_stop)) break;
-                    if (lane == 0) mb_expect(&full[st], STB);
-                    __syncwarp();
-                    if (lane < 8) {
+                    int yj[8];
 #pragma unroll
-                        for (int h = 0; h < NH; h++)
-                            tma_box(ring + (size_t)st * STB + h * 16384 + lane * 2048, &map, w.s_kvh * HD + h * 64,
-                                    y == yend ? yend : y + kv * kPageRows, &full[st]);
+                    for (int i = 0; i < 8; i++) yj[i] = __shfl_sync(0xffffffffu, y == yend ? yend : y + kv * kPageRows, i);
+                    if (elect()) {
+                        mb_expect(&full[st], STB);
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+#pragma unroll
+                            for (int h = 0; h < NH; h++)
+                                tma_box(ring + (size_t)st * STB + h * 16384 + i * 2048, &map, w.s_kvh * HD + h * 64, yj[i], &full[st]);
                     }
+                    __syncwarp();
                 }
             }
         }
         // copies in flight land before the kernel ends, also after a wait gave up
         for (int p = max(0, pos - NST); p < pos; p++) {
-            int none = 0;
+            int none = 0;  // never set: the wait itself is bounded
             mb_wait(&full[p % NST], (p / NST) & 1, &none);
         }
     } else if (warp == 5) {
-        if (lane == 0) {
+        {
             constexpr uint32_t iqk = um_idesc(128, kTtK, false), ipv = um_idesc(128, HD, true);
+            const uint32_t ring0 = __shfl_sync(0xffffffffu, kv_smem(ring), 0), q0 = um_desc_lo(__shfl_sync(0xffffffffu, kv_smem(sq), 0), 16);
             int it = 0, seg = 0;  // tiles and segments done
             // O += P(i) . V(i); the segment's first one overwrites O
             auto pv = [&](int i, bool first) {
@@ -328,15 +333,18 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                 mb_wait(&full[st], (pos / NST) & 1, &s_stop);
                 if (first && seg > 0) mb_wait(&ofree, (seg - 1) & 1, &s_stop);
                 um_fence_after();
-                const uint32_t vb = kv_smem(ring + (size_t)st * STB), p0 = tmem + kTtS + (i & 1) * 128, px = tmem + kTtX + (i & 1) * 64;
+                const uint32_t vb = um_desc_lo(ring0 + st * STB, 16384), p0 = tmem + kTtS + (i & 1) * 128, px = tmem + kTtX + (i & 1) * 64;
+                if (elect()) {
 #pragma unroll
-                for (int x = PT - 1; x >= 0; x--)  // small terms first
+                    for (int x = PT - 1; x >= 0; x--)  // small terms first
 #pragma unroll
-                    for (int k = 0; k < kTtK / 16; k++)
-                        um_mma_ts(tmem + kTtO, (x == 2 ? px : p0 + x * 64) + k * 8, um_desc(vb + k * 2048, 16384), ipv,
-                                  !(first && x == PT - 1 && k == 0));
-                um_commit(&empty[st]);
-                um_commit(&odone[i & 1]);
+                        for (int k = 0; k < kTtK / 16; k++)
+                            um_mma_ts(tmem + kTtO, (x == 2 ? px : p0 + x * 64) + k * 8, vb + k * (2048 / 16), ipv,
+                                      x == PT - 1 && k == 0 ? !first : true);
+                    um_commit(&empty[st]);
+                    um_commit(&odone[i & 1]);
+                }
+                __syncwarp();
             };
             while (w.next(a, node0)) {
                 for (int t = w.s_a; t < w.s_b; t++, it++) {
@@ -344,21 +352,26 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                     if (t == w.s_a) mb_wait(&qfull, seg & 1, &s_stop);
                     mb_wait(&full[st], (pos / NST) & 1, &s_stop);
                     um_fence_after();
-                    const uint32_t kb = kv_smem(ring + (size_t)st * STB), qb = kv_smem(sq);
+                    const uint32_t kb = um_desc_lo(ring0 + st * STB, 16), s0 = tmem + kTtS + (it & 1) * 128;
+                    if (elect()) {
 #pragma unroll
-                    for (int x = QT - 1; x >= 0; x--)
+                        for (int x = QT - 1; x >= 0; x--)
 #pragma unroll
-                        for (int k = 0; k < HD / 16; k++)
-                            um_mma(tmem + kTtS + (it & 1) * 128, um_desc(qb + x * STB + (k >> 2) * 16384 + (k & 3) * 32, 16),
-                                   um_desc(kb + (k >> 2) * 16384 + (k & 3) * 32, 16), iqk, !(x == QT - 1 && k == 0));
-                    um_commit(&empty[st]);
-                    um_commit(&sfull[it & 1]);
+                            for (int k = 0; k < HD / 16; k++) {
+                                const uint32_t at = ((k >> 2) * 16384 + (k & 3) * 32) / 16;
+                                um_mma(s0, q0 + x * (STB / 16) + at, kb + at, iqk, !(x == QT - 1 && k == 0));
+                            }
+                        um_commit(&empty[st]);
+                        um_commit(&sfull[it & 1]);
+                    }
+                    __syncwarp();
                     if (t > w.s_a) pv(it - 1, t - 1 == w.s_a);
                 }
                 pv(it - 1, w.s_b - 1 == w.s_a);
                 seg++;
             }
-            um_commit(&fin);
+            if (elect()) um_commit(&fin);
+            __syncwarp();
             int none = 0;
             mb_wait(&fin, 0, &none);
         }

@@ -108,23 +108,34 @@ __device__ __forceinline__ void um_commit(uint64_t *b) {
 __host__ __device__ constexpr uint32_t um_idesc(int M, int N, bool b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-// Shared-memory operand in 128-byte-swizzled rows of 64 bf16, 8-row groups
-// 1024 bytes apart; `lbo` (MN-major only): bytes between 64-element columns.
-__device__ __forceinline__ uint64_t um_desc(uint32_t addr, uint32_t lbo) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
-           (2ull << 61);
+// One thread of a converged warp.  The loops that feed the tensor cores and
+// the TMA unit run in whole warps with uniform values, and only the
+// instructions themselves are this thread's: descriptors then stay in uniform
+// registers (a loop of one lane took 70-110 ns a product, more than the
+// product itself).
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+    return p != 0;
 }
-__device__ __forceinline__ void um_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+// Shared-memory operand in 128-byte-swizzled rows of 64 bf16, 8-row groups
+// 1024 bytes apart: the low word (address, and `lbo`, for MN-major operands
+// the bytes between 64-element columns); a step of n bytes adds n / 16 to it.
+__device__ __forceinline__ uint32_t um_desc_lo(uint32_t addr, uint32_t lbo) { return ((addr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16); }
+constexpr uint32_t kUmDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void um_mma(uint32_t d, uint32_t alo, uint32_t blo, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((int)acc)
+        "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %4, 0;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(d),
+        "r"(alo), "r"(blo), "r"(idesc), "r"((int)acc), "r"(kUmDescHi)
         : "memory");
 }
 // A from TMEM (bf16 pairs, one row a lane).
-__device__ __forceinline__ void um_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void um_mma_ts(uint32_t d, uint32_t a, uint32_t blo, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((int)acc)
+        "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %4, 0;\n mov.b64 b, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(blo), "r"(idesc), "r"((int)acc), "r"(kUmDescHi)
         : "memory");
 }
 // 32 lanes x 32 columns of 32-bit words from / 16 columns to this warp's lane quarter.

@@ -20,6 +20,7 @@ struct WeightArgs {
     float scale;
     float *acc;
     int acc_rows;
+    int lg;                    // log2 G
     int block, qbufs, stages;  // query rows of a block (a multiple of 16, <= 128), Q buffers, K stages
 };
 
@@ -68,12 +69,15 @@ struct WeightWalk {
 // tile, the (query, head) pairs its columns, so a thread sums its row's
 // probabilities by itself.  K comes by TMA straight into the K-major operand
 // (128-byte swizzled); fp32 queries enter as three bf16 terms.
-//   warps 0-3  one cached row a thread: exponentials and sums, acc
-//   warp 4     K pages by TMA;  warp 5  MMAs into four S^T tiles
-//   warps 6-9  the next column's queries, log-sum-exps and row bounds
+//   warps 0-15   four groups, one for each of four S^T tiles: a cached row a
+//                thread, exponentials and sums, acc (a group alone would wait
+//                for acc's load in every tile: 47 -> 2X us at 32 x 4096 rows)
+//   warp 16      K pages by TMA;  warp 17  MMAs
+//   warps 18-21  the next column's queries, log-sum-exps and row bounds
 // More than 128 (query, head) rows go in blocks of 128 over the same rows,
-// whose thread adds one block after the other.
-constexpr int kWtThreads = 320;
+// whose thread adds one block after the other: a tile's group goes by the tile's
+// place in the column, the same for every block.
+constexpr int kWtThreads = 22 * 32;
 constexpr int kWtSmem = 222 * 1024;  // of 227 KB: Q buffers and K stages
 template <typename T>
 __host__ __device__ constexpr int wt_terms() { return sizeof(T) == 4 ? 3 : 1; }
@@ -81,13 +85,14 @@ __host__ __device__ constexpr int wt_terms() { return sizeof(T) == 4 ? 3 : 1; }
 template <typename T, int HD>
 __global__ void __launch_bounds__(kWtThreads, 1) cache_weights_tc(const __grid_constant__ WeightArgs a,
                                                                   const __grid_constant__ CUtensorMap map) {
-    constexpr int QT = wt_terms<T>(), NH = HD / 64, STB = NH * 16384, kMaxSt = 8, NS = 4;
+    constexpr int QT = wt_terms<T>(), NH = HD / 64, STB = NH * 16384, kMaxSt = 8, NS = 4;  // NS: S^T tiles and row groups
     extern __shared__ uint8_t dsm[];
     __shared__ __align__(8) uint64_t full[kMaxSt], empty[kMaxSt], sfull[NS], sempty[NS], qfull[2], qempty[2], fin;
     __shared__ uint32_t s_tmem;
     __shared__ int s_scan[kWtThreads / 32], s_start[4], s_stop;
+    __shared__ int s_tok[128];
     __shared__ __align__(16) float2 s_col[2][128];  // of each query row: lse * log2 e, last row it sees
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, NB = a.block, NST = a.stages;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, NB = a.block, NST = a.stages;
     const int half_b = NB * 128, term_b = NH * half_b, qbuf_b = QT * term_b;
     uint8_t *sq = (uint8_t *)(((uintptr_t)dsm + 1023) & ~(uintptr_t)1023);
     uint8_t *ring = sq + a.qbufs * qbuf_b;
@@ -102,13 +107,13 @@ __global__ void __launch_bounds__(kWtThreads, 1) cache_weights_tc(const __grid_c
         }
         for (int i = 0; i < 2; i++) {
             mb_init(&qfull[i], 128);
-            mb_init(&qempty[i], 129);
+            mb_init(&qempty[i], 128 * NS + 1);
         }
         mb_init(&fin, 1);
         s_stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 5) {
+    if (warp == 17) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(kv_smem(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         um_fence_before();
@@ -159,14 +164,14 @@ __global__ void __launch_bounds__(kWtThreads, 1) cache_weights_tc(const __grid_c
         __syncthreads();
     }
     um_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     WeightWalk w;
     w.left = s_start[3];
     w.layer = w.left > 0 ? s_start[0] : 0;
     w.slot = w.left > 0 ? s_start[1] : 0;
     w.rem = w.left > 0 ? s_start[2] : 0;
     w.at = -1;
-    if (warp == 4) {
+    if (warp == 16) {
         const int yend = a.v.layers * a.v.npages * 2 * kPageRows;
         int pos = 0;
         while (w.next(a)) {
@@ -181,107 +186,134 @@ __global__ void __launch_bounds__(kWtThreads, 1) cache_weights_tc(const __grid_c
                         pos--;
                         continue;
                     }
-                    if (lane == 0) mb_expect(&full[st], STB);
-                    __syncwarp();
-                    if (lane < 8) {
+                    int yj[8];
 #pragma unroll
-                        for (int h = 0; h < NH; h++)
-                            tma_box(ring + (size_t)st * STB + h * 16384 + lane * 2048, &map, w.s_kvh * HD + h * 64, y, &full[st]);
+                    for (int i = 0; i < 8; i++) yj[i] = __shfl_sync(0xffffffffu, y, i);
+                    if (elect()) {
+                        mb_expect(&full[st], STB);
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+#pragma unroll
+                            for (int h = 0; h < NH; h++)
+                                tma_box(ring + (size_t)st * STB + h * 16384 + i * 2048, &map, w.s_kvh * HD + h * 64, yj[i], &full[st]);
                     }
+                    __syncwarp();
                 }
         }
         for (int p = max(0, pos - NST); p < pos; p++) {  // copies in flight land before the kernel ends
             int none = 0;
             mb_wait(&full[p % NST], (p / NST) & 1, &none);
         }
-    } else if (warp == 5) {
-        if (lane == 0) {
-            int it = 0, qi = 0;
-            while (w.next(a))
+    } else if (warp == 17) {
+        {
+            const uint32_t ring0 = __shfl_sync(0xffffffffu, kv_smem(ring), 0), sq0 = __shfl_sync(0xffffffffu, kv_smem(sq), 0);
+            int it = 0, qi = 0, turn = 0, used = 0;  // used: parity of each S^T tile's uses
+            while (w.next(a)) {
                 for (int q0 = 0; q0 < w.n * a.G; q0 += NB, qi++) {
                     const int qb = qi % a.qbufs, N = (min(NB, w.n * a.G - q0) + 15) & ~15;
-                    const uint32_t id = um_idesc(128, N, false), qa = kv_smem(sq + qb * qbuf_b);
+                    const uint32_t id = um_idesc(128, N, false), qa = um_desc_lo(sq0 + qb * qbuf_b, 16);
                     mb_wait(&qfull[qb], (qi / a.qbufs) & 1, &s_stop);
                     for (int t = w.s_a; t < w.s_b; t++, it++) {
-                        const int st = it % NST, b = it % NS;
+                        const int st = it % NST, b = (t - w.s_a + turn) % NS;
                         mb_wait(&full[st], (it / NST) & 1, &s_stop);
-                        if (it >= NS) mb_wait(&sempty[b], (it / NS - 1) & 1, &s_stop);
+                        mb_wait(&sempty[b], ((used >> b) & 1) ^ 1, &s_stop);  // passes on the first use
+                        used ^= 1 << b;
                         um_fence_after();
-                        const uint32_t kb = kv_smem(ring + (size_t)st * STB);
+                        const uint32_t kb = um_desc_lo(ring0 + st * STB, 16), s0 = tmem + b * 128;
+                        if (elect()) {
 #pragma unroll
-                        for (int x = QT - 1; x >= 0; x--)  // small terms first
+                            for (int x = QT - 1; x >= 0; x--)  // small terms first
 #pragma unroll
-                            for (int k = 0; k < HD / 16; k++)
-                                um_mma(tmem + b * 128, um_desc(kb + (k >> 2) * 16384 + (k & 3) * 32, 16),
-                                       um_desc(qa + x * term_b + (k >> 2) * half_b + (k & 3) * 32, 16), id, !(x == QT - 1 && k == 0));
-                        um_commit(&empty[st]);
-                        um_commit(&sfull[b]);
+                                for (int k = 0; k < HD / 16; k++)
+                                    um_mma(s0, kb + ((k >> 2) * 16384 + (k & 3) * 32) / 16,
+                                           qa + (x * term_b + (k >> 2) * half_b + (k & 3) * 32) / 16, id, !(x == QT - 1 && k == 0));
+                            um_commit(&empty[st]);
+                            um_commit(&sfull[b]);
+                        }
+                        __syncwarp();
                     }
-                    um_commit(&qempty[qb]);
+                    if (elect()) um_commit(&qempty[qb]);
+                    __syncwarp();
                 }
-            um_commit(&fin);
+                turn++;
+            }
+            if (elect()) um_commit(&fin);
+            __syncwarp();
             int none = 0;
             mb_wait(&fin, 0, &none);
         }
-    } else if (warp >= 6) {
-        const int wl = warp - 6;
+    } else if (warp >= 18) {
+        const int wl = warp - 18;
         int qi = 0;
         while (w.next(a))
             for (int q0 = 0; q0 < w.n * a.G; q0 += NB, qi++) {
                 const int qb = qi % a.qbufs, use = qi / a.qbufs, rows = min(NB, w.n * a.G - q0), N = (rows + 15) & ~15;
                 if (use > 0) mb_wait(&qempty[qb], (use - 1) & 1, &s_stop);
+                const int th = threadIdx.x - 18 * 32;  // a row's token, log-sum-exp and bound
+                if (th < N) {
+                    const int j = (q0 + th) >> a.lg, head = w.s_kvh * a.G + ((q0 + th) & (a.G - 1));
+                    const int t = th < rows ? __ldg(a.sel + (size_t)w.s_slot * a.max_q + j) : -1;
+                    // a query that is left out, or saw nothing (-inf), sees no row
+                    const float e = t >= 0 ? a.lse[w.s_layer * a.lse_layer + (long long)t * a.heads + head] : -INFINITY;
+                    s_col[qb][th] = make_float2(e * 1.4426950408889634f, __int_as_float(e == -INFINITY ? -1 : w.L + j));
+                    s_tok[th] = t;
+                }
+                bar_sync(1, 128);
                 uint8_t *dst0 = sq + qb * qbuf_b;
                 const int half = HD == 128 ? lane >> 4 : 0, c = (lane & 15) * 4;
-#pragma unroll 4
-                for (int r = wl; r < N; r += 4) {
-                    const int j = (q0 + r) / a.G, head = w.s_kvh * a.G + (q0 + r) % a.G;
-                    const int t = r < rows ? __ldg(a.sel + (size_t)w.s_slot * a.max_q + j) : -1;
-                    float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (t >= 0 && (HD == 128 || lane < 16)) {
-                        const T *src = (const T *)a.q + w.s_layer * a.q_layer + t * a.q_ld + (long long)head * HD + half * 64 + c;
-                        if constexpr (sizeof(T) == 4) {
-                            q = *(const float4 *)src;
-                        } else {
-                            const uint2 u = *(const uint2 *)src;
-                            q = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u),
-                                            __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+                const T *src0 = (const T *)a.q + w.s_layer * a.q_layer + (long long)w.s_kvh * a.G * HD + half * 64 + c;
+                for (int r0 = wl; r0 < N; r0 += 16) {  // a warp to a row, four rows in flight
+                    float4 q[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int r = r0 + 4 * i, t = r < N ? s_tok[r] : -1;
+                        q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (t >= 0 && (HD == 128 || lane < 16)) {
+                            const T *src = src0 + t * a.q_ld + ((q0 + r) & (a.G - 1)) * HD;
+                            if constexpr (sizeof(T) == 4) {
+                                q[i] = *(const float4 *)src;
+                            } else {
+                                const uint2 u = *(const uint2 *)src;
+                                q[i] = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u),
+                                                   __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+                            }
                         }
                     }
-                    if (HD == 128 || lane < 16) {
-                        uint32_t lo[QT], hi[QT];
-                        split_bf16<QT>(q.x, q.y, lo);
-                        split_bf16<QT>(q.z, q.w, hi);
-                        uint8_t *dst = dst0 + half * half_b + r * 128 + ((((c >> 3) ^ (r & 7)) << 4) | ((c & 4) << 1));
 #pragma unroll
-                        for (int i = 0; i < QT; i++) *(uint2 *)(dst + i * term_b) = make_uint2(lo[i], hi[i]);
-                    }
-                    if (lane == 0) {
-                        // a query that is left out, or saw nothing (-inf), sees no row
-                        const float e = t >= 0 ? a.lse[w.s_layer * a.lse_layer + (long long)t * a.heads + head] : -INFINITY;
-                        s_col[qb][r] = make_float2(e * 1.4426950408889634f, __int_as_float(e == -INFINITY ? -1 : w.L + j));
+                    for (int i = 0; i < 4; i++) {
+                        const int r = r0 + 4 * i;
+                        if (r < N && (HD == 128 || lane < 16)) {
+                            uint32_t lo[QT], hi[QT];
+                            split_bf16<QT>(q[i].x, q[i].y, lo);
+                            split_bf16<QT>(q[i].z, q[i].w, hi);
+                            uint8_t *dst = dst0 + half * half_b + r * 128 + ((((c >> 3) ^ (r & 7)) << 4) | ((c & 4) << 1));
+#pragma unroll
+                            for (int x = 0; x < QT; x++) *(uint2 *)(dst + x * term_b) = make_uint2(lo[x], hi[x]);
+                        }
                     }
                 }
+                bar_sync(1, 128);  // s_tok is free again
                 fence_async_smem();
                 mb_arrive(&qfull[qb]);
             }
     } else {
-        const int th = threadIdx.x;
+        const int th = threadIdx.x & 127, group = warp >> 2;
         const float sl2 = a.scale * 1.4426950408889634f;
-        int it = 0, qi = 0;
+        int uses = 0, qi = 0, turn = 0;
         while (w.next(a)) {
             float *acc = a.acc + (((size_t)w.s_layer * a.v.slots + w.s_slot) * a.v.kvh + w.s_kvh) * a.acc_rows;
             for (int q0 = 0; q0 < w.n * a.G; q0 += NB, qi++) {
                 const int qb = qi % a.qbufs, N = (min(NB, w.n * a.G - q0) + 15) & ~15;
                 mb_wait(&qfull[qb], (qi / a.qbufs) & 1, &s_stop);
-                for (int t = w.s_a; t < w.s_b; t++, it++) {
-                    const int b = it % NS, r = t * 128 + th;
+                for (int t = w.s_a + (group - turn % NS + NS) % NS; t < w.s_b; t += NS, uses++) {
+                    const int r = t * 128 + th;
                     float sum = r < w.end && (r < w.L || q0 > 0) ? acc[r] : 0.f;
-                    mb_wait(&sfull[b], (it / NS) & 1, &s_stop);
+                    mb_wait(&sfull[group], uses & 1, &s_stop);
                     um_fence_after();
                     float part[2] = {0.f, 0.f};
                     for (int c = 0; c < N; c += 16) {
                         float x[16];
-                        um_ld16(tmem + ((uint32_t)(warp * 32) << 16) + b * 128 + c, x);
+                        um_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + group * 128 + c, x);
                         um_wait_ld<16>(x);
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
@@ -292,15 +324,16 @@ __global__ void __launch_bounds__(kWtThreads, 1) cache_weights_tc(const __grid_c
                         }
                     }
                     um_fence_before();
-                    mb_arrive(&sempty[b]);
+                    mb_arrive(&sempty[group]);
                     if (r < w.end) acc[r] = sum + (part[0] + part[1]);
                 }
                 mb_arrive(&qempty[qb]);
             }
+            turn++;
         }
     }
     __syncthreads();
-    if (warp == 5) {
+    if (warp == 17) {
         um_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
