@@ -10,6 +10,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -55,6 +56,8 @@ bool make_view(const hyc_kv_view *v, KvView &o, const char **why) {
     o.layer_stride = o.npages * o.page_stride;
     return true;
 }
+
+int lg2(int G) { return G == 1 ? 0 : G == 2 ? 1 : G == 4 ? 2 : 3; }
 
 bool group_ok(int heads, int kvh, int &G) {
     if (heads < 1 || heads % kvh) return false;
@@ -347,7 +350,7 @@ cudaError_t go(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, void 
     return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
-// Scratch of one tree attention: the columns' table, then two pieces a range
+// Scratch of one tree attention: the ranges' table, then two pieces a range
 // and row block (a range's first and last column may be split).
 struct TreeWs {
     int ranges, row_blocks;
@@ -358,7 +361,7 @@ TreeWs tree_ws(const KvView &v, int G, int max_nodes, int sms) {
     w.row_blocks = (max_nodes * G + 127) / 128;
     w.ranges = sms / w.row_blocks > 1 ? sms / w.row_blocks : 1;
     const size_t pieces = (size_t)2 * w.ranges * w.row_blocks;
-    w.ml = ((size_t)v.slots * v.kvh * sizeof(int2) + 255) & ~(size_t)255;
+    w.ml = ((size_t)w.ranges * sizeof(int4) + 255) & ~(size_t)255;
     w.o = w.ml + pieces * 128 * sizeof(float2);
     w.bytes = w.o + pieces * 128 * v.hd * sizeof(float);
     return w;
@@ -419,7 +422,8 @@ HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer
     if (sms < 1) return op_fail(err, err_cap, -3, "no usable CUDA device");
     const TreeWs ws = tree_ws(a.v, a.G, max_nodes, sms);
     if (ws_bytes < ws.bytes) return op_fail(err, err_cap, -1, "scratch too small");
-    a.cols = (int2 *)d_ws;
+    a.roots = (int4 *)d_ws;
+    a.lg = lg2(a.G);
     a.part_ml = (float2 *)((char *)d_ws + ws.ml);
     a.part_o = (float *)((char *)d_ws + ws.o);
     a.ranges = ws.ranges;
@@ -427,12 +431,12 @@ HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer
     a.min_tiles = 1;
     CUtensorMap map;
     if (!page_map(a.v, &map)) return op_fail(err, err_cap, -3, "cuTensorMapEncodeTiled failed");
-    const dim3 grid(ws.ranges * ws.row_blocks), mgrid(a.v.slots * a.v.kvh, (max_nodes * a.G + kMergeRows - 1) / kMergeRows);
+    const dim3 grid(ws.ranges * ws.row_blocks), mgrid(ws.ranges, std::min(8 * ws.row_blocks, (max_nodes * a.G + kMergeRows - 1) / kMergeRows));
     cudaError_t e = cudaErrorInvalidValue;
 #define HY_TREE(T_, HD_)                                                                                       \
     {                                                                                                          \
         e = go(tree_attn_tc<T_, HD_>, grid, dim3(kTtThreads), tt_smem<T_, HD_>(), stream, false, a, map);       \
-        if (e == cudaSuccess) e = go(tree_merge<T_, HD_, kTtK>, mgrid, dim3(256), 0, stream, true, a);          \
+        if (e == cudaSuccess) e = go(tree_merge<T_, HD_, kTtK>, mgrid, dim3(kMergeThreads), 0, stream, true, a);          \
     }
     if (q_bf16) {
         if (a.v.hd == 64) HY_TREE(__nv_bfloat16, 64) else HY_TREE(__nv_bfloat16, 128)
@@ -495,7 +499,7 @@ HYC_API int hyc_cache_weights(void *stream, const hyc_kv_view *cache, int heads,
     a.scale = scale;
     a.acc = d_acc;
     a.acc_rows = acc_rows;
-    a.lg = a.G == 1 ? 0 : a.G == 2 ? 1 : a.G == 4 ? 2 : 3;
+    a.lg = lg2(a.G);
     const int sms = device_sms();
     if (sms < 1) return op_fail(err, err_cap, -3, "no usable CUDA device");
     CUtensorMap map;

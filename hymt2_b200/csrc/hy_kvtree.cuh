@@ -21,10 +21,12 @@ struct TreeArgs {
     long long out_ld;
     float *lse;
     // split columns: the pieces' (max, sum) and unnormalised outputs, and for
-    // each (slot, KV head) {first tile, tiles per range}, first < 0: not split
-    int2 *cols;
+    // each range the column that starts in it and goes on in the next one as
+    // {slot, KV head, first tile, tiles per range}; slot < 0: none
+    int4 *roots;
     float2 *part_ml;
     float *part_o;
+    int lg;  // log2 G
     int ranges, row_blocks, min_tiles;
 };
 
@@ -141,28 +143,28 @@ __device__ __forceinline__ TreeWalk<TK> tree_walk(const int *s_start, int range)
 // by pointer doubling: after round k a node knows its next 2^k ancestors.
 // Called by NT threads (NT >= 64) that share named barrier `bar`.
 template <int NT>
-__device__ __forceinline__ void tree_masks(const TreeArgs &a, int t0, int n, int th, int bar, int *s_up,
+__device__ __forceinline__ void tree_masks(const TreeArgs &a, int t0, int n, int th, int bar, int8_t *s_up,
                                            unsigned long long *s_mask) {
     bar_sync(bar, NT);  // the masks of the segment before are no longer read
     int up = -1;
     unsigned long long m = 0;
     if (th < kTreeMax) {
         const int p = th < n ? __ldg(a.parent + t0 + th) : -2;
-        s_up[th] = p;
+        s_up[th] = (int8_t)(p == -2 ? -2 : p < 0 || p >= th ? -1 : p);
     }
     bar_sync(bar, NT);
     if (th < kTreeMax) {
         const int p = s_up[th];
         if (p != -2) {
             m = 1ull << th;
-            if (p >= 0 && p < th && s_up[p] != -2) up = p;
+            if (p >= 0 && s_up[p] != -2) up = p;
         }
     }
     bar_sync(bar, NT);
 #pragma unroll 1
     for (int k = 0; k < 6; k++) {
         if (th < kTreeMax) {
-            s_up[th] = up;
+            s_up[th] = (int8_t)up;
             s_mask[th] = m;
         }
         bar_sync(bar, NT);
@@ -176,11 +178,11 @@ __device__ __forceinline__ void tree_masks(const TreeArgs &a, int t0, int n, int
     bar_sync(bar, NT);
 }
 
-// x_r and v_r of a drafted row whose V is not finite, for one (node, head):
-// the matrix product leaves such rows out, and the nodes that see them add
-// them here, in the order of the rows.
+// p_r v_r of drafted rows whose V is not finite (in dims d0 .. d0 + HD / 2 -
+// 1), for one (node, head): the matrix product leaves such rows out, and the
+// nodes that see them add them here, in the order of the rows.
 template <typename T, int HD>
-__device__ __noinline__ void tree_add_bad(const TreeArgs &a, int slot, int kvh, int L, int t, int head,
+__device__ __noinline__ void tree_add_bad(const TreeArgs &a, int slot, int kvh, int L, int t, int head, int d0,
                                           unsigned long long bad, float sl2, float m, float *o) {
     while (bad) {
         const int j = __ffsll((long long)bad) - 1;
@@ -198,7 +200,7 @@ __device__ __noinline__ void tree_add_bad(const TreeArgs &a, int slot, int kvh, 
             x = fmaf(qq.w, bf16_bits_to_f32(k[d + 3]), x);
         }
         const float p = ex2((a.scale < 0.f ? -x : x) * sl2 - m);
-        for (int d = 0; d < HD; d++) o[d] = fmaf(p, bf16_bits_to_f32(v[d]), o[d]);
+        for (int d = 0; d < HD / 2; d++) o[d] = fmaf(p, bf16_bits_to_f32(v[d0 + d]), o[d]);
     }
 }
 
@@ -206,13 +208,15 @@ __device__ __noinline__ void tree_add_bad(const TreeArgs &a, int slot, int kvh, 
 //
 // One CTA takes up to 128 (node, head) rows, the lanes of a tensor-memory
 // tile, against tiles of 128 cached rows:
-//   warp 4     streams K and V pages by TMA into a ring of stages, 128-byte
+//   warp 8     streams K and V pages by TMA into a ring of stages, 128-byte
 //              swizzled: K rows are the K-major B operand of Q . K^T, V rows
 //              the MN-major B operand of P . V, so nothing is transposed
-//   warp 5     issues S = Q . K^T (two S tiles, so that the next
+//   warp 9     issues S = Q . K^T (two S tiles, so that the next
 //              one runs while this one's softmax does) and O += P . V
-//   warps 0-3  one row a thread: S from tensor memory, running maximum and
-//              sum, P back over S as the A operand in tensor memory
+//   warps 0-7  half a row's tile a thread: S from tensor memory, running
+//              maximum and sum, P back over S as the A operand in tensor
+//              memory (with four warps and a whole row a thread, the softmax
+//              took 2.7 us a tile, twice what its rows take from memory)
 // fp32 queries enter the bf16 products as three bf16 terms (all 24 bits), and
 // so does P for fp32 outputs: K and V are bf16 already, and every sum is
 // fp32.  For bf16 outputs P has two terms (16 bits): one would add an error
@@ -220,7 +224,7 @@ __device__ __noinline__ void tree_add_bad(const TreeArgs &a, int slot, int kvh, 
 // against moves only when it would grow by over 2^8, which rescales O; sums
 // and outputs stay exact under it, as the same one divides out at the end.
 constexpr int kTtK = 128;       // cached rows of a tile
-constexpr int kTtThreads = 192;
+constexpr int kTtThreads = 320, kTtSoft = 256;
 
 template <typename T>
 __host__ __device__ constexpr int tt_qterms() { return sizeof(T) == 4 ? 3 : 1; }
@@ -235,6 +239,7 @@ __host__ __device__ constexpr int tt_stages() {
     const int s = (224 * 1024 - tt_qbytes<T, HD>()) / tt_stage<HD>();
     return s > 8 ? 8 : s;
 }
+// Beside it the kernel has at most 2 KB of static shared memory.
 template <typename T, int HD>
 __host__ __device__ constexpr size_t tt_smem() { return (size_t)tt_qbytes<T, HD>() + (size_t)tt_stages<T, HD>() * tt_stage<HD>() + 1024; }
 
@@ -249,8 +254,10 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
     extern __shared__ uint8_t dsm[];
     __shared__ __align__(8) uint64_t full[NST], empty[NST], sfull[2], pfull[2], odone[2], qfull, ofree, fin;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_scan[kTtThreads / 32], s_start[4], s_up[kTreeMax];
-    __shared__ unsigned long long s_mask[kTreeMax], s_bad[2];
+    __shared__ int s_scan[kTtThreads / 32], s_start[4];
+    __shared__ int8_t s_up[kTreeMax];
+    __shared__ unsigned long long s_mask[kTreeMax], s_bad[2][2];
+    __shared__ float s_half[2][128];
     __shared__ int s_stop;
     uint8_t *sq = (uint8_t *)(((uintptr_t)dsm + 1023) & ~(uintptr_t)1023);
     uint8_t *ring = sq + tt_qbytes<T, HD>();
@@ -265,17 +272,17 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
         }
         for (int i = 0; i < 2; i++) {
             mb_init(&sfull[i], 1);
-            mb_init(&pfull[i], 128);
+            mb_init(&pfull[i], kTtSoft);
             mb_init(&odone[i], 1);
-            s_bad[i] = 0;
+            s_bad[i][0] = s_bad[i][1] = 0;
         }
-        mb_init(&qfull, 128);
-        mb_init(&ofree, 128);
+        mb_init(&qfull, kTtSoft);
+        mb_init(&ofree, kTtSoft);
         mb_init(&fin, 1);
         s_stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 5) {
+    if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(kv_smem(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         um_fence_before();
@@ -286,7 +293,9 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     TreeWalk<kTtK> w = tree_walk<kTtK>(s_start, range);
     const int cap = a.v.page_max * kPageRows;
-    if (warp == 4) {
+    const bool range_root = rb == 0 && threadIdx.x == 0;  // the thread that notes the range's split column
+    if (range_root) a.roots[range] = make_int4(-1, 0, 0, 0);
+    if (warp == 8) {
         // eight pages a tile, K then V; a page that does not exist is read past
         // the end of the map, which fills zeros
         const int y0 = a.layer * a.v.npages * 2 * kPageRows, yend = a.v.layers * a.v.npages * 2 * kPageRows;
@@ -321,7 +330,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             int none = 0;  // never set: the wait itself is bounded
             mb_wait(&full[p % NST], (p / NST) & 1, &none);
         }
-    } else if (warp == 5) {
+    } else if (warp == 9) {
         {
             constexpr uint32_t iqk = um_idesc(128, kTtK, false), ipv = um_idesc(128, HD, true);
             const uint32_t ring0 = __shfl_sync(0xffffffffu, kv_smem(ring), 0), q0 = um_desc_lo(__shfl_sync(0xffffffffu, kv_smem(sq), 0), 16);
@@ -376,27 +385,35 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             mb_wait(&fin, 0, &none);
         }
     } else {
-        const int th = threadIdx.x;
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        const int th = threadIdx.x & 127, h = warp >> 2;  // row, and half of its keys and dims
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const float sl2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);
         int it = 0, seg = 0, last_slot = -1;
-        // the segment's Q into shared memory, a warp to a row
+        // the segment's Q into shared memory, a warp to a row, four in flight
         auto load_q = [&](const TreeWalk<kTtK> &x) {
-            const int rows = min(NB, x.n - node0) * a.G;
-            const int half = HD == 128 ? lane >> 4 : 0, c = (HD == 128 ? lane & 15 : lane) * 4;  // dims half * 64 + c ..
-            if (HD == 128 || lane < 16) {
-#pragma unroll 4
-                for (int r = warp; r < rows; r += 4) {
-                    const T *src = (const T *)a.q + (long long)(x.t0 + node0 + r / a.G) * a.q_ld +
-                                   (long long)(x.s_kvh * a.G + r % a.G) * HD + half * 64 + c;
-                    float4 q = ld_row4(src);
-                    if (a.scale < 0.f) q = make_float4(-q.x, -q.y, -q.z, -q.w);
+            const int rows = min(NB, x.n - node0) << a.lg;
+            const int half = HD == 128 ? lane >> 4 : 0, c = (lane & 15) * 4;  // dims half * 64 + c ..
+            const bool on = HD == 128 || lane < 16;
+            const T *src = (const T *)a.q + (long long)(x.t0 + node0) * a.q_ld + (long long)x.s_kvh * a.G * HD + half * 64 + c;
+            for (int r0 = warp; r0 < rows; r0 += 32) {
+                float4 q[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int r = r0 + 8 * i;
+                    q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (on && r < rows) q[i] = ld_row4(src + (long long)(r >> a.lg) * a.q_ld + (r & (a.G - 1)) * HD);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int r = r0 + 8 * i;
+                    if (!on || r >= rows) continue;
+                    if (a.scale < 0.f) q[i] = make_float4(-q[i].x, -q[i].y, -q[i].z, -q[i].w);
                     uint32_t lo[QT], hi[QT];
-                    split_bf16<QT>(q.x, q.y, lo);
-                    split_bf16<QT>(q.z, q.w, hi);
+                    split_bf16<QT>(q[i].x, q[i].y, lo);
+                    split_bf16<QT>(q[i].z, q[i].w, hi);
                     uint8_t *dst = sq + half * 16384 + r * 128 + ((((c >> 3) ^ (r & 7)) << 4) | ((c & 4) << 1));
 #pragma unroll
-                    for (int i = 0; i < QT; i++) *(uint2 *)(dst + i * STB) = make_uint2(lo[i], hi[i]);
+                    for (int k = 0; k < QT; k++) *(uint2 *)(dst + k * STB) = make_uint2(lo[k], hi[k]);
                 }
             }
             fence_async_smem();
@@ -407,110 +424,114 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
         while (have) {
             const TreeWalk<kTtK> cur = w;
             if (cur.s_slot != last_slot) {
-                tree_masks<128>(a, cur.t0, cur.n, th, 1, s_up, s_mask);
+                tree_masks<kTtSoft>(a, cur.t0, cur.n, threadIdx.x, 1, s_up, s_mask);
                 last_slot = cur.s_slot;
             }
-            const int rows = min(NB, cur.n - node0) * a.G, end = min(cur.L + cur.n, cap);
-            const bool active = warp * 32 < rows;
-            const int node = node0 + th / a.G;
+            const int rows = min(NB, cur.n - node0) << a.lg, end = min(cur.L + cur.n, cap);
+            const bool active = (warp & 3) * 32 < rows;
+            const int node = node0 + (th >> a.lg);
             unsigned long long mask = th < rows ? s_mask[node] : 0;
+            const bool live = mask != 0;  // not a padding node
             if (end - cur.L < 64) mask &= (1ull << max(0, end - cur.L)) - 1;
-            const bool live = th < rows && s_mask[node] != 0;  // not a padding node
             float m = -INFINITY, l = 0.f;
             for (int t = cur.s_a; t < cur.s_b; t++, it++) {
                 const int b = it & 1, r0 = t * kTtK;
-                const bool tail = r0 + kTtK > cur.L;
+                const bool tail = r0 + kTtK > cur.L, first = t == cur.s_a;
                 mb_wait(&sfull[b], (it >> 1) & 1, &s_stop);
                 um_fence_after();
+                const uint32_t sp = tmem + lanes + kTtS + b * 128, px = tmem + lanes + kTtX + b * 64;
+                float s[64], my = -INFINITY;
                 if (active) {
-                    const uint32_t sp = tmem + lanes + kTtS + b * 128, px = tmem + lanes + kTtX + b * 64;
-                    float s[128];
 #pragma unroll
-                    for (int c = 0; c < 4; c++) um_ld32(sp + c * 32, s + c * 32);
-                    um_wait_ld<128>(s);
+                    for (int c = 0; c < 2; c++) um_ld32(sp + h * 64 + c * 32, s + c * 32);
+                    um_wait_ld<64>(s);
                     if (tail || !live) {
-                        // bits of the tile's rows that this node sees
-                        unsigned long long lo = 0, hi = 0;
-                        if (live) {
-                            const int c = cur.L - r0;  // cached rows of the tile
-                            if (c >= 64) {
-                                lo = ~0ull;
-                                hi = c >= 128 ? ~0ull : ((1ull << (c - 64)) - 1) | (mask << (c - 64));
-                            } else if (c > 0) {
-                                lo = ((1ull << c) - 1) | (mask << c);
-                                hi = mask >> (64 - c);
-                            } else {
-                                lo = -c >= 64 ? 0 : mask >> -c;
-                            }
-                        }
+                        // bits of this half's rows that the node sees
+                        const int c = cur.L - r0 - h * 64;  // cached rows among them
+                        unsigned long long see = 0;
+                        if (live) see = c >= 64 ? ~0ull : c > 0 ? ((1ull << c) - 1) | (mask << c) : -c >= 64 ? 0 : mask >> -c;
 #pragma unroll
-                        for (int c = 0; c < 128; c++)
-                            if (!(((c < 64 ? lo : hi) >> (c & 63)) & 1)) s[c] = -INFINITY;
+                        for (int i = 0; i < 64; i++)
+                            if (!((see >> i) & 1)) s[i] = -INFINITY;
                     }
                     float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int c = 4; c < 128; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-                    const float my = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-                    if (t == cur.s_a) {
-                        m = my;
-                    } else if (__any_sync(0xffffffffu, my > m + 8.f)) {
-                        mb_wait(&odone[(it - 1) & 1], ((it - 1) >> 1) & 1, &s_stop);
-                        um_fence_after();
-                        const float mn = my > m + 8.f ? my : m, f = m == -INFINITY ? 1.f : ex2(m - mn);
+                    for (int i = 4; i < 64; i++) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+                    my = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+                }
+                // both halves have read S, and whether any row's maximum moves
+                if (bar_or(2, kTtSoft, active && (first || my > m + 8.f))) {
+                    s_half[h][th] = my;
+                    bar_sync(1, kTtSoft);
+                    const float tm = fmaxf(my, s_half[h ^ 1][th]);
+                    if (first) {
+                        m = tm;
+                    } else {
+                        const float mn = tm > m + 8.f ? tm : m, f = m == -INFINITY ? 1.f : ex2(m - mn);
+                        const bool moved = mn > m;
                         m = mn;
                         l *= f;
+                        if (active && __any_sync(0xffffffffu, moved)) {
+                            mb_wait(&odone[(it - 1) & 1], ((it - 1) >> 1) & 1, &s_stop);
+                            um_fence_after();
 #pragma unroll
-                        for (int c = 0; c < HD / 32; c++) {
-                            float o[32];
-                            um_ld32(tmem + lanes + kTtO + c * 32, o);
-                            um_wait_ld<32>(o);
+                            for (int c = 0; c < HD / 64; c++) {
+                                const uint32_t at = tmem + lanes + kTtO + h * (HD / 2) + c * 32;
+                                float o[32];
+                                um_ld32(at, o);
+                                um_wait_ld<32>(o);
 #pragma unroll
-                            for (int i = 0; i < 32; i++) o[i] *= f;
-                            um_st32(tmem + lanes + kTtO + c * 32, o);
+                                for (int i = 0; i < 32; i++) o[i] *= f;
+                                um_st32(at, o);
+                            }
+                            um_wait_st();
                         }
-                        um_wait_st();
                     }
+                }
+                if (active) {
                     const float mr = m == -INFINITY ? 0.f : m;
                     float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
+                    for (int c = 0; c < 2; c++) {
                         uint32_t p[PT][16];
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
                             const float p0 = ex2(fmaf(s[c * 32 + 2 * i], sl2, -mr)), p1 = ex2(fmaf(s[c * 32 + 2 * i + 1], sl2, -mr));
-                            ls[c] += p0 + p1;
+                            ls[i & 3] += p0 + p1;
                             uint32_t x[PT];
                             split_bf16<PT>(p0, p1, x);
 #pragma unroll
                             for (int k = 0; k < PT; k++) p[k][i] = x[k];
                         }
-                        um_st16(sp + c * 16, p[0]);
-                        um_st16(sp + 64 + c * 16, p[1]);
-                        if constexpr (PT == 3) um_st16(px + c * 16, p[PT - 1]);
+                        um_st16(sp + h * 32 + c * 16, p[0]);
+                        um_st16(sp + 64 + h * 32 + c * 16, p[1]);
+                        if constexpr (PT == 3) um_st16(px + h * 32 + c * 16, p[PT - 1]);
                     }
                     l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
                     um_wait_st();
                 }
                 if (tail) {
                     // V rows that no node sees become zeros (a product with a
-                    // probability of 0 must be 0), and so do drafted rows that
-                    // are not finite, which the nodes that see them add at the end
+                    // probability of 0 must be 0), and so do halves of drafted
+                    // rows that are not finite, which the nodes that see them
+                    // add at the end
                     const int pos = 2 * it + 1, st = pos % NST, r = r0 + th;
                     mb_wait(&full[st], (pos / NST) & 1, &s_stop);
                     if (r >= cur.L) {
-                        uint8_t *vr = ring + (size_t)st * STB + th * 128;
+                        uint8_t *vr = ring + (size_t)st * STB + (HD == 128 ? h * 16384 : 0) + th * 128;
+                        const int c0 = HD == 128 ? 0 : h * 4;  // its 16-byte chunks
                         bool bad = false;
                         if (r < end)
-                            for (int i = 0; i < NH * 8; i++) {
-                                const uint4 u = *(const uint4 *)(vr + (i >> 3) * 16384 + (i & 7) * 16);
+                            for (int i = 0; i < HD / 16; i++) {
+                                const uint4 u = *(const uint4 *)(vr + (((c0 + i) ^ (th & 7)) << 4));
                                 const uint32_t x[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
                                 for (int k = 0; k < 4; k++)
                                     bad |= (x[k] & 0x7f80u) == 0x7f80u || (x[k] & 0x7f800000u) == 0x7f800000u;
                             }
-                        if (bad) atomicOr(&s_bad[seg & 1], 1ull << (r - cur.L));
+                        if (bad) atomicOr(&s_bad[seg & 1][h], 1ull << (r - cur.L));
                         if (bad || r >= end)
-                            for (int i = 0; i < NH * 8; i++) *(uint4 *)(vr + (i >> 3) * 16384 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            for (int i = 0; i < HD / 16; i++) *(uint4 *)(vr + (((c0 + i) ^ (th & 7)) << 4)) = make_uint4(0, 0, 0, 0);
                     }
                     fence_async_smem();
                 }
@@ -521,44 +542,45 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             // while the last P . V runs
             have = w.next(a, node0);
             if (have) load_q(w);
+            s_half[h][th] = l;
+            bar_sync(1, kTtSoft);  // and s_bad is complete
+            l = h ? s_half[0][th] + l : l + s_half[1][th];
+            const unsigned long long bad = s_bad[seg & 1][h] & mask;
+            if (th == 0) s_bad[(seg + 1) & 1][h] = 0;
+            const bool whole = cur.s_a == 0 && cur.s_b == cur.T;
             mb_wait(&odone[(it - 1) & 1], ((it - 1) >> 1) & 1, &s_stop);
             um_fence_after();
-            bar_sync(1, 128);  // s_bad is complete
-            const unsigned long long bad = s_bad[seg & 1] & mask;
-            if (th == 0) s_bad[(seg + 1) & 1] = 0;
-            const bool whole = cur.s_a == 0 && cur.s_b == cur.T;
             if (active) {
-                float o[HD];
+                constexpr int W = HD / 2;
+                float o[W];
 #pragma unroll
-                for (int c = 0; c < HD / 32; c++) um_ld32(tmem + lanes + kTtO + c * 32, o + c * 32);
-                um_wait_ld<HD>(o);
+                for (int c = 0; c < W / 32; c++) um_ld32(tmem + lanes + kTtO + h * W + c * 32, o + c * 32);
+                um_wait_ld<W>(o);
                 um_fence_before();
                 mb_arrive(&ofree);
                 if (th < rows) {
-                    const int tok = cur.t0 + node, head = cur.s_kvh * a.G + th % a.G;
+                    const int tok = cur.t0 + node, head = cur.s_kvh * a.G + (th & (a.G - 1));
                     if (bad && l > 0.f) {
-                        float x[HD];  // its address is taken: o stays in registers
+                        float x[W];  // its address is taken: o stays in registers
 #pragma unroll
-                        for (int d = 0; d < HD; d++) x[d] = o[d];
-                        tree_add_bad<T, HD>(a, cur.s_slot, cur.s_kvh, cur.L, tok, head, bad, sl2, m, x);
+                        for (int d = 0; d < W; d++) x[d] = o[d];
+                        tree_add_bad<T, HD>(a, cur.s_slot, cur.s_kvh, cur.L, tok, head, h * W, bad, sl2, m, x);
 #pragma unroll
-                        for (int d = 0; d < HD; d++) o[d] = x[d];
+                        for (int d = 0; d < W; d++) o[d] = x[d];
                     }
                     if (whole) {
                         const float inv = l == 0.f ? 0.f : 1.0f / l;
-                        T *dst = (T *)a.out + (long long)tok * a.out_ld + (long long)head * HD;
+                        T *dst = (T *)a.out + (long long)tok * a.out_ld + (long long)head * HD + h * W;
 #pragma unroll
-                        for (int d = 0; d < HD; d += 4) {
-                            if (l == 0.f) st_row4(dst + d, 0.f, 0.f, 0.f, 0.f);
-                            else st_row4(dst + d, o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
-                        }
-                        if (a.lse) a.lse[(long long)tok * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                        for (int d = 0; d < W; d += 4) st_row4(dst + d, o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
+                        if (a.lse && h == 0)
+                            a.lse[(long long)tok * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
                     } else {
                         const int piece = (2 * range + (cur.s_g != cur.g0)) * a.row_blocks + rb;
-                        a.part_ml[(size_t)piece * 128 + th] = make_float2(m, l);
-                        float *po = a.part_o + (size_t)piece * 128 * HD + th * 8;
+                        if (h == 0) a.part_ml[(size_t)piece * 128 + th] = make_float2(m, l);
+                        float *po = a.part_o + (size_t)piece * 128 * HD + h * W * 128 + th * 8;
 #pragma unroll
-                        for (int d = 0; d < HD; d += 8) {
+                        for (int d = 0; d < W; d += 8) {
                             *(float4 *)(po + d * 128) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
                             *(float4 *)(po + d * 128 + 4) = make_float4(o[d + 4], o[d + 5], o[d + 6], o[d + 7]);
                         }
@@ -567,78 +589,85 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             } else {
                 mb_arrive(&ofree);
             }
-            if (th == 0 && cur.s_a == 0 && rb == 0)
-                a.cols[cur.s_slot * a.v.kvh + cur.s_kvh] = make_int2(whole ? -1 : cur.s_g, s_start[3]);
-            bar_sync(1, 128);
+            if (range_root && cur.s_a == 0 && !whole) a.roots[range] = make_int4(cur.s_slot, cur.s_kvh, cur.s_g, s_start[3]);
+            bar_sync(1, kTtSoft);
             seg++;
         }
     }
     __syncthreads();
-    if (warp == 5) {
+    if (warp == 9) {
         um_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
 }
 
-// grid (slots * kv heads, blocks of kMergeRows rows): joins the pieces of a
-// split column, a warp to a (node, head) row, hd / 32 dims a lane: M = max m_i,
-// out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i, in the order of the pieces.
-constexpr int kMergeRows = 16;
+// grid (ranges, blocks of rows): joins the pieces of the column that starts in
+// a range and goes on in the next: M = max m_i, out = sum 2^(m_i - M) o_i / sum
+// 2^(m_i - M) l_i.  Four warps to a (node, head) row, each every fourth piece,
+// hd / 32 dims a lane, joined in a fixed order.
+constexpr int kMergeRows = 4, kMergeThreads = kMergeRows * 128;
 template <typename T, int HD, int TK>
-__global__ void __launch_bounds__(256) tree_merge(const __grid_constant__ TreeArgs a) {
+__global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constant__ TreeArgs a) {
     constexpr int D = HD / 32;
+    __shared__ float s_o[kMergeRows][4][HD], s_s[kMergeRows][4];
     pdl_wait();
-    const int slot = blockIdx.x / a.v.kvh, kvh = blockIdx.x % a.v.kvh, lane = threadIdx.x & 31;
+    const int4 root = a.roots[blockIdx.x];
+    if (root.x < 0) return;
+    const int lane = threadIdx.x & 31, row = threadIdx.x >> 7, part = (threadIdx.x >> 5) & 3;
     int L, t0, n;
-    tree_span(a.v, a.len, a.off, a.max_nodes, slot, L, t0, n);
-    if ((int)blockIdx.y * kMergeRows >= n * a.G) return;
-    const int2 col = a.cols[blockIdx.x];
-    if (col.x < 0) return;
-    const int T_ = TreeWalk<TK>::tiles(L, n, a.v.page_max * kPageRows), C = col.y;
-    const int p0 = col.x / C, p1 = (col.x + T_ - 1) / C, NB = 128 / a.G;
-    for (int r = blockIdx.y * kMergeRows + (threadIdx.x >> 5); r < min(n * a.G, (int)(blockIdx.y + 1) * kMergeRows); r += 8) {
-        const int node = r / a.G, rb = node / NB, lr = r - rb * 128;
-        auto piece = [&](int p) { return (size_t)((2 * p + (p * C < col.x)) * a.row_blocks + rb); };
-        float M = -INFINITY;
-        for (int p = p0 + lane; p <= p1; p += 32) {
-            const float2 ml = a.part_ml[piece(p) * 128 + lr];
-            if (ml.y != 0.f) M = fmaxf(M, ml.x);
-        }
-        M = warp_max(M);
-        float S = 0.f, o[D];
+    tree_span(a.v, a.len, a.off, a.max_nodes, root.x, L, t0, n);
+    const int T_ = TreeWalk<TK>::tiles(L, n, a.v.page_max * kPageRows), C = root.w;
+    const int p0 = root.z / C, p1 = (root.z + T_ - 1) / C, rows = n * a.G;
+    for (int r0 = blockIdx.y * kMergeRows; r0 < rows; r0 += gridDim.y * kMergeRows) {
+        const int r = r0 + row, node = r / a.G, rb = r >> 7, lr = r & 127;
+        const auto piece = [&](int p) { return (size_t)((2 * p + (p * C < root.z)) * a.row_blocks + rb); };
+        float M = -INFINITY, S = 0.f, o[D];
 #pragma unroll
         for (int d = 0; d < D; d++) o[d] = 0.f;
         const int d0 = lane * D;
-#pragma unroll 4
-        for (int p = p0; p <= p1; p++) {
-            const size_t pc = piece(p);
-            const float2 ml = a.part_ml[pc * 128 + lr];
-            const float *po = a.part_o + pc * 128 * HD + (d0 >> 3) * 1024 + lr * 8 + (d0 & 7);
-            float v[D];
-            if constexpr (D == 4) {
-                const float4 x = *(const float4 *)po;
-                v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-            } else {
-                const float2 x = *(const float2 *)po;
-                v[0] = x.x, v[1] = x.y;
+        if (r < rows) {
+            for (int p = p0 + lane; p <= p1; p += 32) {
+                const float2 ml = a.part_ml[piece(p) * 128 + lr];
+                if (ml.y != 0.f) M = fmaxf(M, ml.x);
             }
-            if (ml.y == 0.f) continue;  // nothing seen in this piece
-            const float f = ex2(ml.x - M);
-            S = fmaf(ml.y, f, S);
+            M = warp_max(M);
+#pragma unroll 4
+            for (int p = p0 + part; p <= p1; p += 4) {
+                const size_t pc = piece(p);
+                const float2 ml = a.part_ml[pc * 128 + lr];
+                const float *po = a.part_o + pc * 128 * HD + (d0 >> 3) * 1024 + lr * 8 + (d0 & 7);
+                float v[D];
+                if constexpr (D == 4) {
+                    const float4 x = *(const float4 *)po;
+                    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+                } else {
+                    const float2 x = *(const float2 *)po;
+                    v[0] = x.x, v[1] = x.y;
+                }
+                const float f = ml.y == 0.f ? 0.f : ex2(ml.x - M);  // 0: nothing seen in this piece
+                S = fmaf(ml.y, f, S);
 #pragma unroll
-            for (int d = 0; d < D; d++) o[d] = fmaf(v[d], f, o[d]);
+                for (int d = 0; d < D; d++) o[d] = fmaf(v[d], f, o[d]);
+            }
         }
-        const int tok = t0 + node, head = kvh * a.G + r % a.G;
-        T *dst = (T *)a.out + (long long)tok * a.out_ld + (long long)head * HD + d0;
-        const float inv = S == 0.f ? 0.f : 1.0f / S;
-        if constexpr (D == 4) {
-            st_row4(dst, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-        } else if constexpr (sizeof(T) == 4) {
-            *(float2 *)dst = make_float2(o[0] * inv, o[1] * inv);
-        } else {
-            *(uint32_t *)dst = pack_bf16(o[0] * inv, o[1] * inv);
+#pragma unroll
+        for (int d = 0; d < D; d++) s_o[row][part][d0 + d] = o[d];
+        if (lane == 0) s_s[row][part] = S;
+        __syncthreads();
+        if (part == 0 && r < rows) {
+            S = (s_s[row][0] + s_s[row][1]) + (s_s[row][2] + s_s[row][3]);
+            const float inv = S == 0.f ? 0.f : 1.0f / S;
+#pragma unroll
+            for (int d = 0; d < D; d++)
+                o[d] = ((s_o[row][0][d0 + d] + s_o[row][1][d0 + d]) + (s_o[row][2][d0 + d] + s_o[row][3][d0 + d])) * inv;
+            const int tok = t0 + node, head = root.y * a.G + r % a.G;
+            T *dst = (T *)a.out + (long long)tok * a.out_ld + (long long)head * HD + d0;
+            if constexpr (D == 4) st_row4(dst, o[0], o[1], o[2], o[3]);
+            else if constexpr (sizeof(T) == 4) *(float2 *)dst = make_float2(o[0], o[1]);
+            else *(uint32_t *)dst = pack_bf16(o[0], o[1]);
+            if (a.lse && lane == 0) a.lse[(long long)tok * a.heads + head] = S == 0.f ? -INFINITY : (M + log2f(S)) * 0.6931471805599453f;
         }
-        if (a.lse && lane == 0) a.lse[(long long)tok * a.heads + head] = S == 0.f ? -INFINITY : (M + log2f(S)) * 0.6931471805599453f;
+        __syncthreads();
     }
 }
 

@@ -97,6 +97,17 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// Barrier of `threads` threads that tells each whether any of them said v.
+__device__ __forceinline__ bool bar_or(int id, int threads, bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 q, %3, 0;\n barrier.cta.red.or.pred p, %1, %2, q;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(r)
+        : "r"(id), "r"(threads), "r"((uint32_t)v)
+        : "memory");
+    return r != 0;
+}
+
 // ---------------------------------------------------------------- tcgen05
 
 __device__ __forceinline__ void um_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
