@@ -59,6 +59,10 @@ bool make_view(const hyc_kv_view *v, KvView &o, const char **why) {
 
 int lg2(int G) { return G == 1 ? 0 : G == 2 ? 1 : G == 4 ? 2 : 3; }
 
+// Rows (nodes x heads of a group) up to which a tree takes the narrow form,
+// the least tiles of one of its ranges, and its most CTAs an SM.
+constexpr int kNarrowRows = 32, kNarrowTiles = 1, kNarrowCtas = 3;
+
 bool group_ok(int heads, int kvh, int &G) {
     if (heads < 1 || heads % kvh) return false;
     G = heads / kvh;
@@ -90,6 +94,12 @@ bool page_map(const KvView &v, CUtensorMap *map) {
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <typename T, int HD, typename F>
+bool raise_narrow(F raise) {
+    return raise((const void *)tree_attn_mma<T, HD, 1>, tn_smem<T, HD, 1>()) && raise((const void *)tree_attn_mma<T, HD, 2>, tn_smem<T, HD, 2>()) &&
+           raise((const void *)tree_attn_mma<T, HD, 3>, tn_smem<T, HD, 3>()) && raise((const void *)tree_attn_mma<T, HD, 4>, tn_smem<T, HD, 4>());
+}
+
 // SMs of the current device, with the kernels' shared-memory limits raised on
 // its first use; 0 when there is no usable device.
 int device_sms() {
@@ -109,6 +119,8 @@ int device_sms() {
         !raise((const void *)tree_attn_tc<float, 128>, tt_smem<float, 128>()) ||
         !raise((const void *)tree_attn_tc<__nv_bfloat16, 64>, tt_smem<__nv_bfloat16, 64>()) ||
         !raise((const void *)tree_attn_tc<__nv_bfloat16, 128>, tt_smem<__nv_bfloat16, 128>()) ||
+        !raise_narrow<float, 64>(raise) || !raise_narrow<float, 128>(raise) || !raise_narrow<__nv_bfloat16, 64>(raise) ||
+        !raise_narrow<__nv_bfloat16, 128>(raise) ||
         !raise((const void *)cache_weights_tc<float, 64>, kWtSmem + 1024) ||
         !raise((const void *)cache_weights_tc<float, 128>, kWtSmem + 1024) ||
         !raise((const void *)cache_weights_tc<__nv_bfloat16, 64>, kWtSmem + 1024) ||
@@ -350,20 +362,24 @@ cudaError_t go(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, void 
     return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
-// Scratch of one tree attention: the ranges' table, then two pieces a range
-// and row block (a range's first and last column may be split).
+// One tree attention's form and its scratch: the ranges' table, then two
+// pieces a range and row block (a range's first and last column may be split).
+// Up to 32 (node, head) rows take the narrow form, with a warp to a range.
 struct TreeWs {
-    int ranges, row_blocks;
+    bool narrow;
+    int ranges, row_blocks, rows;  // rows: of a piece
     size_t ml, o, bytes;
 };
 TreeWs tree_ws(const KvView &v, int G, int max_nodes, int sms) {
     TreeWs w;
-    w.row_blocks = (max_nodes * G + 127) / 128;
-    w.ranges = sms / w.row_blocks > 1 ? sms / w.row_blocks : 1;
+    w.narrow = max_nodes * G <= kNarrowRows;
+    w.row_blocks = w.narrow ? 1 : (max_nodes * G + 127) / 128;
+    w.rows = w.narrow ? (max_nodes * G + 7) & ~7 : 128;
+    w.ranges = w.narrow ? sms * kNarrowCtas : sms / w.row_blocks > 1 ? sms / w.row_blocks : 1;
     const size_t pieces = (size_t)2 * w.ranges * w.row_blocks;
     w.ml = ((size_t)w.ranges * sizeof(int4) + 255) & ~(size_t)255;
-    w.o = w.ml + pieces * 128 * sizeof(float2);
-    w.bytes = w.o + pieces * 128 * v.hd * sizeof(float);
+    w.o = w.ml + ((pieces * w.rows * sizeof(float2) + 255) & ~(size_t)255);
+    w.bytes = w.o + pieces * w.rows * v.hd * sizeof(float);
     return w;
 }
 
@@ -428,15 +444,35 @@ HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer
     a.part_o = (float *)((char *)d_ws + ws.o);
     a.ranges = ws.ranges;
     a.row_blocks = ws.row_blocks;
+    cudaError_t e = cudaErrorInvalidValue;
+    const dim3 mgrid(4 * sms);
+    if (ws.narrow) {
+        a.min_tiles = kNarrowTiles;
+        // as many CTAs as an SM holds (ranges are equal shares, so all of them
+        // should run at once), by shared memory and the kernel's register bound
+#define HY_NT(T_, HD_, NT_)                                                                                             \
+    if (ws.rows == 8 * NT_) {                                                                                           \
+        a.ranges = sms * std::min(kNarrowCtas, (int)(227 * 1024 / (tn_smem<T_, HD_, NT_>() + 2048)));                             \
+        e = go(tree_attn_mma<T_, HD_, NT_>, dim3(a.ranges), dim3(kTnThreads), tn_smem<T_, HD_, NT_>(), stream, false, a); \
+        if (e == cudaSuccess) e = go(tree_merge<T_, HD_, kTnK>, mgrid, dim3(kMergeThreads), 0, stream, true, a, ws.rows); \
+    }
+#define HY_TREE(T_, HD_) HY_NT(T_, HD_, 1) HY_NT(T_, HD_, 2) HY_NT(T_, HD_, 3) HY_NT(T_, HD_, 4)
+        if (q_bf16 && a.v.hd == 64) { HY_TREE(__nv_bfloat16, 64) }
+        else if (q_bf16) { HY_TREE(__nv_bfloat16, 128) }
+        else if (a.v.hd == 64) { HY_TREE(float, 64) }
+        else { HY_TREE(float, 128) }
+#undef HY_TREE
+#undef HY_NT
+        return done(e, err, err_cap);
+    }
     a.min_tiles = 1;
     CUtensorMap map;
     if (!page_map(a.v, &map)) return op_fail(err, err_cap, -3, "cuTensorMapEncodeTiled failed");
-    const dim3 grid(ws.ranges * ws.row_blocks), mgrid(ws.ranges, std::min(8 * ws.row_blocks, (max_nodes * a.G + kMergeRows - 1) / kMergeRows));
-    cudaError_t e = cudaErrorInvalidValue;
-#define HY_TREE(T_, HD_)                                                                                       \
-    {                                                                                                          \
-        e = go(tree_attn_tc<T_, HD_>, grid, dim3(kTtThreads), tt_smem<T_, HD_>(), stream, false, a, map);       \
-        if (e == cudaSuccess) e = go(tree_merge<T_, HD_, kTtK>, mgrid, dim3(kMergeThreads), 0, stream, true, a);          \
+    const dim3 grid(ws.ranges * ws.row_blocks);
+#define HY_TREE(T_, HD_)                                                                                                \
+    {                                                                                                                   \
+        e = go(tree_attn_tc<T_, HD_>, grid, dim3(kTtThreads), tt_smem<T_, HD_>(), stream, false, a, map);                \
+        if (e == cudaSuccess) e = go(tree_merge<T_, HD_, kTtK>, mgrid, dim3(kMergeThreads), 0, stream, true, a, 0);       \
     }
     if (q_bf16) {
         if (a.v.hd == 64) HY_TREE(__nv_bfloat16, 64) else HY_TREE(__nv_bfloat16, 128)

@@ -34,6 +34,16 @@ __device__ __forceinline__ void st_row4(float *p, float a, float b, float c, flo
 __device__ __forceinline__ void st_row4(__nv_bfloat16 *p, float a, float b, float c, float d) {
     *(uint2 *)p = make_uint2(pack_bf16(a, b), pack_bf16(c, d));
 }
+// Eight values of a row, 32 (bf16: 16) bytes a lane.
+__device__ __forceinline__ void st_row8(float *p, const float *v, float f) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0] * f), "f"(v[1] * f), "f"(v[2] * f),
+                 "f"(v[3] * f), "f"(v[4] * f), "f"(v[5] * f), "f"(v[6] * f), "f"(v[7] * f)
+                 : "memory");
+}
+__device__ __forceinline__ void st_row8(__nv_bfloat16 *p, const float *v, float f) {
+    *(uint4 *)p = make_uint4(pack_bf16(v[0] * f, v[1] * f), pack_bf16(v[2] * f, v[3] * f), pack_bf16(v[4] * f, v[5] * f),
+                             pack_bf16(v[6] * f, v[7] * f));
+}
 __device__ __forceinline__ float4 ld_row4(const float *p) { return *(const float4 *)p; }
 __device__ __forceinline__ float4 ld_row4(const __nv_bfloat16 *p) {
     const uint2 u = *(const uint2 *)p;
@@ -82,9 +92,9 @@ struct TreeWalk {
     }
 };
 
-// The walk's start for this CTA's range.  Every thread takes a run of slots;
-// s_scan holds blockDim.x / 32 + 2 ints of scratch, s_start 4.
-template <int TK>
+// The walks' starts for NR ranges from `range` on.  Every thread takes a run of
+// slots; s_scan holds blockDim.x / 32 ints of scratch, s_start 4 for each range.
+template <int TK, int NR>
 __device__ __forceinline__ void tree_plan(const TreeArgs &a, int range, int *s_scan, int *s_start) {
     const int th = threadIdx.x, nth = blockDim.x, lane = th & 31, w = th >> 5, cap = a.v.page_max * kPageRows;
     const int per = (a.v.slots + nth - 1) / nth, b0 = min(a.v.slots, th * per), b1 = min(a.v.slots, b0 + per);
@@ -107,22 +117,27 @@ __device__ __forceinline__ void tree_plan(const TreeArgs &a, int range, int *s_s
         if (i < w) before += s_scan[i];
         total += s_scan[i];
     }
-    const int C = max((total + a.ranges - 1) / a.ranges, a.min_tiles), g0 = range * C;
-    if (th == 0) {
-        s_start[2] = max(0, min(C, total - g0));  // tiles of this range
-        s_start[3] = C;
+    const int C = max((total + a.ranges - 1) / a.ranges, a.min_tiles);
+    if (th < NR) {
+        const long long g0 = (long long)(range + th) * C;
+        s_start[4 * th + 2] = (int)max(0LL, min((long long)C, total - g0));  // tiles of this range
+        s_start[4 * th + 3] = C;
     }
-    if (g0 >= before && g0 < before + sum) {
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+        const long long g0 = (long long)(range + i) * C;
+        if (g0 < before || g0 >= before + sum) continue;
+        int at = before;
         for (int s = b0; s < b1; s++) {
             int L, t0, n;
             tree_span(a.v, a.len, a.off, a.max_nodes, s, L, t0, n);
             const int c = TreeWalk<TK>::tiles(L, n, cap) * a.v.kvh;
-            if (g0 < before + c) {
-                s_start[0] = s;
-                s_start[1] = g0 - before;
+            if (g0 < at + c) {
+                s_start[4 * i] = s;
+                s_start[4 * i + 1] = (int)g0 - at;
                 break;
             }
-            before += c;
+            at += c;
         }
     }
     __syncthreads();
@@ -134,48 +149,22 @@ __device__ __forceinline__ TreeWalk<TK> tree_walk(const int *s_start, int range)
     w.left = s_start[2];
     w.slot = w.left > 0 ? s_start[0] : 0;
     w.rem = w.left > 0 ? s_start[1] : 0;
-    w.g = w.g0 = range * s_start[3];
+    w.g = w.g0 = w.left > 0 ? range * s_start[3] : 0;
     w.at = -1;
     return w;
 }
 
-// Ancestor masks of a slot's nodes (bit j of s_mask[i]: node i sees node j),
-// by pointer doubling: after round k a node knows its next 2^k ancestors.
-// Called by NT threads (NT >= 64) that share named barrier `bar`.
-template <int NT>
-__device__ __forceinline__ void tree_masks(const TreeArgs &a, int t0, int n, int th, int bar, int8_t *s_up,
-                                           unsigned long long *s_mask) {
-    bar_sync(bar, NT);  // the masks of the segment before are no longer read
-    int up = -1;
+// A node's parent as the walk below takes it: -2 padding, -1 none.
+__device__ __forceinline__ int tree_parent(const TreeArgs &a, int t0, int n, int i) {
+    const int p = i < n ? __ldg(a.parent + t0 + i) : -2;
+    return p == -2 ? -2 : p < 0 || p >= i ? -1 : p;
+}
+// Bits of the nodes that node i sees: itself and its ancestors up to the root
+// or to a padding node.  Parents lie below their nodes, so the walk ends.
+__device__ __forceinline__ unsigned long long tree_mask(const int8_t *s_up, int i) {
     unsigned long long m = 0;
-    if (th < kTreeMax) {
-        const int p = th < n ? __ldg(a.parent + t0 + th) : -2;
-        s_up[th] = (int8_t)(p == -2 ? -2 : p < 0 || p >= th ? -1 : p);
-    }
-    bar_sync(bar, NT);
-    if (th < kTreeMax) {
-        const int p = s_up[th];
-        if (p != -2) {
-            m = 1ull << th;
-            if (p >= 0 && s_up[p] != -2) up = p;
-        }
-    }
-    bar_sync(bar, NT);
-#pragma unroll 1
-    for (int k = 0; k < 6; k++) {
-        if (th < kTreeMax) {
-            s_up[th] = (int8_t)up;
-            s_mask[th] = m;
-        }
-        bar_sync(bar, NT);
-        if (th < kTreeMax && up >= 0) {
-            m |= s_mask[up];
-            up = s_up[up];
-        }
-        bar_sync(bar, NT);
-    }
-    if (th < kTreeMax) s_mask[th] = m;
-    bar_sync(bar, NT);
+    for (int p = i; p >= 0 && s_up[p] != -2; p = s_up[p]) m |= 1ull << p;
+    return m;
 }
 
 // p_r v_r of drafted rows whose V is not finite (in dims d0 .. d0 + HD / 2 -
@@ -256,7 +245,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
     __shared__ uint32_t s_tmem;
     __shared__ int s_scan[kTtThreads / 32], s_start[4];
     __shared__ int8_t s_up[kTreeMax];
-    __shared__ unsigned long long s_mask[kTreeMax], s_bad[2][2];
+    __shared__ unsigned long long s_bad[2][2];
     __shared__ float s_half[2][128];
     __shared__ int s_stop;
     uint8_t *sq = (uint8_t *)(((uintptr_t)dsm + 1023) & ~(uintptr_t)1023);
@@ -288,7 +277,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
         um_fence_before();
     }
     pdl_wait();
-    tree_plan<kTtK>(a, range, s_scan, s_start);
+    tree_plan<kTtK, 1>(a, range, s_scan, s_start);
     um_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     TreeWalk<kTtK> w = tree_walk<kTtK>(s_start, range);
@@ -302,6 +291,14 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
         int pos = 0;
         while (w.next(a, node0)) {
             const int pages = (min(w.L + w.n, cap) + kPageRows - 1) / kPageRows;
+            // the segment's queries towards L2: the softmax warps load them when
+            // the segment before has used its own
+            for (int i = lane; i < (min(NB, w.n - node0) << a.lg) * (HD * (int)sizeof(T) / 128); i += 32) {
+                const int e = i * (128 / (int)sizeof(T)), r = e / HD;
+                const T *q = (const T *)a.q + (long long)(w.t0 + node0 + (r >> a.lg)) * a.q_ld +
+                             (long long)(w.s_kvh * a.G + (r & (a.G - 1))) * HD + e % HD;
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+            }
             for (int t = w.s_a; t < w.s_b; t++) {
                 const int j = t * (kTtK / kPageRows) + (lane & 7);
                 int pg = j < pages ? __ldg(a.v.pages + (size_t)w.s_slot * a.v.page_max + j) : -1;
@@ -388,23 +385,26 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
         const int th = threadIdx.x & 127, h = warp >> 2;  // row, and half of its keys and dims
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const float sl2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);
-        int it = 0, seg = 0, last_slot = -1;
-        // the segment's Q into shared memory, a warp to a row, four in flight
+        int it = 0, seg = 0;
+        int up = -1;
+        // the segment's Q into shared memory, a warp to a row, eight in flight,
+        // and its nodes' parents on their way
         auto load_q = [&](const TreeWalk<kTtK> &x) {
             const int rows = min(NB, x.n - node0) << a.lg;
+            if (threadIdx.x < kTreeMax) up = tree_parent(a, x.t0, x.n, threadIdx.x);
             const int half = HD == 128 ? lane >> 4 : 0, c = (lane & 15) * 4;  // dims half * 64 + c ..
             const bool on = HD == 128 || lane < 16;
             const T *src = (const T *)a.q + (long long)(x.t0 + node0) * a.q_ld + (long long)x.s_kvh * a.G * HD + half * 64 + c;
-            for (int r0 = warp; r0 < rows; r0 += 32) {
-                float4 q[4];
+            for (int r0 = warp; r0 < rows; r0 += 64) {
+                float4 q[8];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
+                for (int i = 0; i < 8; i++) {
                     const int r = r0 + 8 * i;
                     q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (on && r < rows) q[i] = ld_row4(src + (long long)(r >> a.lg) * a.q_ld + (r & (a.G - 1)) * HD);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
+                for (int i = 0; i < 8; i++) {
                     const int r = r0 + 8 * i;
                     if (!on || r >= rows) continue;
                     if (a.scale < 0.f) q[i] = make_float4(-q[i].x, -q[i].y, -q[i].z, -q[i].w);
@@ -423,14 +423,12 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
         if (have) load_q(w);
         while (have) {
             const TreeWalk<kTtK> cur = w;
-            if (cur.s_slot != last_slot) {
-                tree_masks<kTtSoft>(a, cur.t0, cur.n, threadIdx.x, 1, s_up, s_mask);
-                last_slot = cur.s_slot;
-            }
+            if (threadIdx.x < kTreeMax) s_up[threadIdx.x] = (int8_t)up;
+            bar_sync(1, kTtSoft);
             const int rows = min(NB, cur.n - node0) << a.lg, end = min(cur.L + cur.n, cap);
             const bool active = (warp & 3) * 32 < rows;
             const int node = node0 + (th >> a.lg);
-            unsigned long long mask = th < rows ? s_mask[node] : 0;
+            unsigned long long mask = th < rows ? tree_mask(s_up, node) : 0;
             const bool live = mask != 0;  // not a padding node
             if (end - cur.L < 64) mask &= (1ull << max(0, end - cur.L)) - 1;
             float m = -INFINITY, l = 0.f;
@@ -572,7 +570,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                         const float inv = l == 0.f ? 0.f : 1.0f / l;
                         T *dst = (T *)a.out + (long long)tok * a.out_ld + (long long)head * HD + h * W;
 #pragma unroll
-                        for (int d = 0; d < W; d += 4) st_row4(dst + d, o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
+                        for (int d = 0; d < W; d += 8) st_row8(dst + d, o + d, inv);
                         if (a.lse && h == 0)
                             a.lse[(long long)tok * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
                     } else {
@@ -580,10 +578,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                         if (h == 0) a.part_ml[(size_t)piece * 128 + th] = make_float2(m, l);
                         float *po = a.part_o + (size_t)piece * 128 * HD + h * W * 128 + th * 8;
 #pragma unroll
-                        for (int d = 0; d < W; d += 8) {
-                            *(float4 *)(po + d * 128) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
-                            *(float4 *)(po + d * 128 + 4) = make_float4(o[d + 4], o[d + 5], o[d + 6], o[d + 7]);
-                        }
+                        for (int d = 0; d < W; d += 8) st_row8(po + d * 128, o + d, 1.f);
                     }
                 }
             } else {
@@ -601,70 +596,474 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
     }
 }
 
-// grid (ranges, blocks of rows): joins the pieces of the column that starts in
-// a range and goes on in the next: M = max m_i, out = sum 2^(m_i - M) o_i / sum
-// 2^(m_i - M) l_i.  Four warps to a (node, head) row, each every fourth piece,
-// hd / 32 dims a lane, joined in a fixed order.
-constexpr int kMergeRows = 4, kMergeThreads = kMergeRows * 128;
-template <typename T, int HD, int TK>
-__global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constant__ TreeArgs a) {
-    constexpr int D = HD / 32;
-    __shared__ float s_o[kMergeRows][4][HD], s_s[kMergeRows][4];
+// ---------------------------------------------------------------- narrow trees: mma.sync
+//
+// Up to 32 (node, head) rows, as single tokens and small drafts have, where a
+// 128-row tensor-memory tile would run nearly empty and its set-up would not
+// pay: small CTAs, several to an SM, that hide one another's waits.  Tiles of
+// 64 cached rows; S^T = K Q^T and O^T = V^T P^T with the cached rows (and
+// dims) as the 16-row operand and the query rows as the 8-column one, so NT
+// tiles of 8 columns waste little on 4 or 20 rows.  Warp w takes the 16 keys
+// of the tile's page w, then hd / 4 dims of O^T over all keys: the output needs
+// no join between warps, and P^T crosses between them as operand fragments (by
+// 8x8 transposes in registers, then shared memory).  K's next tile is copied
+// while this one's V is multiplied, and V's while the next scores are made, so
+// one buffer each is enough.  The terms of fp32 queries and probabilities and
+// the lagging maximum are those of the wide form.
+constexpr int kTnWarps = 4, kTnThreads = kTnWarps * 32, kTnK = 64;
+
+template <typename T, int HD, int NT>
+__host__ __device__ constexpr int tn_qbytes() { return tt_qterms<T>() * (HD / 16) * NT * 256; }
+template <typename T, int HD, int NT>
+__host__ __device__ constexpr size_t tn_smem() {
+    return (size_t)2 * kTnK * HD * 2 + tn_qbytes<T, HD, NT>() + (size_t)tt_pterms<T>() * 4 * NT * 256;
+}
+
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(p)
+                 : "memory");
+}
+__device__ __forceinline__ void ldm4t(uint32_t (&r)[4], uint32_t p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(p)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t mat_t(uint32_t x) {  // 8x8 transpose of bf16 pairs across the warp
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+template <typename T, int HD, int NT>
+__global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_constant__ TreeArgs a) {
+    constexpr int QT = tt_qterms<T>(), PT = tt_pterms<T>(), CH = HD / 8, KS = HD / 16, MT = HD / 64, ROW = HD * 2;
+    constexpr int RPI = kTnThreads / CH, NI = kTnK / RPI;  // rows a copy step covers, steps a tile
+    extern __shared__ __align__(128) uint8_t dsm[];
+    __shared__ int s_scan[kTnWarps], s_start[4];
+    __shared__ int8_t s_up[kTreeMax];
+    __shared__ float s_mx[kTnWarps][NT * 8];
+    __shared__ unsigned long long s_bad;
+    uint8_t *bk = dsm, *bv = dsm + kTnK * ROW;
+    uint2 *qf = (uint2 *)(bv + kTnK * ROW);    // Q fragments [term][16 dims][8 rows][lane]
+    uint2 *pf = qf + QT * KS * NT * 32;        // P fragments [term][page][8 rows][lane]
+    const int th = threadIdx.x, warp = th >> 5, lane = th & 31, g = lane >> 2, tq = lane & 3, range = blockIdx.x;
+    pdl_trigger();
     pdl_wait();
-    const int4 root = a.roots[blockIdx.x];
-    if (root.x < 0) return;
-    const int lane = threadIdx.x & 31, row = threadIdx.x >> 7, part = (threadIdx.x >> 5) & 3;
-    int L, t0, n;
-    tree_span(a.v, a.len, a.off, a.max_nodes, root.x, L, t0, n);
-    const int T_ = TreeWalk<TK>::tiles(L, n, a.v.page_max * kPageRows), C = root.w;
-    const int p0 = root.z / C, p1 = (root.z + T_ - 1) / C, rows = n * a.G;
-    for (int r0 = blockIdx.y * kMergeRows; r0 < rows; r0 += gridDim.y * kMergeRows) {
-        const int r = r0 + row, node = r / a.G, rb = r >> 7, lr = r & 127;
-        const auto piece = [&](int p) { return (size_t)((2 * p + (p * C < root.z)) * a.row_blocks + rb); };
-        float M = -INFINITY, S = 0.f, o[D];
+    tree_plan<kTnK, 1>(a, range, s_scan, s_start);
+    if (th == 0) {
+        a.roots[range] = make_int4(-1, 0, 0, 0);
+        s_bad = 0;
+    }
+    const int cap = a.v.page_max * kPageRows;
+    const float sl2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);
+    TreeWalk<kTnK> wi = tree_walk<kTnK>(s_start, range), wc = wi;
+    bool more = wi.next(a, 0);
+    int it = more ? wi.s_a : 0;  // the tile to copy next, of column wi
+    int pgs[kTnK / kPageRows];   // its pages
+    auto pages = [&]() {
 #pragma unroll
-        for (int d = 0; d < D; d++) o[d] = 0.f;
-        const int d0 = lane * D;
-        if (r < rows) {
+        for (int i = 0; i < kTnK / kPageRows; i++) {
+            pgs[i] = -1;
+            if (more && it * kTnK + i * kPageRows < wi.L + wi.n) pgs[i] = a.v.page(wi.s_slot, it * kTnK + i * kPageRows);
+        }
+    };
+    // K (kv = 0) or V rows of that tile; rows that do not exist become zeros
+    auto copy = [&](int kv) {
+        if (more) {
+            const int c = th % CH, r0 = th / CH, end = min(wi.L + wi.n, cap) - it * kTnK;
+            const uint32_t dst = kv_smem(kv ? bv : bk);
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int r = r0 + i * RPI, pg = pgs[(i * RPI) / kPageRows];
+                const uint16_t *p = a.v.kv + a.v.row(a.layer, max(pg, 0), r) + (long long)kv * kPageRows * a.v.kvd + wi.s_kvh * HD + c * 8;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + r * ROW + ((c ^ (r & 7)) << 4)), "l"(p),
+                             "r"(pg >= 0 && r < end ? 16 : 0)
+                             : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    pages();
+    copy(0);
+    copy(1);
+    while (wc.next(a, 0)) {
+        const int rows = wc.n << a.lg, end = min(wc.L + wc.n, cap);
+        // parents, and the queries as B fragments: lane (g, t) holds row g, dims 2t, 2t + 1, 2t + 8, 2t + 9 of 16
+        if (th < kTreeMax) s_up[th] = (int8_t)tree_parent(a, wc.t0, wc.n, th);
+        unsigned dead = 0;  // bit 2 nt + j: this lane's row is a padding node's
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int row = nt * 8 + 2 * tq + j;
+                if (row < rows && __ldg(a.parent + wc.t0 + (row >> a.lg)) == -2) dead |= 1u << (2 * nt + j);
+            }
+        {
+            const T *q0 = (const T *)a.q + (long long)wc.t0 * a.q_ld + (long long)wc.s_kvh * a.G * HD + 2 * tq;
+            const float sg = a.scale < 0.f ? -1.f : 1.f;
+            constexpr int NF = KS * NT / kTnWarps;
+            float2 x[NF][2];
+#pragma unroll
+            for (int f = 0; f < NF; f++) {
+                const int k = (f * kTnWarps + warp) / NT, nt = (f * kTnWarps + warp) % NT, r = nt * 8 + g;
+                const T *q = q0 + (long long)(r >> a.lg) * a.q_ld + (r & (a.G - 1)) * HD + k * 16;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    x[f][h] = make_float2(0.f, 0.f);
+                    if (r < rows) {
+                        if constexpr (sizeof(T) == 4) {
+                            x[f][h] = *(const float2 *)(q + h * 8);
+                        } else {
+                            const uint32_t u = *(const uint32_t *)(q + h * 8);
+                            x[f][h] = make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int f = 0; f < NF; f++) {
+                uint32_t b0[QT], b1[QT];
+                split_bf16<QT>(x[f][0].x * sg, x[f][0].y * sg, b0);
+                split_bf16<QT>(x[f][1].x * sg, x[f][1].y * sg, b1);
+#pragma unroll
+                for (int i = 0; i < QT; i++) qf[(i * KS * NT + f * kTnWarps + warp) * 32 + lane] = make_uint2(b0[i], b1[i]);
+            }
+        }
+        // O^T: o[mt][nt] = {(dim g, row 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1)} of 16 dims x 8 rows
+        float o[MT][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.f;
+        }
+        for (int t = wc.s_a; t < wc.s_b; t++) {
+            const int r0 = t * kTnK;
+            const bool tail = r0 + kTnK > wc.L;
+            if (++it == wi.s_b) {  // the copies' next tile, and its pages on their way
+                more = wi.next(a, 0);
+                it = wi.s_a;
+            }
+            pages();
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            __syncthreads();  // K and Q are there
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+            if (r0 + warp * 16 < end) {
+                const int kr = warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+                const uint32_t sk = kv_smem(bk) + kr * ROW;
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    uint32_t ka[4];
+                    ldm4(ka, sk + (((2 * k + (lane >> 4)) ^ (kr & 7)) << 4));
+#pragma unroll
+                    for (int i = QT - 1; i >= 0; i--)  // small terms first
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            const uint2 b = qf[((i * KS + k) * NT + nt) * 32 + lane];
+                            mma_16816(s[nt], ka, b.x, b.y);
+                        }
+                }
+            }
+            bool grow = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    unsigned long long mk = 0;
+                    const int row = nt * 8 + 2 * tq + j;
+                    if (tail && row < rows) mk = tree_mask(s_up, row >> a.lg);
+                    const bool hide = (dead >> (2 * nt + j)) & 1;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float x = s[nt][2 * h + j] * sl2;
+                        const int r = r0 + warp * 16 + g + h * 8;
+                        if (hide || (tail && !(r < wc.L || (r < end && ((mk >> (r - wc.L)) & 1))))) x = -INFINITY;
+                        s[nt][2 * h + j] = x;
+                        grow |= x > m[nt][j] + 8.f;
+                    }
+                }
+            if (bar_or(1, kTnThreads, grow)) {  // K has been read by all; does any maximum move?
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        float x = fmaxf(s[nt][j], s[nt][2 + j]);
+#pragma unroll
+                        for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+                        if (g == 0) s_mx[warp][nt * 8 + 2 * tq + j] = x;
+                    }
+                __syncthreads();
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int row = nt * 8 + 2 * tq + j;
+                        const float x = fmaxf(fmaxf(s_mx[0][row], s_mx[1][row]), fmaxf(s_mx[2][row], s_mx[3][row]));
+                        const float mn = x > m[nt][j] + 8.f ? x : m[nt][j], f = m[nt][j] == -INFINITY ? 1.f : ex2(m[nt][j] - mn);
+                        m[nt][j] = mn;
+                        l[nt][j] *= f;
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            o[mt][nt][j] *= f;
+                            o[mt][nt][2 + j] *= f;
+                        }
+                    }
+            }
+            copy(0);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float p[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) p[j] = ex2(s[nt][j] - (m[nt][j & 1] == -INFINITY ? 0.f : m[nt][j & 1]));
+                l[nt][0] += p[0] + p[2];
+                l[nt][1] += p[1] + p[3];
+                uint32_t x[PT], y[PT];
+                split_bf16<PT>(p[0], p[1], x);
+                split_bf16<PT>(p[2], p[3], y);
+#pragma unroll
+                for (int i = 0; i < PT; i++) pf[((i * 4 + warp) * NT + nt) * 32 + lane] = make_uint2(mat_t(x[i]), mat_t(y[i]));
+            }
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            __syncthreads();  // P and V are there
+            if (tail) {
+                // drafted rows whose V is not finite become zeros; the nodes
+                // that see them add them at the end
+                for (int r = max(wc.L - r0, 0) + warp; r < min(end - r0, kTnK); r += kTnWarps) {
+                    bool x = false;
+                    uint4 *p = (uint4 *)(bv + r * ROW + (lane % CH) * 16);
+                    if (lane < CH) {
+                        const uint4 u = *p;
+                        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) x |= (w[k] & 0x7f80u) == 0x7f80u || (w[k] & 0x7f800000u) == 0x7f800000u;
+                    }
+                    if (__any_sync(0xffffffffu, x)) {
+                        if (lane < CH) *p = make_uint4(0, 0, 0, 0);
+                        if (lane == 0) atomicOr(&s_bad, 1ull << (r0 + r - wc.L));
+                    }
+                }
+                __syncthreads();
+            }
+            const int vr = (lane & 7) + (lane >> 4) * 8;
+            const uint32_t sv = kv_smem(bv) + vr * ROW;
+#pragma unroll
+            for (int ks = 0; ks < kTnK / 16; ks++) {
+                if (r0 + ks * 16 >= end) break;
+                uint32_t va[MT][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+                    ldm4t(va[mt], sv + ks * 16 * ROW + (((2 * (warp * MT + mt) + ((lane >> 3) & 1)) ^ (vr & 7)) << 4));
+#pragma unroll
+                for (int i = PT - 1; i >= 0; i--)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        const uint2 b = pf[((i * 4 + ks) * NT + nt) * 32 + lane];
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) mma_16816(o[mt][nt], va[mt], b.x, b.y);
+                    }
+            }
+            __syncthreads();  // P and V have been read
+            copy(1);
+        }
+        // the rows' sums: a warp's lanes, then the four warps
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+#pragma unroll
+                for (int w = 4; w < 32; w <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], w);
+                if (g == 0) s_mx[warp][nt * 8 + 2 * tq + j] = l[nt][j];
+            }
+        __syncthreads();
+        for (unsigned long long bad = s_bad; bad; bad &= bad - 1) {  // rare: p_r v_r of the rows left out above
+            const int j = __ffsll((long long)bad) - 1, pg = a.v.page(wc.s_slot, wc.L + j);
+            if (pg < 0) continue;
+            const uint16_t *kr = a.v.kv + a.v.row(a.layer, pg, wc.L + j) + wc.s_kvh * HD, *vr = kr + kPageRows * a.v.kvd;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+                for (int c = 0; c < 8 && nt * 8 + c < rows; c++) {
+                    const int row = nt * 8 + c;
+                    if (!((tree_mask(s_up, row >> a.lg) >> j) & 1)) continue;
+                    const T *q = (const T *)a.q + (long long)(wc.t0 + (row >> a.lg)) * a.q_ld +
+                                 (long long)(wc.s_kvh * a.G + (row & (a.G - 1))) * HD;
+                    float x = 0.f;
+                    for (int d = lane; d < HD; d += 32) x = fmaf((float)q[d], bf16_bits_to_f32(kr[d]), x);
+                    x = warp_sum(x);
+                    if ((c >> 1) != tq) continue;
+                    const float p = ex2((a.scale < 0.f ? -x : x) * sl2 - (c & 1 ? m[nt][1] : m[nt][0]));
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        const int d = (warp * MT + mt) * 16 + g;
+                        const float v0 = p * bf16_bits_to_f32(vr[d]), v1 = p * bf16_bits_to_f32(vr[d + 8]);
+                        if (c & 1) {
+                            o[mt][nt][1] += v0;
+                            o[mt][nt][3] += v1;
+                        } else {
+                            o[mt][nt][0] += v0;
+                            o[mt][nt][2] += v1;
+                        }
+                    }
+                }
+        }
+        const bool whole = wc.s_a == 0 && wc.s_b == wc.T;
+        const size_t piece = (size_t)2 * range + (wc.s_g != wc.g0);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int row = nt * 8 + 2 * tq + j;
+                if (row >= rows) continue;
+                const int tok = wc.t0 + (row >> a.lg), head = wc.s_kvh * a.G + (row & (a.G - 1));
+                const float L = (s_mx[0][row] + s_mx[1][row]) + (s_mx[2][row] + s_mx[3][row]);
+                if (whole) {
+                    const float inv = L == 0.f ? 0.f : 1.0f / L;
+                    T *dst = (T *)a.out + (long long)tok * a.out_ld + (long long)head * HD + warp * MT * 16 + g;
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        dst[mt * 16] = (T)(o[mt][nt][j] * inv);
+                        dst[mt * 16 + 8] = (T)(o[mt][nt][2 + j] * inv);
+                    }
+                    if (a.lse && g == 0 && warp == 0)
+                        a.lse[(long long)tok * a.heads + head] = L == 0.f ? -INFINITY : (m[nt][j] + log2f(L)) * 0.6931471805599453f;
+                } else {
+                    float *dst = a.part_o + (piece * (NT * 8) + row) * HD + warp * MT * 16 + g;
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        dst[mt * 16] = o[mt][nt][j];
+                        dst[mt * 16 + 8] = o[mt][nt][2 + j];
+                    }
+                    if (g == 0 && warp == 0) a.part_ml[piece * (NT * 8) + row] = make_float2(m[nt][j], L);
+                }
+            }
+        if (th == 0 && wc.s_a == 0 && !whole) a.roots[range] = make_int4(wc.s_slot, wc.s_kvh, wc.s_g, s_start[3]);
+        __syncthreads();
+        if (th == 0) s_bad = 0;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// ---------------------------------------------------------------- joining the pieces
+//
+// For the columns that start in one range and go on in the next: M = max m_i,
+// out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i over the pieces in order.  A
+// warp takes a (node, head) row, hd / 32 dims a lane, of a work list over all
+// such columns.  Pieces of the narrow form are `rows_per` rows of HD values;
+// those of the wide one (rows_per = 0) [8 dims][128 rows][8].
+constexpr int kMergeThreads = 256;
+template <typename T, int HD, int TK>
+__global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constant__ TreeArgs a, int rows_per) {
+    constexpr int D = HD / 32, W = kMergeThreads / 32;
+    __shared__ int s_scan[W];
+    __shared__ int4 s_root[W];
+    __shared__ int s_row[W];
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // rows of the columns that start in this thread's ranges
+    int sum = 0, total = 0;
+    const int per = (a.ranges + kMergeThreads - 1) / kMergeThreads, b0 = min(a.ranges, (int)threadIdx.x * per), b1 = min(a.ranges, b0 + per);
+    const auto count = [&](const int4 &root) {
+        if (root.x < 0) return 0;
+        int L, t0, n;
+        tree_span(a.v, a.len, a.off, a.max_nodes, root.x, L, t0, n);
+        return n * a.G;
+    };
+#pragma unroll 8
+    for (int i = b0; i < b1; i++) sum += count(a.roots[i]);
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) s_scan[warp] = incl;
+    __syncthreads();
+    int before = incl - sum;
+    for (int i = 0; i < W; i++) {
+        if (i < warp) before += s_scan[i];
+        total += s_scan[i];
+    }
+    for (int row0 = blockIdx.x * W; row0 < total; row0 += gridDim.x * W) {
+        // the CTA's next W rows: whoever's ranges hold one says so
+        if (before < row0 + W && before + sum > row0) {
+            int at = before;
+            for (int i = b0; i < b1; i++) {
+                const int4 root = a.roots[i];
+                const int c = count(root);
+                for (int x = max(at, row0); x < min(at + c, row0 + W); x++) {
+                    s_root[x - row0] = root;
+                    s_row[x - row0] = x - at;
+                }
+                at += c;
+            }
+        }
+        __syncthreads();
+        if (row0 + warp < total) {
+            const int4 root = s_root[warp];
+            const int r = s_row[warp], node = r / a.G;
+            int L, t0, n;
+            tree_span(a.v, a.len, a.off, a.max_nodes, root.x, L, t0, n);
+            const int T_ = TreeWalk<TK>::tiles(L, n, a.v.page_max * kPageRows), C = root.w;
+            const int p0 = root.z / C, p1 = (root.z + T_ - 1) / C, d0 = lane * D;
+            const auto piece = [&](int p) { return (size_t)2 * p + (p * C < root.z); };
+            const auto ml_at = [&](int p) {
+                return rows_per ? a.part_ml[piece(p) * rows_per + r] : a.part_ml[(piece(p) * a.row_blocks + (r >> 7)) * 128 + (r & 127)];
+            };
+            float M = -INFINITY;
             for (int p = p0 + lane; p <= p1; p += 32) {
-                const float2 ml = a.part_ml[piece(p) * 128 + lr];
+                const float2 ml = ml_at(p);
                 if (ml.y != 0.f) M = fmaxf(M, ml.x);
             }
             M = warp_max(M);
-#pragma unroll 4
-            for (int p = p0 + part; p <= p1; p += 4) {
-                const size_t pc = piece(p);
-                const float2 ml = a.part_ml[pc * 128 + lr];
-                const float *po = a.part_o + pc * 128 * HD + (d0 >> 3) * 1024 + lr * 8 + (d0 & 7);
-                float v[D];
-                if constexpr (D == 4) {
-                    const float4 x = *(const float4 *)po;
-                    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-                } else {
-                    const float2 x = *(const float2 *)po;
-                    v[0] = x.x, v[1] = x.y;
+            float S = 0.f, o[D];
+#pragma unroll
+            for (int d = 0; d < D; d++) o[d] = 0.f;
+            for (int q0 = p0; q0 <= p1; q0 += 8) {  // eight pieces in flight
+                float v[8][D];
+                float2 ml[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    ml[i] = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int d = 0; d < D; d++) v[i][d] = 0.f;
+                    if (q0 + i > p1) continue;
+                    ml[i] = ml_at(q0 + i);
+                    const float *po = rows_per ? a.part_o + (piece(q0 + i) * rows_per + r) * HD + d0
+                                               : a.part_o + (piece(q0 + i) * a.row_blocks + (r >> 7)) * 128 * HD + (d0 >> 3) * 1024 +
+                                                     (r & 127) * 8 + (d0 & 7);
+                    if constexpr (D == 4) {
+                        const float4 x = *(const float4 *)po;
+                        v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+                    } else {
+                        const float2 x = *(const float2 *)po;
+                        v[i][0] = x.x, v[i][1] = x.y;
+                    }
                 }
-                const float f = ml.y == 0.f ? 0.f : ex2(ml.x - M);  // 0: nothing seen in this piece
-                S = fmaf(ml.y, f, S);
 #pragma unroll
-                for (int d = 0; d < D; d++) o[d] = fmaf(v[d], f, o[d]);
+                for (int i = 0; i < 8; i++) {
+                    const float f = ml[i].y == 0.f ? 0.f : ex2(ml[i].x - M);  // 0: nothing seen in this piece
+                    S = fmaf(ml[i].y, f, S);
+#pragma unroll
+                    for (int d = 0; d < D; d++) o[d] = fmaf(v[i][d], f, o[d]);
+                }
             }
-        }
-#pragma unroll
-        for (int d = 0; d < D; d++) s_o[row][part][d0 + d] = o[d];
-        if (lane == 0) s_s[row][part] = S;
-        __syncthreads();
-        if (part == 0 && r < rows) {
-            S = (s_s[row][0] + s_s[row][1]) + (s_s[row][2] + s_s[row][3]);
             const float inv = S == 0.f ? 0.f : 1.0f / S;
-#pragma unroll
-            for (int d = 0; d < D; d++)
-                o[d] = ((s_o[row][0][d0 + d] + s_o[row][1][d0 + d]) + (s_o[row][2][d0 + d] + s_o[row][3][d0 + d])) * inv;
             const int tok = t0 + node, head = root.y * a.G + r % a.G;
             T *dst = (T *)a.out + (long long)tok * a.out_ld + (long long)head * HD + d0;
-            if constexpr (D == 4) st_row4(dst, o[0], o[1], o[2], o[3]);
-            else if constexpr (sizeof(T) == 4) *(float2 *)dst = make_float2(o[0], o[1]);
-            else *(uint32_t *)dst = pack_bf16(o[0], o[1]);
+            if constexpr (D == 4) st_row4(dst, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+            else if constexpr (sizeof(T) == 4) *(float2 *)dst = make_float2(o[0] * inv, o[1] * inv);
+            else *(uint32_t *)dst = pack_bf16(o[0] * inv, o[1] * inv);
             if (a.lse && lane == 0) a.lse[(long long)tok * a.heads + head] = S == 0.f ? -INFINITY : (M + log2f(S)) * 0.6931471805599453f;
         }
         __syncthreads();

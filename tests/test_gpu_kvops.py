@@ -160,6 +160,16 @@ def test_tree_attention_shapes_of_trees(bf16):
     check_tree(rng, 2, 4, 128, bf16, [70, 33, 50, 0, 9, 64, 12], trees)
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("G,n", [(1, 32), (4, 8), (4, 5), (8, 4), (4, 40), (1, 60)])
+def test_tree_attention_padding_over_long_caches(G, n, hd, bf16):
+    """Padding nodes see no row of a cache of several tiles either, and one-node trees stand beside them."""
+    rng = np.random.default_rng(G + n + hd)
+    trees = [random_tree(rng, n, pad=n // 2), random_tree(rng, 1), np.full(n, -2), random_tree(rng, n - 1, pad=1)]
+    check_tree(rng, 2, G, hd, bf16, [700, 300, 511, 64], trees, max_nodes=n)
+
+
 def test_tree_attention_many_ragged_slots():
     rng = np.random.default_rng(8)
     lens = [int(x) for x in rng.integers(0, 400, 90)]
