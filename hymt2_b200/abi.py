@@ -123,6 +123,11 @@ SIGNATURES = {
     "hyc_trace": (I, [P, I]),
     "hyc_trace_read": (I, [P, P, I]),
     "hyc_attention_decode_noalloc": (I, [P, I, I, I, I, P, F, P, P, P, P, P, P, P, P, C.c_char_p, I]),
+    "hyc_tree_prepare": (I, [P, I, I]),
+    "hyc_tree_open": (I, [P, I, I]),
+    "hyc_tree_forward": (I, [P, P, P, P, P, I, P, P, P]),
+    "hyc_tree_evict": (I, [P, I, I, I]),
+    "hyc_tree_state": (I, [P, I, P, P, P]),
     "hyc_kvops_timeouts": (I, []),
     "hyc_tree_attention_ws": (Z, [KV, I, I]),
     "hyc_tree_attention": (I, [P, KV, I, I, I, P, P, P, P, LL, I, F, P, LL, P, P, Z, C.c_char_p, I]),

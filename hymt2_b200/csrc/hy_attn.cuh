@@ -42,6 +42,7 @@ struct AttnArgs {
     // pages[slot * page_max + pos / kPageRows], page_stride elements per page
     // (kc / vc: page 0's K / V rows of this layer)
     const int *tok_pos, *tok_slot;
+    const int *tok_row;     // cache row of token t where it is not its position (drafted trees)
     const int *pages;
     int page_max;
     long long page_stride;
@@ -97,7 +98,7 @@ __global__ void rope_norm_store(const __grid_constant__ AttnArgs a) {
     // the grid strides over the tokens (a few CTAs per SM, not one per token)
     for (int t = blockIdx.x; t < a.nt; t += gridDim.x) {
     const int pos = attn_tok_pos(a, t);
-    const long long kvr = attn_kv_row(a, attn_tok_slot(a, t), pos);
+    const long long kvr = attn_kv_row(a, attn_tok_slot(a, t), a.tok_row ? a.tok_row[t] : pos);
     const float *cs = a.rope_cos + (size_t)pos * a.half, *sn = a.rope_sin + (size_t)pos * a.half;
     float *row = a.qkv + (size_t)t * a.qkv_ld;
     for (int hh = w; hh < a.heads + a.kv_heads; hh += blockDim.x >> 5) {

@@ -748,6 +748,9 @@ struct Fwd {
     const int *tok_pos, *tok_slot;
     const int *qblk;              // batch: attention query blocks (first token, count)
     int nqb;
+    const int *tok_row;           // drafted trees: cache row of token t
+    bool tree;                    // their attention (hy_tree.cuh)
+    size_t qkv_stride;            // q | k | v of layer li at qkv + li * qkv_stride (0: one buffer for all)
 };
 
 Fwd fwd_single(HyCtx *c, const int *pos_ptr) {
@@ -765,6 +768,8 @@ Fwd fwd_single(HyCtx *c, const int *pos_ptr) {
     f.pos_ptr = pos_ptr;
     return f;
 }
+
+bool tree_attention(HyCtx *c, const Fwd &f, const AttnArgs &aa, int li, int nt, bool pdl);
 
 bool gateup_forward(HyCtx *c, const Fwd &f, const Layer &L, int nt, bool pdl) {
     GemvArgs a = gemv_args(nt, c->H);
@@ -841,7 +846,7 @@ bool layer_forward(HyCtx *c, const Fwd &f, int li, int nt, bool pdl) {
     // whose o_proj runs on the tensor cores: the attention kernel writes the
     // GEMM's tiled Q8_K input itself (whole blocks: G * hd a multiple of 256)
     HyWeight *wo[1] = {L.o};
-    const bool fuse_oq = f.tok_slot && f.qblk && f.nqb == nt && L.o->k == c->qd &&
+    const bool fuse_oq = !f.tree && f.tok_slot && f.qblk && f.nqb == nt && L.o->k == c->qd &&
                          ((c->heads / c->kvh) * c->hd) % 256 == 0 && tc_usable(c, nt, wo, 1);
     {
         HyWeight *ws[3] = {L.q, L.k, L.v};
@@ -903,7 +908,8 @@ bool layer_forward(HyCtx *c, const Fwd &f, int li, int nt, bool pdl) {
             aa.tcad = c->d_tcad;
             aa.tc_nb = c->qd / 256;
         }
-        if (!attention(c, aa, nt, pdl)) return false;
+        aa.tok_row = f.tok_row;
+        if (f.tree ? !tree_attention(c, f, aa, li, nt, pdl) : !attention(c, aa, nt, pdl)) return false;
     }
     {
         // tensor parallelism: the rank's partial product, then h += the sum over ranks
@@ -962,8 +968,11 @@ bool head_forward(HyCtx *c, const float *x, bool store_logits, bool argmax, bool
 }
 
 bool layers_forward(HyCtx *c, const Fwd &f, int nt, bool pdl) {
-    for (int li = 0; li < c->L; li++)
-        if (!layer_forward(c, f, li, nt, pdl)) return false;
+    Fwd fl = f;
+    for (int li = 0; li < c->L; li++) {
+        fl.qkv = f.qkv + li * f.qkv_stride;
+        if (!layer_forward(c, fl, li, nt, pdl)) return false;
+    }
     return true;
 }
 
@@ -1656,6 +1665,7 @@ bool fused_forward(void *impl, hy_fused_args *a) {
 }
 
 #include "hy_batch.cuh"
+#include "hy_tree.cuh"
 
 // Failure-detection probe: the bounded waits of the persistent decode kernel
 // (grid barrier on its arrival counter) and of the tensor-core GEMM (an
@@ -1947,6 +1957,71 @@ HYC_API int hyc_batch_kv_read(void *impl, int slot, int layer, int npos, uint16_
         if (cudaMemcpyAsync(k + o, kc, bytes, cudaMemcpyDeviceToHost, c->st) != cudaSuccess ||
             cudaMemcpyAsync(v + o, vc, bytes, cudaMemcpyDeviceToHost, c->st) != cudaSuccess)
             return -1;
+    }
+    return cudaStreamSynchronize(c->st) == cudaSuccess ? 0 : -1;
+}
+
+HYC_API int hyc_tree_prepare(void *impl, int max_nodes, int weights) {
+    HyCtx *c = (HyCtx *)impl;
+    if (!c || c->broken || !c->bat || cudaSetDevice(c->dev) != cudaSuccess) return -1;
+    return tree_prepare(c, max_nodes, weights != 0) ? 0 : -1;
+}
+
+HYC_API int hyc_tree_open(void *impl, int slot, int rows) {
+    HyCtx *c = (HyCtx *)impl;
+    if (!c || c->broken || !c->bat || !c->bat->tree || cudaSetDevice(c->dev) != cudaSuccess) return -1;
+    Batch &b = *c->bat;
+    if (slot < 0 || slot >= b.slots || rows < 0 || rows > b.slot_ctx) return -1;
+    TreeState &t = *b.tree;
+    t.len[(size_t)slot] = t.pos[(size_t)slot] = rows;
+    if (t.acc) {  // no query of this sequence has been counted yet
+        const size_t col = (size_t)c->kvh * tree_rows(b) * 4;
+        if (cudaMemset2DAsync((char *)t.acc + slot * col, b.slots * col, 0, col, (size_t)c->L, c->st) != cudaSuccess) {
+            fail(c, "tree_open", cudaGetLastError());
+            return -1;
+        }
+    }
+    return 0;
+}
+
+HYC_API int hyc_tree_forward(void *impl, const int *tokens, const int *parent, const int *off, const int *forced, int vocab_out,
+                             int *accepted, int *path, int *next) {
+    HyCtx *c = (HyCtx *)impl;
+    if (!c || c->broken || !c->bat || !c->bat->tree || !tokens || !parent || !off || !accepted || !path || !next ||
+        cudaSetDevice(c->dev) != cudaSuccess)
+        return -1;
+    const int vo = vocab_out > 0 && vocab_out <= c->outw->n ? vocab_out : c->outw->n;
+    if (!tree_run(c, tokens, parent, off, forced, vo)) return -1;
+    const TreeState &t = *c->bat->tree;
+    const size_t S = (size_t)c->bat->slots;
+    const int *out = t.h_int + t.in_ints;
+    memcpy(accepted, out + S, S * 4);
+    memcpy(next, out + 2 * S, S * 4);
+    memcpy(path, out + 3 * S, S * t.max_nodes * 4);
+    return 0;
+}
+
+HYC_API int hyc_tree_evict(void *impl, int budget, int sinks, int recent) {
+    HyCtx *c = (HyCtx *)impl;
+    if (!c || c->broken || !c->bat || !c->bat->tree || cudaSetDevice(c->dev) != cudaSuccess) return -1;
+    return tree_evict(c, budget, sinks, recent) ? 0 : -1;
+}
+
+HYC_API int hyc_tree_state(void *impl, int slot, int *rows, int *pos, float *weights) {
+    HyCtx *c = (HyCtx *)impl;
+    if (!c || c->broken || !c->bat || !c->bat->tree || cudaSetDevice(c->dev) != cudaSuccess) return -1;
+    const Batch &b = *c->bat;
+    const TreeState &t = *b.tree;
+    if (slot < 0 || slot >= b.slots || (weights && !t.weights)) return -1;
+    if (rows) *rows = t.len[(size_t)slot];
+    if (pos) *pos = t.pos[(size_t)slot];
+    if (weights && t.len[(size_t)slot] > 0) {
+        const size_t R = (size_t)tree_rows(b) * 4, n = (size_t)t.len[(size_t)slot] * 4;
+        for (int l = 0; l < c->L; l++)
+            if (cudaMemcpy2DAsync(weights + (size_t)l * c->kvh * t.len[(size_t)slot], n,
+                                  (const char *)t.acc + ((size_t)l * b.slots + slot) * c->kvh * R, R, n, (size_t)c->kvh,
+                                  cudaMemcpyDeviceToHost, c->st) != cudaSuccess)
+                return -1;
     }
     return cudaStreamSynchronize(c->st) == cudaSuccess ? 0 : -1;
 }

@@ -26,6 +26,8 @@
 // recomputed for its logits.  When a prompt has been fed, its full pages are
 // sealed into the cache.
 
+struct TreeState;  // drafted trees and the bounded cache (hy_tree.cuh)
+
 struct Batch {
     int slots = 0, slot_ctx = 0, max_tokens = 0, max_out = 0;
     int page_max = 0;  // pages per slot: ceil(slot_ctx / kPageRows)
@@ -40,6 +42,8 @@ struct Batch {
     float *sel = nullptr;  // [max_out][H] residual rows for the head
     float *logits = nullptr;  // [max_out][vocab]
     int *d_ids = nullptr, *h_ids = nullptr;
+    TreeState *tree = nullptr;
+    bool in_tree = false;  // the pass being run is one of drafted trees
     long long page_stride(const HyCtx *c) const { return (long long)2 * kPageRows * c->kvd; }
     size_t layer_stride(const HyCtx *c) const { return (size_t)npages * page_stride(c); }
     size_t kv_elems(const HyCtx *c) const { return (size_t)c->L * layer_stride(c); }
@@ -106,9 +110,13 @@ __global__ void kv_copy_page(uint16_t *kv, size_t layer_stride, long long page_s
 
 // ---------------------------------------------------------------- host side
 
+void tree_free(Batch *b);
+void fwd_tree(HyCtx *c, Fwd &f);
+
 void batch_free(HyCtx *c) {
     Batch *b = c->bat;
     if (!b) return;
+    tree_free(b);
     cudaFree(b->kv);
     cudaFree(b->h);
     cudaFree(b->qkv);
@@ -190,6 +198,7 @@ Fwd fwd_batch(HyCtx *c) {
     f.tok_slot = b.slot();
     f.qblk = b.d_in + b.qblk_off();
     f.nqb = b.nqb;
+    if (b.in_tree) fwd_tree(c, f);
     return f;
 }
 

@@ -311,6 +311,7 @@ class DeviceModel:
         mo = slots if max_out is None else max_out
         if self.be.lib.hyc_batch_prepare(self.be.impl, slots, slot_ctx, max_tokens, mo) != 0:
             raise BackendError("batch_prepare: " + self.be.error())
+        self.batch_slots, self.batch_ctx, self.batch_tokens = slots, slot_ctx, max_tokens
         self.batch_vocab = self.g.tensors.get("output.weight", self.g.tensors["token_embd.weight"]).n
 
     def batch_forward(self, tokens, slots, positions, out_rows, want_logits: bool = False):
@@ -334,6 +335,55 @@ class DeviceModel:
         if self.be.lib.hyc_batch_kv_read(self.be.impl, slot, layer, npos, k.ctypes.data, v.ctypes.data) != 0:
             raise BackendError("batch_kv_read")
         return k.reshape(npos, kvd), v.reshape(npos, kvd)
+
+    # ---- drafted trees and a bounded cache
+    def tree_prepare(self, max_nodes: int, weights: bool = False) -> None:
+        if self.be.lib.hyc_tree_prepare(self.be.impl, max_nodes, int(weights)) != 0:
+            raise BackendError("tree_prepare: " + self.be.error())
+        self.tree_nodes = max_nodes
+
+    def tree_open(self, slot: int, rows: int) -> None:
+        """Slot holds rows 0 .. rows - 1 (batch_forward at those positions) and goes on from there."""
+        if self.be.lib.hyc_tree_open(self.be.impl, slot, rows) != 0:
+            raise BackendError("tree_open: " + (self.be.error() or "bad slot or rows"))
+
+    def tree_forward(self, trees, slots: int, forced=None):
+        """One pass over a tree of drafted tokens for each slot.
+
+        trees: {slot: (tokens, parents)}, node 0 the token the slot's sequence ends with (parent -1); forced: the
+        slots whose nodes are a given chain, all kept.  Returns {slot: (kept tokens, the model's next token)}."""
+        off = np.zeros(slots + 1, dtype=np.int32)
+        for s, (tk, _) in trees.items():
+            off[s + 1] = len(tk)
+        off = np.cumsum(off, dtype=np.int32)
+        order = sorted(trees)
+        tk = np.concatenate([np.asarray(trees[s][0], dtype=np.int32) for s in order])
+        pa = np.concatenate([np.asarray(trees[s][1], dtype=np.int32) for s in order])
+        if len(tk) != len(pa):
+            raise ValueError("a tree has as many parents as tokens")
+        fo = np.zeros(slots, dtype=np.int32)
+        fo[list(forced or ())] = 1
+        acc, nxt = np.zeros(slots, dtype=np.int32), np.zeros(slots, dtype=np.int32)
+        path = np.zeros((slots, self.tree_nodes), dtype=np.int32)
+        if self.be.lib.hyc_tree_forward(self.be.impl, tk.ctypes.data, pa.ctypes.data, off.ctypes.data, fo.ctypes.data,
+                                        self.vocab_out, acc.ctypes.data, path.ctypes.data, nxt.ctypes.data) != 0:
+            raise BackendError("tree_forward: " + self.be.error())
+        return {s: (tk[path[s, :acc[s]]].tolist(), int(nxt[s])) for s in order}
+
+    def tree_evict(self, budget: int, sinks: int, recent: int) -> None:
+        if self.be.lib.hyc_tree_evict(self.be.impl, budget, sinks, recent) != 0:
+            raise BackendError("tree_evict: " + self.be.error())
+
+    def tree_state(self, slot: int, weights: bool = False):
+        """(rows, next position, accumulated weights [layers][kv_heads][rows] or None) of a slot."""
+        rows, pos = C.c_int(), C.c_int()
+        rc = self.be.lib.hyc_tree_state(self.be.impl, slot, C.byref(rows), C.byref(pos), None)
+        w = np.zeros((self.hp.n_layer, self.hp.kv_heads, rows.value), dtype=np.float32) if weights else None
+        if rc == 0 and weights:
+            rc = self.be.lib.hyc_tree_state(self.be.impl, slot, None, None, w.ctypes.data)
+        if rc != 0:
+            raise BackendError("tree_state: " + (self.be.error() or "bad slot, or weights are not kept"))
+        return rows.value, pos.value, w
 
     def serve(self, prompts, max_new: int, step_tokens: int, stop=()):
         """Greedy generation for many requests with continuous batching.

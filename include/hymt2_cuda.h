@@ -204,6 +204,39 @@ HYC_API int hyc_serve(void *impl, const int *prompts, const int *prompt_off, int
                       const int *stop_ids, int n_stop, int vocab_out, int step_tokens, int *out_ids, int *out_len,
                       hyc_serve_stats *stats);
 
+/* ---- drafted trees and a bounded cache on the batch engine -------------
+ * (additive extension; the reference's loop feeds one token per step,
+ * src/model.c:943-954, and its cache only grows, :804-808).  After
+ * hyc_batch_prepare, with max_out >= the nodes of a pass:
+ * hyc_tree_prepare: trees of up to max_nodes (<= 64) nodes a slot; weights !=
+ * 0 also keeps the accumulated attention weights that eviction goes by.  All
+ * slots are empty.
+ * hyc_tree_open: slot holds rows 0 .. rows - 1, filled by hyc_batch_forward at
+ * positions 0 .. rows - 1, and goes on at position rows; its weights are zero.
+ * hyc_tree_forward: one pass.  Slot s gets the nodes off[s] .. off[s + 1] - 1
+ * (host arrays, off [slots + 1], off[0] = 0; no nodes leaves the slot as it
+ * is): node 0 is the token its sequence ends with (parent -1), every other
+ * node a guess that follows its parent (numbered within the tree, below the
+ * node).  accepted[s] nodes are kept: node 0 and the longest path on which
+ * every token is the model's own choice after the one before; path[s]
+ * [max_nodes] are their token numbers (-1 behind), next[s] the model's choice
+ * after the last of them, which is node 0 of the slot's next tree.  Slots with
+ * forced[s] != 0 (forced may be NULL) keep all their nodes, a given chain such
+ * as a prompt's last tokens.  The ids are those of one-token steps.
+ * hyc_tree_evict: every slot with more than budget rows keeps its first
+ * `sinks`, last `recent` and, in each layer and KV head, its heaviest other
+ * rows, budget in all; positions go on.
+ * hyc_tree_state: a slot's rows and next position, and (optional, where
+ * weights are kept) its weights [layers][kv_heads][rows].
+ * hyc_batch_kv_read reads the slot's rows.  All return 0 or -1
+ * (hyc_last_error). */
+HYC_API int hyc_tree_prepare(void *impl, int max_nodes, int weights);
+HYC_API int hyc_tree_open(void *impl, int slot, int rows);
+HYC_API int hyc_tree_forward(void *impl, const int *tokens, const int *parent, const int *off, const int *forced, int vocab_out,
+                             int *accepted, int *path, int *next);
+HYC_API int hyc_tree_evict(void *impl, int budget, int sinks, int recent);
+HYC_API int hyc_tree_state(void *impl, int slot, int *rows, int *pos, float *weights);
+
 /* ---- kernel-level hooks for parity tests (host buffers, synchronous) -- */
 
 /* Device Q8_K quantiser on x[nt][k]; writes full host blocks. */
