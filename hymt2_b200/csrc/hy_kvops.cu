@@ -100,6 +100,11 @@ bool raise_narrow(F raise) {
            raise((const void *)tree_attn_mma<T, HD, 3>, tn_smem<T, HD, 3>()) && raise((const void *)tree_attn_mma<T, HD, 4>, tn_smem<T, HD, 4>());
 }
 
+template <typename T, int HD, typename F>
+bool raise_wide(F raise) {
+    return raise((const void *)tree_attn_tc<T, HD, 64>, kTtSmem + 1024) && raise((const void *)tree_attn_tc<T, HD, 128>, kTtSmem + 1024);
+}
+
 // SMs of the current device, with the kernels' shared-memory limits raised on
 // its first use; 0 when there is no usable device.
 int device_sms() {
@@ -115,10 +120,8 @@ int device_sms() {
     const auto raise = [](const void *k, size_t b) {
         return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)b) == cudaSuccess;
     };
-    if (!raise((const void *)tree_attn_tc<float, 64>, tt_smem<float, 64>()) ||
-        !raise((const void *)tree_attn_tc<float, 128>, tt_smem<float, 128>()) ||
-        !raise((const void *)tree_attn_tc<__nv_bfloat16, 64>, tt_smem<__nv_bfloat16, 64>()) ||
-        !raise((const void *)tree_attn_tc<__nv_bfloat16, 128>, tt_smem<__nv_bfloat16, 128>()) ||
+    if (!raise_wide<float, 64>(raise) || !raise_wide<float, 128>(raise) || !raise_wide<__nv_bfloat16, 64>(raise) ||
+        !raise_wide<__nv_bfloat16, 128>(raise) ||
         !raise_narrow<float, 64>(raise) || !raise_narrow<float, 128>(raise) || !raise_narrow<__nv_bfloat16, 64>(raise) ||
         !raise_narrow<__nv_bfloat16, 128>(raise) ||
         !raise((const void *)cache_weights_tc<float, 64>, kWtSmem + 1024) ||
@@ -214,7 +217,7 @@ struct EvictArgs {
     float *acc_out;
 };
 
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 512;  // a quarter of the select's bins
 
 // Order-preserving key of an accumulated weight: NaN as -inf, -0 as 0.
 __device__ __forceinline__ uint32_t weight_key(float v) {
@@ -224,12 +227,19 @@ __device__ __forceinline__ uint32_t weight_key(float v) {
 }
 
 // grid (layers * slots * kv heads): the kept rows of one cache column, in
-// order.  A radix select over the candidates' 32-bit keys (8 bits a pass)
-// finds the lightest kept key T and how many rows equal to T stay; one ordered
-// pass then writes the rows that are forced, above T, or among those.
+// order.  A radix select over the candidates' 32-bit keys finds the lightest
+// kept key T and how many rows equal to T stay; one ordered pass then writes
+// the rows that are forced, above T, or among those.  Three passes of 11, 11
+// and 10 bits: the first one's bins hold the sign, the exponent and two more
+// bits, so that weights of a few magnitudes spread over many bins (by bytes,
+// nearly all fell into three, and their shared-memory additions into one
+// another: 47 us for 768 columns of 6100 rows).  A warp whose keys all fall
+// into one bin adds them once.
+constexpr int kSelBins = 2048;
 __global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constant__ EvictArgs a) {
-    __shared__ unsigned hist[256], wsum[2][kSelThreads / 32];
+    __shared__ unsigned hist[kSelBins], wsum[2][kSelThreads / 32];
     __shared__ unsigned s_prefix, s_need;
+    pdl_trigger();
     const int idx = blockIdx.x, kvh = idx % a.v.kvh, s = (idx / a.v.kvh) % a.v.slots, layer = idx / (a.v.kvh * a.v.slots);
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n = min(min(max(a.len[s], 0), a.acc_rows), a.v.page_max * kPageRows);
@@ -253,77 +263,106 @@ __global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constan
         s_prefix = 0;
         s_need = want;
     }
-    for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
-        for (int i = threadIdx.x; i < 256; i += kSelThreads) hist[i] = 0;
+    for (int pass = 0; pass < 3 && want > 0; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const unsigned bins = pass == 2 ? 1024 : 2048;
+        for (int i = threadIdx.x; i < kSelBins; i += kSelThreads) hist[i] = 0;
         __syncthreads();
-        const unsigned prefix = s_prefix, hmask = shift == 24 ? 0u : ~0u << (shift + 8);
-        for (int r = c0 + threadIdx.x; r < c1; r += kSelThreads) {
-            const uint32_t k = weight_key(acc[r]);
-            if ((k & hmask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (w == 0) {
-            // lane l: bins 255 - 8 l .. 248 - 8 l, counted from the heaviest
-            unsigned c[8], t = 0;
+        const unsigned prefix = s_prefix, need = s_need, above = pass == 0 ? 0u : pass == 1 ? ~0u << 21 : ~0u << 10;
+        for (int r0 = c0; r0 < c1; r0 += 4 * kSelThreads) {
+            float v[4];
 #pragma unroll
-            for (int i = 0; i < 8; i++) t += c[i] = hist[255 - 8 * lane - i];
-            unsigned incl = t;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += y;
+            for (int i = 0; i < 4; i++) {
+                const int r = r0 + i * kSelThreads + threadIdx.x;
+                v[i] = r < c1 ? acc[r] : 0.f;
             }
-            const unsigned need = s_need;
-            unsigned before = incl - t;
-            if (before < need && need <= incl) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if (before < need && need <= before + c[i]) {
-                        s_prefix = prefix | ((unsigned)(255 - 8 * lane - i) << shift);
-                        s_need = need - before;
-                        before = 0xffffffffu;
-                        break;
-                    }
-                    before += c[i];
+            for (int i = 0; i < 4; i++) {
+                const uint32_t k = weight_key(v[i]);
+                const bool in = r0 + i * kSelThreads + (int)threadIdx.x < c1 && (k & above) == prefix;
+                const unsigned bin = (k >> shift) & (bins - 1), who = __ballot_sync(0xffffffffu, in);
+                if (!who) continue;
+                const unsigned first = __shfl_sync(0xffffffffu, bin, __ffs(who) - 1);
+                if (__all_sync(0xffffffffu, !in || bin == first)) {
+                    if (lane == 0) atomicAdd(&hist[first], __popc(who));
+                } else if (in) {
+                    atomicAdd(&hist[bin], 1u);
                 }
             }
+        }
+        __syncthreads();
+        // thread t: bins 2047 - 4 t .. 2044 - 4 t, counted from the heaviest
+        unsigned c[4], t = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) t += c[i] = hist[kSelBins - 1 - 4 * threadIdx.x - i];
+        unsigned incl = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) wsum[0][w] = incl;
+        __syncthreads();
+        unsigned before = incl - t;
+        for (int i = 0; i < w; i++) before += wsum[0][i];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (before < need && need <= before + c[i]) {  // one bin of one thread
+                s_prefix = prefix | ((unsigned)(kSelBins - 1 - 4 * threadIdx.x - i) << shift);
+                s_need = need - before;
+            }
+            before += c[i];
         }
         __syncthreads();
     }
     __syncthreads();
     const unsigned T = s_prefix, need = want > 0 ? s_need : 0;
-    unsigned base = 0, ties = 0;  // kept and tied rows so far
-    for (int r0 = 0; r0 < n; r0 += kSelThreads) {
-        const int r = r0 + threadIdx.x;
-        const float v = r < n ? acc[r] : 0.f;
-        const bool cand = r >= c0 && r < c1;
+    // thread t owns a run of rows: it counts them, learns how many stand before
+    // them, and writes those that stay
+    const int run = (n + kSelThreads - 1) / kSelThreads, r0 = min(n, (int)threadIdx.x * run), r1 = min(n, r0 + run);
+    const auto kind = [&](int r, float v) {  // 1: stays, 2: tied, 0: goes
+        if (r < c0 || r >= c1) return 1;
+        if (want == 0) return 0;
         const uint32_t k = weight_key(v);
-        const bool sure = r < n && (!cand || (want > 0 && k > T)), tie = cand && want > 0 && k == T;
-        const unsigned bs = __ballot_sync(0xffffffffu, sure), bt = __ballot_sync(0xffffffffu, tie);
-        if (lane == 0) {
-            wsum[0][w] = __popc(bs);
-            wsum[1][w] = __popc(bt);
+        return k > T ? 1 : k == T ? 2 : 0;
+    };
+    unsigned sure = 0, tied = 0;
+#pragma unroll 4
+    for (int r = r0; r < r1; r++) {
+        const int k = kind(r, acc[r]);
+        sure += k == 1;
+        tied += k == 2;
+    }
+    unsigned is = sure, it = tied;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, is, o), z = __shfl_up_sync(0xffffffffu, it, o);
+        if (lane >= o) {
+            is += y;
+            it += z;
         }
-        __syncthreads();
-        unsigned ps = 0, pt = 0, as = 0, at = 0;
-        for (int i = 0; i < kSelThreads / 32; i++) {
-            if (i < w) {
-                ps += wsum[0][i];
-                pt += wsum[1][i];
-            }
-            as += wsum[0][i];
-            at += wsum[1][i];
+    }
+    if (lane == 31) {
+        wsum[0][w] = is;
+        wsum[1][w] = it;
+    }
+    __syncthreads();
+    unsigned bs = is - sure, bt = it - tied;  // rows before this run that stay for sure, and tied ones
+    for (int i = 0; i < w; i++) {
+        bs += wsum[0][i];
+        bt += wsum[1][i];
+    }
+#pragma unroll 4
+    for (int r = r0; r < r1; r++) {
+        const float v = acc[r];
+        const int k = kind(r, v);
+        if (k == 1 || (k == 2 && bt < need)) {
+            const unsigned j = bs + min(bt, need);
+            kept[j] = r;
+            acc_out[j] = v;
         }
-        const unsigned below = (1u << lane) - 1;
-        const unsigned tr = ties + pt + __popc(bt & below);               // this row's rank among the ties
-        const unsigned sr = base + ps + __popc(bs & below) + min(tr, need) - min(ties, need);
-        if (sure || (tie && tr < need)) {
-            kept[sr] = r;
-            acc_out[sr] = v;
-        }
-        base += as + min(ties + at, need) - min(ties, need);
-        ties += at;
-        __syncthreads();
+        bs += k == 1;
+        bt += k == 2;
     }
 }
 
@@ -334,6 +373,7 @@ __global__ void __launch_bounds__(256) evict_gather(const __grid_constant__ Evic
     const int idx = blockIdx.x, kvh = idx % a.v.kvh, s = (idx / a.v.kvh) % a.v.slots, layer = idx / (a.v.kvh * a.v.slots);
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n = min(min(min(max(a.len[s], 0), a.acc_rows), a.v.page_max * kPageRows), a.budget);
+    pdl_wait();  // the kept rows
     const int per = a.v.hd / 16;  // elements a lane moves: 8 or 4
     const long long col = (lane >> 4) * (long long)kPageRows * a.v.kvd + kvh * a.v.hd + (lane & 15) * per;
     for (int j = blockIdx.y * kGatherRows + w; j < min(n, (int)(blockIdx.y + 1) * kGatherRows); j += 8) {
@@ -471,7 +511,8 @@ HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer
     const dim3 grid(ws.ranges * ws.row_blocks);
 #define HY_TREE(T_, HD_)                                                                                                \
     {                                                                                                                   \
-        e = go(tree_attn_tc<T_, HD_>, grid, dim3(kTtThreads), tt_smem<T_, HD_>(), stream, false, a, map);                \
+        e = max_nodes * a.G <= 64 ? go(tree_attn_tc<T_, HD_, 64>, grid, dim3(kTtThreads), kTtSmem + 1024, stream, false, a, map) \
+                                  : go(tree_attn_tc<T_, HD_, 128>, grid, dim3(kTtThreads), kTtSmem + 1024, stream, false, a, map); \
         if (e == cudaSuccess) e = go(tree_merge<T_, HD_, kTtK>, mgrid, dim3(kMergeThreads), 0, stream, true, a, 0);       \
     }
     if (q_bf16) {
@@ -586,7 +627,7 @@ HYC_API int hyc_cache_evict(void *stream, const hyc_kv_view *cache, const hyc_kv
     if (cols > 0x7fffffff || budget > (1 << 21)) return op_fail(err, err_cap, -1, "cache or budget too large");
     cudaError_t e = go(evict_select, dim3((unsigned)cols), dim3(kSelThreads), 0, stream, false, a);
     if (e == cudaSuccess)
-        e = go(evict_gather, dim3((unsigned)cols, (budget + kGatherRows - 1) / kGatherRows), dim3(256), 0, stream, false, a);
+        e = go(evict_gather, dim3((unsigned)cols, (budget + kGatherRows - 1) / kGatherRows), dim3(256), 0, stream, true, a);
     return done(e, err, err_cap);
 }
 

@@ -159,6 +159,10 @@ __device__ __forceinline__ int tree_parent(const TreeArgs &a, int t0, int n, int
     const int p = i < n ? __ldg(a.parent + t0 + i) : -2;
     return p == -2 ? -2 : p < 0 || p >= i ? -1 : p;
 }
+// One segment of a walk, as the softmax warps share it.
+struct TreeSeg {
+    int have, slot, kvh, a, b, g, piece, L, t0, n, T;
+};
 // Bits of the nodes that node i sees: itself and its ancestors up to the root
 // or to a padding node.  Parents lie below their nodes, so the walk ends.
 __device__ __forceinline__ unsigned long long tree_mask(const int8_t *s_up, int i) {
@@ -221,24 +225,26 @@ template <typename T>
 __host__ __device__ constexpr int tt_pterms() { return sizeof(T) == 4 ? 3 : 2; }
 template <int HD>
 __host__ __device__ constexpr int tt_stage() { return (HD / 64) * 128 * 128; }
+// Shared memory: the Q terms of 64 or 128 rows (a product reads 128 rows from
+// there on, whatever lies behind, and the rows past the last are not used),
+// then K / V stages.  Beside it the kernel has at most 2 KB of static shared memory.
+constexpr int kTtSmem = 224 * 1024, kTtMaxSt = 8;
 template <typename T, int HD>
-__host__ __device__ constexpr int tt_qbytes() { return tt_qterms<T>() * tt_stage<HD>(); }
+__host__ __device__ constexpr int tt_qbytes(int qrows) { return tt_qterms<T>() * (HD / 64) * qrows * 128; }
 template <typename T, int HD>
-__host__ __device__ constexpr int tt_stages() {
-    const int s = (224 * 1024 - tt_qbytes<T, HD>()) / tt_stage<HD>();
-    return s > 8 ? 8 : s;
+__host__ __device__ constexpr int tt_stages(int qrows) {
+    const int s = (kTtSmem - ((tt_qbytes<T, HD>(qrows) + 1023) & ~1023)) / tt_stage<HD>();
+    return s > kTtMaxSt ? kTtMaxSt : s;
 }
-// Beside it the kernel has at most 2 KB of static shared memory.
-template <typename T, int HD>
-__host__ __device__ constexpr size_t tt_smem() { return (size_t)tt_qbytes<T, HD>() + (size_t)tt_stages<T, HD>() * tt_stage<HD>() + 1024; }
 
 // Tensor memory columns: S / P of tiles 2i and 2i + 1 (P's third term apart), O.
 constexpr uint32_t kTtS = 0, kTtO = 256, kTtX = 384;
 
-template <typename T, int HD>
+template <typename T, int HD, int QR>
 __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_constant__ TreeArgs a,
                                                               const __grid_constant__ CUtensorMap map) {
-    constexpr int QT = tt_qterms<T>(), PT = tt_pterms<T>(), NH = HD / 64, NST = tt_stages<T, HD>(), STB = tt_stage<HD>();
+    constexpr int QT = tt_qterms<T>(), PT = tt_pterms<T>(), NH = HD / 64, STB = tt_stage<HD>();
+    constexpr int NST = tt_stages<T, HD>(QR), QH = QR * 128, QTB = NH * QH;  // stages; bytes of a term's half, and of a term
     static_assert(NST >= 4, "K and V of two tiles in flight");
     extern __shared__ uint8_t dsm[];
     __shared__ __align__(8) uint64_t full[NST], empty[NST], sfull[2], pfull[2], odone[2], qfull, ofree, fin;
@@ -248,8 +254,10 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
     __shared__ unsigned long long s_bad[2][2];
     __shared__ float s_half[2][128];
     __shared__ int s_stop;
+    __shared__ TreeSeg s_seg[2];
+    __shared__ TreeWalk<kTtK> s_walk;  // the softmax warps' walk: in registers it would cost them spills
     uint8_t *sq = (uint8_t *)(((uintptr_t)dsm + 1023) & ~(uintptr_t)1023);
-    uint8_t *ring = sq + tt_qbytes<T, HD>();
+    uint8_t *ring = sq + ((QT * QTB + 1023) & ~1023);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rb = blockIdx.x % a.row_blocks, range = blockIdx.x / a.row_blocks;
     const int NB = 128 / a.G, node0 = rb * NB;  // nodes of a row block
@@ -289,6 +297,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
         // the end of the map, which fills zeros
         const int y0 = a.layer * a.v.npages * 2 * kPageRows, yend = a.v.layers * a.v.npages * 2 * kPageRows;
         int pos = 0;
+        RingPos at;
         while (w.next(a, node0)) {
             const int pages = (min(w.L + w.n, cap) + kPageRows - 1) / kPageRows;
             // the segment's queries towards L2: the softmax warps load them when
@@ -301,11 +310,11 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             }
             for (int t = w.s_a; t < w.s_b; t++) {
                 const int j = t * (kTtK / kPageRows) + (lane & 7);
-                int pg = j < pages ? __ldg(a.v.pages + (size_t)w.s_slot * a.v.page_max + j) : -1;
+                const int pg = j < pages ? __ldg(a.v.pages + (size_t)w.s_slot * a.v.page_max + j) : -1;
                 const int y = pg < 0 || pg >= a.v.npages ? yend : y0 + pg * 2 * kPageRows;
-                for (int kv = 0; kv < 2; kv++, pos++) {
-                    const int st = pos % NST, use = pos / NST;
-                    if (use > 0) mb_wait(&empty[st], (use - 1) & 1, &s_stop);
+                for (int kv = 0; kv < 2; kv++, pos++, at.next(NST)) {
+                    const int st = at.st;
+                    mb_wait(&empty[st], at.use ^ 1, &s_stop);  // passes on a stage's first use
                     if (__any_sync(0xffffffffu, *(volatile int *)&s_stop)) break;
                     int yj[8];
 #pragma unroll
@@ -332,11 +341,14 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             constexpr uint32_t iqk = um_idesc(128, kTtK, false), ipv = um_idesc(128, HD, true);
             const uint32_t ring0 = __shfl_sync(0xffffffffu, kv_smem(ring), 0), q0 = um_desc_lo(__shfl_sync(0xffffffffu, kv_smem(sq), 0), 16);
             int it = 0, seg = 0;  // tiles and segments done
+            RingPos at_k, at_v;   // K and V of the next tiles
+            at_v.next(NST);
             // O += P(i) . V(i); the segment's first one overwrites O
             auto pv = [&](int i, bool first) {
-                const int pos = 2 * i + 1, st = pos % NST;
+                const int st = at_v.st;
                 mb_wait(&pfull[i & 1], (i >> 1) & 1, &s_stop);
-                mb_wait(&full[st], (pos / NST) & 1, &s_stop);
+                mb_wait(&full[st], at_v.use, &s_stop);
+                at_v.next(NST, 2);
                 if (first && seg > 0) mb_wait(&ofree, (seg - 1) & 1, &s_stop);
                 um_fence_after();
                 const uint32_t vb = um_desc_lo(ring0 + st * STB, 16384), p0 = tmem + kTtS + (i & 1) * 128, px = tmem + kTtX + (i & 1) * 64;
@@ -354,9 +366,10 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             };
             while (w.next(a, node0)) {
                 for (int t = w.s_a; t < w.s_b; t++, it++) {
-                    const int pos = 2 * it, st = pos % NST;
+                    const int st = at_k.st;
                     if (t == w.s_a) mb_wait(&qfull, seg & 1, &s_stop);
-                    mb_wait(&full[st], (pos / NST) & 1, &s_stop);
+                    mb_wait(&full[st], at_k.use, &s_stop);
+                    at_k.next(NST, 2);
                     um_fence_after();
                     const uint32_t kb = um_desc_lo(ring0 + st * STB, 16), s0 = tmem + kTtS + (it & 1) * 128;
                     if (elect()) {
@@ -364,8 +377,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                         for (int x = QT - 1; x >= 0; x--)
 #pragma unroll
                             for (int k = 0; k < HD / 16; k++) {
-                                const uint32_t at = ((k >> 2) * 16384 + (k & 3) * 32) / 16;
-                                um_mma(s0, q0 + x * (STB / 16) + at, kb + at, iqk, !(x == QT - 1 && k == 0));
+                                um_mma(s0, q0 + (x * QTB + (k >> 2) * QH + (k & 3) * 32) / 16, kb + ((k >> 2) * 16384 + (k & 3) * 32) / 16, iqk,
+                                       !(x == QT - 1 && k == 0));
                             }
                         um_commit(&empty[st]);
                         um_commit(&sfull[it & 1]);
@@ -387,54 +400,77 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
         const float sl2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);
         int it = 0, seg = 0;
         int up = -1;
-        // the segment's Q into shared memory, a warp to a row, eight in flight,
+        // the segment's Q into shared memory, a warp to a row, eight or sixteen in flight,
         // and its nodes' parents on their way
-        auto load_q = [&](const TreeWalk<kTtK> &x) {
+        auto load_q = [&](const TreeSeg &x) {
             const int rows = min(NB, x.n - node0) << a.lg;
             if (threadIdx.x < kTreeMax) up = tree_parent(a, x.t0, x.n, threadIdx.x);
             const int half = HD == 128 ? lane >> 4 : 0, c = (lane & 15) * 4;  // dims half * 64 + c ..
             const bool on = HD == 128 || lane < 16;
-            const T *src = (const T *)a.q + (long long)(x.t0 + node0) * a.q_ld + (long long)x.s_kvh * a.G * HD + half * 64 + c;
-            for (int r0 = warp; r0 < rows; r0 += 64) {
-                float4 q[8];
+            const T *src = (const T *)a.q + (long long)(x.t0 + node0) * a.q_ld + (long long)x.kvh * a.G * HD + half * 64 + c;
+            constexpr int B = sizeof(T) == 4 ? 8 : 16;
+            for (int r0 = warp; r0 < rows; r0 += 8 * B) {
+                float4 q[B];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
+                for (int i = 0; i < B; i++) {
                     const int r = r0 + 8 * i;
                     q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (on && r < rows) q[i] = ld_row4(src + (long long)(r >> a.lg) * a.q_ld + (r & (a.G - 1)) * HD);
                 }
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
+                for (int i = 0; i < B; i++) {
                     const int r = r0 + 8 * i;
                     if (!on || r >= rows) continue;
                     if (a.scale < 0.f) q[i] = make_float4(-q[i].x, -q[i].y, -q[i].z, -q[i].w);
                     uint32_t lo[QT], hi[QT];
                     split_bf16<QT>(q[i].x, q[i].y, lo);
                     split_bf16<QT>(q[i].z, q[i].w, hi);
-                    uint8_t *dst = sq + half * 16384 + r * 128 + ((((c >> 3) ^ (r & 7)) << 4) | ((c & 4) << 1));
+                    uint8_t *dst = sq + half * QH + r * 128 + ((((c >> 3) ^ (r & 7)) << 4) | ((c & 4) << 1));
 #pragma unroll
-                    for (int k = 0; k < QT; k++) *(uint2 *)(dst + k * STB) = make_uint2(lo[k], hi[k]);
+                    for (int k = 0; k < QT; k++) *(uint2 *)(dst + k * QTB) = make_uint2(lo[k], hi[k]);
                 }
             }
             fence_async_smem();
             mb_arrive(&qfull);
         };
-        bool have = w.next(a, node0);
-        if (have) load_q(w);
-        while (have) {
-            const TreeWalk<kTtK> cur = w;
+        // one thread takes the walk a segment ahead
+        auto advance = [&](TreeSeg &x) {
+            TreeWalk<kTtK> v = s_walk;
+            x.have = v.next(a, node0);
+            x.slot = v.s_slot;
+            x.kvh = v.s_kvh;
+            x.a = v.s_a;
+            x.b = v.s_b;
+            x.g = v.s_g;
+            x.piece = v.s_g != v.g0;
+            x.L = v.L;
+            x.t0 = v.t0;
+            x.n = v.n;
+            x.T = v.T;
+            s_walk = v;
+        };
+        if (threadIdx.x == 0) {
+            s_walk = w;
+            advance(s_seg[0]);
+        }
+        bar_sync(1, kTtSoft);
+        if (s_seg[0].have) load_q(s_seg[0]);
+        while (s_seg[seg & 1].have) {
+            const TreeSeg &cur = s_seg[seg & 1];
             if (threadIdx.x < kTreeMax) s_up[threadIdx.x] = (int8_t)up;
             bar_sync(1, kTtSoft);
-            const int rows = min(NB, cur.n - node0) << a.lg, end = min(cur.L + cur.n, cap);
+            if (threadIdx.x == 0) advance(s_seg[(seg + 1) & 1]);
+            const int L = cur.L, t1 = cur.b, rows = min(NB, cur.n - node0) << a.lg, end = min(L + cur.n, cap);
             const bool active = (warp & 3) * 32 < rows;
             const int node = node0 + (th >> a.lg);
             unsigned long long mask = th < rows ? tree_mask(s_up, node) : 0;
             const bool live = mask != 0;  // not a padding node
-            if (end - cur.L < 64) mask &= (1ull << max(0, end - cur.L)) - 1;
+            if (end - L < 64) mask &= (1ull << max(0, end - L)) - 1;
             float m = -INFINITY, l = 0.f;
-            for (int t = cur.s_a; t < cur.s_b; t++, it++) {
+            bool first = true;
+            for (int t = cur.a; t < t1; t++, it++, first = false) {
                 const int b = it & 1, r0 = t * kTtK;
-                const bool tail = r0 + kTtK > cur.L, first = t == cur.s_a;
+                const bool tail = r0 + kTtK > L;
                 mb_wait(&sfull[b], (it >> 1) & 1, &s_stop);
                 um_fence_after();
                 const uint32_t sp = tmem + lanes + kTtS + b * 128, px = tmem + lanes + kTtX + b * 64;
@@ -445,7 +481,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                     um_wait_ld<64>(s);
                     if (tail || !live) {
                         // bits of this half's rows that the node sees
-                        const int c = cur.L - r0 - h * 64;  // cached rows among them
+                        const int c = L - r0 - h * 64;  // cached rows among them
                         unsigned long long see = 0;
                         if (live) see = c >= 64 ? ~0ull : c > 0 ? ((1ull << c) - 1) | (mask << c) : -c >= 64 ? 0 : mask >> -c;
 #pragma unroll
@@ -515,7 +551,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                     // add at the end
                     const int pos = 2 * it + 1, st = pos % NST, r = r0 + th;
                     mb_wait(&full[st], (pos / NST) & 1, &s_stop);
-                    if (r >= cur.L) {
+                    if (r >= L) {
                         uint8_t *vr = ring + (size_t)st * STB + (HD == 128 ? h * 16384 : 0) + th * 128;
                         const int c0 = HD == 128 ? 0 : h * 4;  // its 16-byte chunks
                         bool bad = false;
@@ -527,7 +563,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                                 for (int k = 0; k < 4; k++)
                                     bad |= (x[k] & 0x7f80u) == 0x7f80u || (x[k] & 0x7f800000u) == 0x7f800000u;
                             }
-                        if (bad) atomicOr(&s_bad[seg & 1][h], 1ull << (r - cur.L));
+                        if (bad) atomicOr(&s_bad[seg & 1][h], 1ull << (r - L));
                         if (bad || r >= end)
                             for (int i = 0; i < HD / 16; i++) *(uint4 *)(vr + (((c0 + i) ^ (th & 7)) << 4)) = make_uint4(0, 0, 0, 0);
                     }
@@ -538,14 +574,13 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             }
             // every S of the segment is done, so the next one's Q may go in
             // while the last P . V runs
-            have = w.next(a, node0);
-            if (have) load_q(w);
+            if (s_seg[(seg + 1) & 1].have) load_q(s_seg[(seg + 1) & 1]);
             s_half[h][th] = l;
             bar_sync(1, kTtSoft);  // and s_bad is complete
             l = h ? s_half[0][th] + l : l + s_half[1][th];
             const unsigned long long bad = s_bad[seg & 1][h] & mask;
             if (th == 0) s_bad[(seg + 1) & 1][h] = 0;
-            const bool whole = cur.s_a == 0 && cur.s_b == cur.T;
+            const bool whole = cur.a == 0 && t1 == cur.T;
             mb_wait(&odone[(it - 1) & 1], ((it - 1) >> 1) & 1, &s_stop);
             um_fence_after();
             if (active) {
@@ -557,12 +592,12 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                 um_fence_before();
                 mb_arrive(&ofree);
                 if (th < rows) {
-                    const int tok = cur.t0 + node, head = cur.s_kvh * a.G + (th & (a.G - 1));
+                    const int tok = cur.t0 + node, head = cur.kvh * a.G + (th & (a.G - 1));
                     if (bad && l > 0.f) {
                         float x[W];  // its address is taken: o stays in registers
 #pragma unroll
                         for (int d = 0; d < W; d++) x[d] = o[d];
-                        tree_add_bad<T, HD>(a, cur.s_slot, cur.s_kvh, cur.L, tok, head, h * W, bad, sl2, m, x);
+                        tree_add_bad<T, HD>(a, cur.slot, cur.kvh, L, tok, head, h * W, bad, sl2, m, x);
 #pragma unroll
                         for (int d = 0; d < W; d++) o[d] = x[d];
                     }
@@ -574,7 +609,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                         if (a.lse && h == 0)
                             a.lse[(long long)tok * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
                     } else {
-                        const int piece = (2 * range + (cur.s_g != cur.g0)) * a.row_blocks + rb;
+                        const int piece = (2 * range + cur.piece) * a.row_blocks + rb;
                         if (h == 0) a.part_ml[(size_t)piece * 128 + th] = make_float2(m, l);
                         float *po = a.part_o + (size_t)piece * 128 * HD + h * W * 128 + th * 8;
 #pragma unroll
@@ -584,7 +619,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             } else {
                 mb_arrive(&ofree);
             }
-            if (range_root && cur.s_a == 0 && !whole) a.roots[range] = make_int4(cur.s_slot, cur.s_kvh, cur.s_g, s_start[3]);
+            if (range_root && cur.a == 0 && !whole) a.roots[range] = make_int4(cur.slot, cur.kvh, cur.g, s_start[3]);
             bar_sync(1, kTtSoft);
             seg++;
         }
@@ -957,30 +992,35 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
 // ---------------------------------------------------------------- joining the pieces
 //
 // For the columns that start in one range and go on in the next: M = max m_i,
-// out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i over the pieces in order.  A
-// warp takes a (node, head) row, hd / 32 dims a lane, of a work list over all
-// such columns.  Pieces of the narrow form are `rows_per` rows of HD values;
-// those of the wide one (rows_per = 0) [8 dims][128 rows][8].
+// out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i over the pieces.  A work list
+// over all such columns' (node, head) rows; 1, 2, 4 or 8 warps take a row, as
+// many as keep the grid busy (few rows have many pieces), every so many-th
+// piece each, hd / 32 dims a lane, joined in a fixed order.  Pieces of the
+// narrow form are `rows_per` rows of HD values; those of the wide one (rows_per
+// = 0) [8 dims][128 rows][8].
 constexpr int kMergeThreads = 256;
 template <typename T, int HD, int TK>
 __global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constant__ TreeArgs a, int rows_per) {
     constexpr int D = HD / 32, W = kMergeThreads / 32;
     __shared__ int s_scan[W];
-    __shared__ int4 s_root[W];
-    __shared__ int s_row[W];
+    __shared__ float s_part[W][HD], s_m[W], s_l[W];
+    __shared__ int4 s_col[W], s_at[W];  // a row's {slot, KV head, first tile, tiles per range}, {row, first token, tiles, -}
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // rows of the columns that start in this thread's ranges
+    // rows of the columns that start in this thread's ranges (one column a range at most)
     int sum = 0, total = 0;
     const int per = (a.ranges + kMergeThreads - 1) / kMergeThreads, b0 = min(a.ranges, (int)threadIdx.x * per), b1 = min(a.ranges, b0 + per);
-    const auto count = [&](const int4 &root) {
+    const auto count = [&](const int4 &root, int &t0, int &tiles) {
         if (root.x < 0) return 0;
-        int L, t0, n;
+        int L, n;
         tree_span(a.v, a.len, a.off, a.max_nodes, root.x, L, t0, n);
+        tiles = TreeWalk<TK>::tiles(L, n, a.v.page_max * kPageRows);
         return n * a.G;
     };
-#pragma unroll 8
-    for (int i = b0; i < b1; i++) sum += count(a.roots[i]);
+    for (int i = b0; i < b1; i++) {
+        int t0, tiles;
+        sum += count(a.roots[i], t0, tiles);
+    }
     int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -994,54 +1034,47 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constan
         if (i < warp) before += s_scan[i];
         total += s_scan[i];
     }
-    for (int row0 = blockIdx.x * W; row0 < total; row0 += gridDim.x * W) {
-        // the CTA's next W rows: whoever's ranges hold one says so
-        if (before < row0 + W && before + sum > row0) {
+    int wpr = W;  // warps of a row
+    while (wpr > 1 && total * wpr > (int)gridDim.x * W) wpr >>= 1;
+    const int RPC = W / wpr, mine = warp / wpr, part = warp % wpr;
+    for (int row0 = blockIdx.x * RPC; row0 < total; row0 += gridDim.x * RPC) {
+        // the CTA's next rows: whoever's ranges hold one says so
+        if (before < row0 + RPC && before + sum > row0) {
             int at = before;
             for (int i = b0; i < b1; i++) {
                 const int4 root = a.roots[i];
-                const int c = count(root);
-                for (int x = max(at, row0); x < min(at + c, row0 + W); x++) {
-                    s_root[x - row0] = root;
-                    s_row[x - row0] = x - at;
+                int t0 = 0, tiles = 0;
+                const int c = count(root, t0, tiles);
+                for (int x = max(at, row0); x < min(at + c, row0 + RPC); x++) {
+                    s_col[x - row0] = root;
+                    s_at[x - row0] = make_int4(x - at, t0, tiles, 0);
                 }
                 at += c;
             }
         }
         __syncthreads();
-        if (row0 + warp < total) {
-            const int4 root = s_root[warp];
-            const int r = s_row[warp], node = r / a.G;
-            int L, t0, n;
-            tree_span(a.v, a.len, a.off, a.max_nodes, root.x, L, t0, n);
-            const int T_ = TreeWalk<TK>::tiles(L, n, a.v.page_max * kPageRows), C = root.w;
-            const int p0 = root.z / C, p1 = (root.z + T_ - 1) / C, d0 = lane * D;
-            const auto piece = [&](int p) { return (size_t)2 * p + (p * C < root.z); };
-            const auto ml_at = [&](int p) {
-                return rows_per ? a.part_ml[piece(p) * rows_per + r] : a.part_ml[(piece(p) * a.row_blocks + (r >> 7)) * 128 + (r & 127)];
-            };
-            float M = -INFINITY;
-            for (int p = p0 + lane; p <= p1; p += 32) {
-                const float2 ml = ml_at(p);
-                if (ml.y != 0.f) M = fmaxf(M, ml.x);
-            }
-            M = warp_max(M);
-            float S = 0.f, o[D];
+        const bool on = row0 + mine < total;
+        float M = -INFINITY, S = 0.f, o[D];
 #pragma unroll
-            for (int d = 0; d < D; d++) o[d] = 0.f;
-            for (int q0 = p0; q0 <= p1; q0 += 8) {  // eight pieces in flight
+        for (int d = 0; d < D; d++) o[d] = 0.f;
+        const int d0 = lane * D;
+        if (on) {
+            const int4 root = s_col[mine], me = s_at[mine];
+            const int r = me.x, C = root.w, p0 = root.z / C + part, p1 = (root.z + me.z - 1) / C;
+            for (int q0 = p0; q0 <= p1; q0 += 8 * wpr) {  // eight pieces in flight
                 float v[8][D];
                 float2 ml[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    ml[i] = make_float2(0.f, 0.f);
+                    ml[i] = make_float2(-INFINITY, 0.f);
 #pragma unroll
                     for (int d = 0; d < D; d++) v[i][d] = 0.f;
-                    if (q0 + i > p1) continue;
-                    ml[i] = ml_at(q0 + i);
-                    const float *po = rows_per ? a.part_o + (piece(q0 + i) * rows_per + r) * HD + d0
-                                               : a.part_o + (piece(q0 + i) * a.row_blocks + (r >> 7)) * 128 * HD + (d0 >> 3) * 1024 +
-                                                     (r & 127) * 8 + (d0 & 7);
+                    const int p = q0 + i * wpr;
+                    if (p > p1) continue;
+                    const size_t pc = ((size_t)2 * p + (p * C < root.z)) * a.row_blocks + (rows_per ? 0 : r >> 7);
+                    ml[i] = a.part_ml[rows_per ? pc * rows_per + r : pc * 128 + (r & 127)];
+                    const float *po = a.part_o + (rows_per ? (pc * rows_per + r) * HD + d0
+                                                           : pc * 128 * HD + (d0 >> 3) * 1024 + (r & 127) * 8 + (d0 & 7));
                     if constexpr (D == 4) {
                         const float4 x = *(const float4 *)po;
                         v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
@@ -1050,6 +1083,15 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constan
                         v[i][0] = x.x, v[i][1] = x.y;
                     }
                 }
+                float mn = M;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (ml[i].y != 0.f) mn = fmaxf(mn, ml[i].x);
+                const float old = M == -INFINITY ? 0.f : ex2(M - mn);
+                M = mn;
+                S *= old;
+#pragma unroll
+                for (int d = 0; d < D; d++) o[d] *= old;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const float f = ml[i].y == 0.f ? 0.f : ex2(ml[i].x - M);  // 0: nothing seen in this piece
@@ -1058,8 +1100,33 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constan
                     for (int d = 0; d < D; d++) o[d] = fmaf(v[i][d], f, o[d]);
                 }
             }
+        }
+        if (wpr > 1) {
+            if (lane == 0) {
+                s_m[warp] = M;
+                s_l[warp] = S;
+            }
+#pragma unroll
+            for (int d = 0; d < D; d++) s_part[warp][d0 + d] = o[d];
+            __syncthreads();
+            if (part == 0) {
+                for (int i = 1; i < wpr; i++) M = fmaxf(M, s_m[warp + i]);
+                S = 0.f;
+#pragma unroll
+                for (int d = 0; d < D; d++) o[d] = 0.f;
+                for (int i = 0; i < wpr; i++) {
+                    const float l = s_l[warp + i], f = l == 0.f ? 0.f : ex2(s_m[warp + i] - M);
+                    S = fmaf(l, f, S);
+#pragma unroll
+                    for (int d = 0; d < D; d++) o[d] = fmaf(s_part[warp + i][d0 + d], f, o[d]);
+                }
+            }
+        }
+        if (on && part == 0) {
+            const int4 root = s_col[mine], me = s_at[mine];
+            const int r = me.x;
             const float inv = S == 0.f ? 0.f : 1.0f / S;
-            const int tok = t0 + node, head = root.y * a.G + r % a.G;
+            const int tok = me.y + r / a.G, head = root.y * a.G + r % a.G;
             T *dst = (T *)a.out + (long long)tok * a.out_ld + (long long)head * HD + d0;
             if constexpr (D == 4) st_row4(dst, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
             else if constexpr (sizeof(T) == 4) *(float2 *)dst = make_float2(o[0] * inv, o[1] * inv);

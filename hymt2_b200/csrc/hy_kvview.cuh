@@ -85,6 +85,19 @@ __device__ __forceinline__ void mb_wait(uint64_t *b, unsigned parity, int *stop)
         }
     }
 }
+// A place in a ring of stages: its stage, and the parity of that stage's use.
+// (Counting up: a division by the ring's length a stage cost 0.5 us a tile.)
+struct RingPos {
+    int st = 0;
+    unsigned use = 0;
+    __device__ __forceinline__ void next(int stages, int by = 1) {
+        st += by;
+        if (st >= stages) {
+            st -= stages;
+            use ^= 1;
+        }
+    }
+};
 __device__ __forceinline__ void tma_box(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
@@ -200,6 +213,22 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+        " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
 }
 // bf16 pair, lo in the low half.
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {

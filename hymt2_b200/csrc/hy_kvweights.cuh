@@ -91,7 +91,9 @@ __global__ void __launch_bounds__(kWtThreads, 1) cache_weights_tc(const __grid_c
     __shared__ uint32_t s_tmem;
     __shared__ int s_scan[kWtThreads / 32], s_start[4], s_stop;
     __shared__ int s_tok[128];
-    __shared__ __align__(16) float2 s_col[2][128];  // of each query row: lse * log2 e, last row it sees
+    __shared__ unsigned s_counts[2];
+    __shared__ __align__(16) float s_lse[2][128];  // of each query row: -lse * log2 e,
+    __shared__ __align__(16) int s_last[2][128];   // and the last cached row it sees
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, NB = a.block, NST = a.stages;
     const int half_b = NB * 128, term_b = NH * half_b, qbuf_b = QT * term_b;
     uint8_t *sq = (uint8_t *)(((uintptr_t)dsm + 1023) & ~(uintptr_t)1023);
@@ -174,14 +176,15 @@ __global__ void __launch_bounds__(kWtThreads, 1) cache_weights_tc(const __grid_c
     if (warp == 16) {
         const int yend = a.v.layers * a.v.npages * 2 * kPageRows;
         int pos = 0;
+        RingPos at;
         while (w.next(a)) {
             const int pages = (w.end + kPageRows - 1) / kPageRows;
             for (int q0 = 0; q0 < w.n * a.G; q0 += NB)
-                for (int t = w.s_a; t < w.s_b; t++, pos++) {
-                    const int j = t * 8 + (lane & 7), st = pos % NST, use = pos / NST;
+                for (int t = w.s_a; t < w.s_b; t++, pos++, at.next(NST)) {
+                    const int j = t * 8 + (lane & 7), st = at.st;
                     const int pg = j < pages ? __ldg(a.v.pages + (size_t)w.s_slot * a.v.page_max + j) : -1;
                     const int y = pg < 0 || pg >= a.v.npages ? yend : (w.s_layer * a.v.npages + pg) * 2 * kPageRows;
-                    if (use > 0) mb_wait(&empty[st], (use - 1) & 1, &s_stop);
+                    mb_wait(&empty[st], at.use ^ 1, &s_stop);  // passes on a stage's first use
                     if (__any_sync(0xffffffffu, *(volatile int *)&s_stop)) {
                         pos--;
                         continue;
@@ -207,15 +210,16 @@ __global__ void __launch_bounds__(kWtThreads, 1) cache_weights_tc(const __grid_c
     } else if (warp == 17) {
         {
             const uint32_t ring0 = __shfl_sync(0xffffffffu, kv_smem(ring), 0), sq0 = __shfl_sync(0xffffffffu, kv_smem(sq), 0);
-            int it = 0, qi = 0, turn = 0, used = 0;  // used: parity of each S^T tile's uses
+            RingPos at;
+            int qi = 0, turn = 0, used = 0;  // used: parity of each S^T tile's uses
             while (w.next(a)) {
                 for (int q0 = 0; q0 < w.n * a.G; q0 += NB, qi++) {
                     const int qb = qi % a.qbufs, N = (min(NB, w.n * a.G - q0) + 15) & ~15;
                     const uint32_t id = um_idesc(128, N, false), qa = um_desc_lo(sq0 + qb * qbuf_b, 16);
                     mb_wait(&qfull[qb], (qi / a.qbufs) & 1, &s_stop);
-                    for (int t = w.s_a; t < w.s_b; t++, it++) {
-                        const int st = it % NST, b = (t - w.s_a + turn) % NS;
-                        mb_wait(&full[st], (it / NST) & 1, &s_stop);
+                    for (int t = w.s_a; t < w.s_b; t++, at.next(NST)) {
+                        const int st = at.st, b = (t - w.s_a + turn) % NS;
+                        mb_wait(&full[st], at.use, &s_stop);
                         mb_wait(&sempty[b], ((used >> b) & 1) ^ 1, &s_stop);  // passes on the first use
                         used ^= 1 << b;
                         um_fence_after();
@@ -255,17 +259,27 @@ __global__ void __launch_bounds__(kWtThreads, 1) cache_weights_tc(const __grid_c
                     const int t = th < rows ? __ldg(a.sel + (size_t)w.s_slot * a.max_q + j) : -1;
                     // a query that is left out, or saw nothing (-inf), sees no row
                     const float e = t >= 0 ? a.lse[w.s_layer * a.lse_layer + (long long)t * a.heads + head] : -INFINITY;
-                    s_col[qb][th] = make_float2(e * 1.4426950408889634f, __int_as_float(e == -INFINITY ? -1 : w.L + j));
+                    s_lse[qb][th] = e * -1.4426950408889634f;
+                    s_last[qb][th] = e == -INFINITY ? -1 : w.L + j;
                     s_tok[th] = t;
                 }
                 bar_sync(1, 128);
+                if (wl == 0) {
+                    unsigned ok = 0;
+                    for (int i = 0; i < N; i += 32) {  // two groups of 16 a step
+                        const unsigned m = __ballot_sync(0xffffffffu, i + lane < N && s_last[qb][i + lane] >= 0);
+                        ok |= ((m & 0xffffu) == 0xffffu ? 1u : 0u) << (i >> 4) | (m >> 16 == 0xffffu ? 2u : 0u) << (i >> 4);
+                    }
+                    if (lane == 0) s_counts[qb] = ok;
+                }
                 uint8_t *dst0 = sq + qb * qbuf_b;
                 const int half = HD == 128 ? lane >> 4 : 0, c = (lane & 15) * 4;
                 const T *src0 = (const T *)a.q + w.s_layer * a.q_layer + (long long)w.s_kvh * a.G * HD + half * 64 + c;
-                for (int r0 = wl; r0 < N; r0 += 16) {  // a warp to a row, four rows in flight
-                    float4 q[4];
+                constexpr int B = 4;
+                for (int r0 = wl; r0 < N; r0 += 4 * B) {  // a warp to a row, four rows in flight (eight: 74 -> 95 us at 31 queries)
+                    float4 q[B];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
+                    for (int i = 0; i < B; i++) {
                         const int r = r0 + 4 * i, t = r < N ? s_tok[r] : -1;
                         q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                         if (t >= 0 && (HD == 128 || lane < 16)) {
@@ -280,7 +294,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) cache_weights_tc(const __grid_c
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
+                    for (int i = 0; i < B; i++) {
                         const int r = r0 + 4 * i;
                         if (r < N && (HD == 128 || lane < 16)) {
                             uint32_t lo[QT], hi[QT];
@@ -305,27 +319,43 @@ __global__ void __launch_bounds__(kWtThreads, 1) cache_weights_tc(const __grid_c
             for (int q0 = 0; q0 < w.n * a.G; q0 += NB, qi++) {
                 const int qb = qi % a.qbufs, N = (min(NB, w.n * a.G - q0) + 15) & ~15;
                 mb_wait(&qfull[qb], (qi / a.qbufs) & 1, &s_stop);
+                const unsigned counts = s_counts[qb];  // bit c: all of queries 16 c .. 16 c + 15 count
                 for (int t = w.s_a + (group - turn % NS + NS) % NS; t < w.s_b; t += NS, uses++) {
                     const int r = t * 128 + th;
                     float sum = r < w.end && (r < w.L || q0 > 0) ? acc[r] : 0.f;
                     mb_wait(&sfull[group], uses & 1, &s_stop);
                     um_fence_after();
-                    float part[2] = {0.f, 0.f};
+                    float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    const bool open = t * 128 + 127 <= w.L;  // all rows of the tile are seen by all queries that count
                     for (int c = 0; c < N; c += 16) {
                         float x[16];
                         um_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + group * 128 + c, x);
                         um_wait_ld<16>(x);
+                        float2 p[8];
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            const float4 e = *(const float4 *)&s_col[qb][c + i];
-                            const float p0 = ex2(fmaf(x[i], sl2, -e.x)), p1 = ex2(fmaf(x[i + 1], sl2, -e.z));
-                            part[0] += r <= __float_as_int(e.y) ? p0 : 0.f;
-                            part[1] += r <= __float_as_int(e.w) ? p1 : 0.f;
+                        for (int i = 0; i < 16; i += 4) {
+                            const float4 e = *(const float4 *)&s_lse[qb][c + i];
+                            const float2 y0 = fma2(make_float2(x[i], x[i + 1]), make_float2(sl2, sl2), make_float2(e.x, e.y));
+                            const float2 y1 = fma2(make_float2(x[i + 2], x[i + 3]), make_float2(sl2, sl2), make_float2(e.z, e.w));
+                            p[i / 2] = make_float2(ex2(y0.x), ex2(y0.y));
+                            p[i / 2 + 1] = make_float2(ex2(y1.x), ex2(y1.y));
                         }
+                        if (!open || !((counts >> (c >> 4)) & 1)) {
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4) {
+                                const int4 e = *(const int4 *)&s_last[qb][c + i];
+                                if (r > e.x) p[i / 2].x = 0.f;
+                                if (r > e.y) p[i / 2].y = 0.f;
+                                if (r > e.z) p[i / 2 + 1].x = 0.f;
+                                if (r > e.w) p[i / 2 + 1].y = 0.f;
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; i++) part[i & 1] = add2(part[i & 1], p[i]);
                     }
                     um_fence_before();
                     mb_arrive(&sempty[group]);
-                    if (r < w.end) acc[r] = sum + (part[0] + part[1]);
+                    if (r < w.end) acc[r] = sum + ((part[0].x + part[0].y) + (part[1].x + part[1].y));
                 }
                 mb_arrive(&qempty[qb]);
             }
