@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
     __shared__ int s_scan[kTnWarps], s_start[4];
     __shared__ int8_t s_up[kTreeMax];
     __shared__ float s_mx[kTnWarps][NT * 8];
-    __shared__ unsigned long long s_bad;
+    __shared__ unsigned long long s_bad, s_mask[NT * 8];  // s_mask: what a query row's node sees of its tree
     uint8_t *bk = dsm, *bv = dsm + kTnK * ROW;
     uint2 *qf = (uint2 *)(bv + kTnK * ROW);    // Q fragments [term][16 dims][8 rows][lane]
     uint2 *pf = qf + QT * KS * NT * 32;        // P fragments [term][page][8 rows][lane]
@@ -703,25 +703,28 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
     TreeWalk<kTnK> wi = tree_walk<kTnK>(s_start, range), wc = wi;
     bool more = wi.next(a, 0);
     int it = more ? wi.s_a : 0;  // the tile to copy next, of column wi
-    int pgs[kTnK / kPageRows];   // its pages
+    const uint16_t *src[kTnK / kPageRows];  // its pages' K rows of this thread (first row and chunk), null: no page
+    const int cc = th % CH, cr = th / CH;   // this thread's chunk of a row, and its first row of a copy step's
     auto pages = [&]() {
+        const int p0 = it * (kTnK / kPageRows), n = (min(wi.L + wi.n, cap) + kPageRows - 1) / kPageRows;
+        const uint16_t *base = a.v.kv + a.layer * a.v.layer_stride + (long long)cr * a.v.kvd + wi.s_kvh * HD + cc * 8;
 #pragma unroll
         for (int i = 0; i < kTnK / kPageRows; i++) {
-            pgs[i] = -1;
-            if (more && it * kTnK + i * kPageRows < wi.L + wi.n) pgs[i] = a.v.page(wi.s_slot, it * kTnK + i * kPageRows);
+            const int pg = more && p0 + i < n ? __ldg(a.v.pages + (size_t)wi.s_slot * a.v.page_max + p0 + i) : -1;
+            src[i] = pg >= 0 && pg < a.v.npages ? base + (long long)pg * a.v.page_stride : nullptr;
         }
     };
     // K (kv = 0) or V rows of that tile; rows that do not exist become zeros
     auto copy = [&](int kv) {
         if (more) {
-            const int c = th % CH, r0 = th / CH, end = min(wi.L + wi.n, cap) - it * kTnK;
-            const uint32_t dst = kv_smem(kv ? bv : bk);
+            const int end = min(wi.L + wi.n, cap) - it * kTnK, off = kv * kPageRows * a.v.kvd;
+            const uint32_t dst = kv_smem(kv ? bv : bk) + cr * ROW + ((cc ^ (cr & 7)) << 4);
 #pragma unroll
-            for (int i = 0; i < NI; i++) {
-                const int r = r0 + i * RPI, pg = pgs[(i * RPI) / kPageRows];
-                const uint16_t *p = a.v.kv + a.v.row(a.layer, max(pg, 0), r) + (long long)kv * kPageRows * a.v.kvd + wi.s_kvh * HD + c * 8;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + r * ROW + ((c ^ (r & 7)) << 4)), "l"(p),
-                             "r"(pg >= 0 && r < end ? 16 : 0)
+            for (int i = 0; i < NI; i++) {  // rows cr + i * RPI: RPI is 8 or 16, so the swizzle stays
+                const uint16_t *pg = src[(i * RPI) / kPageRows];
+                const bool ok = pg && cr + i * RPI < end;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i * RPI * ROW),
+                             "l"(ok ? pg + off + (i * RPI % kPageRows) * a.v.kvd : a.v.kv), "r"(ok ? 16 : 0)
                              : "memory");
             }
         }
@@ -791,7 +794,8 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
             }
             pages();
             asm volatile("cp.async.wait_group 1;" ::: "memory");
-            __syncthreads();  // K and Q are there
+            __syncthreads();  // K, Q and the parents are there
+            if (tail && th < NT * 8) s_mask[th] = th < rows ? tree_mask(s_up, th >> a.lg) : 0;  // read past the next barrier
             float s[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
@@ -811,20 +815,23 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
                         }
                 }
             }
+            if (tail) __syncthreads();  // s_mask
             bool grow = false;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    unsigned long long mk = 0;
-                    const int row = nt * 8 + 2 * tq + j;
-                    if (tail && row < rows) mk = tree_mask(s_up, row >> a.lg);
-                    const bool hide = (dead >> (2 * nt + j)) & 1;
+                    unsigned see = (dead >> (2 * nt + j)) & 1 ? 0u : 0xffffu;  // of the page's 16 rows
+                    if (tail) {
+                        const unsigned long long mk = s_mask[nt * 8 + 2 * tq + j];
+                        const int c = wc.L - r0 - warp * 16;  // cached rows among them
+                        const unsigned own = c >= 16 ? 0xffffu : c > 0 ? ((1u << c) - 1) | (unsigned)(mk << c) : -c < 64 ? (unsigned)(mk >> -c) : 0u;
+                        see &= own & (end - r0 - warp * 16 >= 16 ? 0xffffu : end - r0 - warp * 16 > 0 ? (1u << (end - r0 - warp * 16)) - 1 : 0u);
+                    }
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         float x = s[nt][2 * h + j] * sl2;
-                        const int r = r0 + warp * 16 + g + h * 8;
-                        if (hide || (tail && !(r < wc.L || (r < end && ((mk >> (r - wc.L)) & 1))))) x = -INFINITY;
+                        if (!((see >> (g + h * 8)) & 1)) x = -INFINITY;
                         s[nt][2 * h + j] = x;
                         grow |= x > m[nt][j] + 8.f;
                     }
@@ -1061,11 +1068,12 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constan
         if (on) {
             const int4 root = s_col[mine], me = s_at[mine];
             const int r = me.x, C = root.w, p0 = root.z / C + part, p1 = (root.z + me.z - 1) / C;
-            for (int q0 = p0; q0 <= p1; q0 += 8 * wpr) {  // eight pieces in flight
-                float v[8][D];
-                float2 ml[8];
+            constexpr int B = 4;
+            for (int q0 = p0; q0 <= p1; q0 += B * wpr) {  // four pieces in flight
+                float v[B][D];
+                float2 ml[B];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
+                for (int i = 0; i < B; i++) {
                     ml[i] = make_float2(-INFINITY, 0.f);
 #pragma unroll
                     for (int d = 0; d < D; d++) v[i][d] = 0.f;
@@ -1085,7 +1093,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constan
                 }
                 float mn = M;
 #pragma unroll
-                for (int i = 0; i < 8; i++)
+                for (int i = 0; i < B; i++)
                     if (ml[i].y != 0.f) mn = fmaxf(mn, ml[i].x);
                 const float old = M == -INFINITY ? 0.f : ex2(M - mn);
                 M = mn;
@@ -1093,7 +1101,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constan
 #pragma unroll
                 for (int d = 0; d < D; d++) o[d] *= old;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
+                for (int i = 0; i < B; i++) {
                     const float f = ml[i].y == 0.f ? 0.f : ex2(ml[i].x - M);  // 0: nothing seen in this piece
                     S = fmaf(ml[i].y, f, S);
 #pragma unroll
