@@ -213,11 +213,21 @@ __device__ __noinline__ void tree_add_bad(const TreeArgs &a, int slot, int kvh, 
 // fp32 queries enter the bf16 products as three bf16 terms (all 24 bits), and
 // so does P for fp32 outputs: K and V are bf16 already, and every sum is
 // fp32.  For bf16 outputs P has two terms (16 bits): one would add an error
-// as large as the output's own rounding.  The maximum that P is taken
-// against moves only when it would grow by over 2^8, which rescales O; sums
-// and outputs stay exact under it, as the same one divides out at the end.
+// as large as the output's own rounding.  The tensor cores cut, not round,
+// what they add to an fp32 accumulator: over n products the sum falls short by
+// about n 2^-26 of itself (1.8e-5 over 125 tiles).  So O leaves tensor memory
+// for registers after every tile (fp32 outputs; every 32nd for bf16 ones),
+// where sums round, and the small terms of a tile go first, while its sum is
+// small.  The maximum that P is taken against moves only when it would grow by
+// over 2^8, which rescales O; sums and outputs stay exact under it, as the same
+// one divides out at the end.
 constexpr int kTtK = 128;       // cached rows of a tile
-constexpr int kTtThreads = 320, kTtSoft = 256;
+constexpr int kTtThreads = 384, kTtSoft = 256;
+// Registers of a softmax thread and of the others: 256 * 216 + 128 * 72 = 384 * 168, what the block is launched with.
+constexpr int kTtRegsSoft = 216, kTtRegsFeed = 72;
+// Tiles that O adds up in tensor memory before it goes to registers.
+template <typename T>
+__host__ __device__ constexpr int tt_flush() { return sizeof(T) == 4 ? 1 : 32; }
 
 template <typename T>
 __host__ __device__ constexpr int tt_qterms() { return sizeof(T) == 4 ? 3 : 1; }
@@ -253,7 +263,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
     __shared__ int8_t s_up[kTreeMax];
     __shared__ unsigned long long s_bad[2][2];
     __shared__ float s_half[2][128];
-    __shared__ int s_stop;
+    __shared__ int s_stop, s_fresh[2];  // s_fresh: P . V of this tile starts O anew
     __shared__ TreeSeg s_seg[2];
     __shared__ TreeWalk<kTtK> s_walk;  // the softmax warps' walk: in registers it would cost them spills
     uint8_t *sq = (uint8_t *)(((uintptr_t)dsm + 1023) & ~(uintptr_t)1023);
@@ -292,6 +302,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
     const int cap = a.v.page_max * kPageRows;
     const bool range_root = rb == 0 && threadIdx.x == 0;  // the thread that notes the range's split column
     if (range_root) a.roots[range] = make_int4(-1, 0, 0, 0);
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTtRegsFeed));
     if (warp == 8) {
         // eight pages a tile, K then V; a page that does not exist is read past
         // the end of the map, which fills zeros
@@ -343,7 +355,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             int it = 0, seg = 0;  // tiles and segments done
             RingPos at_k, at_v;   // K and V of the next tiles
             at_v.next(NST);
-            // O += P(i) . V(i); the segment's first one overwrites O
+            // O += P(i) . V(i), or O = ...; the segment's first one also waits for the last segment's O to be read
             auto pv = [&](int i, bool first) {
                 const int st = at_v.st;
                 mb_wait(&pfull[i & 1], (i >> 1) & 1, &s_stop);
@@ -351,6 +363,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                 at_v.next(NST, 2);
                 if (first && seg > 0) mb_wait(&ofree, (seg - 1) & 1, &s_stop);
                 um_fence_after();
+                const bool fresh = s_fresh[i & 1];
                 const uint32_t vb = um_desc_lo(ring0 + st * STB, 16384), p0 = tmem + kTtS + (i & 1) * 128, px = tmem + kTtX + (i & 1) * 64;
                 if (elect()) {
 #pragma unroll
@@ -358,7 +371,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
 #pragma unroll
                         for (int k = 0; k < kTtK / 16; k++)
                             um_mma_ts(tmem + kTtO, (x == 2 ? px : p0 + x * 64) + k * 8, vb + k * (2048 / 16), ipv,
-                                      x == PT - 1 && k == 0 ? !first : true);
+                                      x == PT - 1 && k == 0 ? !fresh : true);
                     um_commit(&empty[st]);
                     um_commit(&odone[i & 1]);
                 }
@@ -394,7 +407,9 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             int none = 0;
             mb_wait(&fin, 0, &none);
         }
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTtRegsSoft));
         const int th = threadIdx.x & 127, h = warp >> 2;  // row, and half of its keys and dims
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const float sl2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);
@@ -466,7 +481,26 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             unsigned long long mask = th < rows ? tree_mask(s_up, node) : 0;
             const bool live = mask != 0;  // not a padding node
             if (end - L < 64) mask &= (1ull << max(0, end - L)) - 1;
-            float m = -INFINITY, l = 0.f;
+            constexpr int W = HD / 2;
+            float m = -INFINITY, l = 0.f, o[W];
+#pragma unroll
+            for (int d = 0; d < W; d++) o[d] = 0.f;
+            // O of the tiles so far, once their last product is done, into o
+            auto flush = [&]() {
+                mb_wait(&odone[(it - 1) & 1], ((it - 1) >> 1) & 1, &s_stop);
+                um_fence_after();
+                if (active) {
+#pragma unroll
+                    for (int c = 0; c < W / 32; c++) {
+                        float x[32];
+                        um_ld32(tmem + lanes + kTtO + h * W + c * 32, x);
+                        um_wait_ld<32>(x);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[c * 32 + i] += x[i];
+                    }
+                }
+            };
+            int since = 0;  // tiles in O that o does not have
             bool first = true;
             for (int t = cur.a; t < t1; t++, it++, first = false) {
                 const int b = it & 1, r0 = t * kTtK;
@@ -502,24 +536,12 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                         m = tm;
                     } else {
                         const float mn = tm > m + 8.f ? tm : m, f = m == -INFINITY ? 1.f : ex2(m - mn);
-                        const bool moved = mn > m;
                         m = mn;
                         l *= f;
-                        if (active && __any_sync(0xffffffffu, moved)) {
-                            mb_wait(&odone[(it - 1) & 1], ((it - 1) >> 1) & 1, &s_stop);
-                            um_fence_after();
+                        flush();
+                        since = 0;
 #pragma unroll
-                            for (int c = 0; c < HD / 64; c++) {
-                                const uint32_t at = tmem + lanes + kTtO + h * (HD / 2) + c * 32;
-                                float o[32];
-                                um_ld32(at, o);
-                                um_wait_ld<32>(o);
-#pragma unroll
-                                for (int i = 0; i < 32; i++) o[i] *= f;
-                                um_st32(at, o);
-                            }
-                            um_wait_st();
-                        }
+                        for (int d = 0; d < W; d++) o[d] *= f;
                     }
                 }
                 if (active) {
@@ -544,6 +566,12 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                     l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
                     um_wait_st();
                 }
+                if (since == tt_flush<T>()) {
+                    flush();
+                    since = 0;
+                }
+                if (threadIdx.x == 0) s_fresh[b] = since == 0;
+                since++;
                 if (tail) {
                     // V rows that no node sees become zeros (a product with a
                     // probability of 0 must be 0), and so do halves of drafted
@@ -581,16 +609,10 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             const unsigned long long bad = s_bad[seg & 1][h] & mask;
             if (th == 0) s_bad[(seg + 1) & 1][h] = 0;
             const bool whole = cur.a == 0 && t1 == cur.T;
-            mb_wait(&odone[(it - 1) & 1], ((it - 1) >> 1) & 1, &s_stop);
-            um_fence_after();
+            flush();
+            um_fence_before();
+            mb_arrive(&ofree);
             if (active) {
-                constexpr int W = HD / 2;
-                float o[W];
-#pragma unroll
-                for (int c = 0; c < W / 32; c++) um_ld32(tmem + lanes + kTtO + h * W + c * 32, o + c * 32);
-                um_wait_ld<W>(o);
-                um_fence_before();
-                mb_arrive(&ofree);
                 if (th < rows) {
                     const int tok = cur.t0 + node, head = cur.kvh * a.G + (th & (a.G - 1));
                     if (bad && l > 0.f) {
@@ -616,8 +638,6 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                         for (int d = 0; d < W; d += 8) st_row8(po + d * 128, o + d, 1.f);
                     }
                 }
-            } else {
-                mb_arrive(&ofree);
             }
             if (range_root && cur.a == 0 && !whole) a.roots[range] = make_int4(cur.slot, cur.kvh, cur.g, s_start[3]);
             bar_sync(1, kTtSoft);
@@ -642,8 +662,9 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
 // of the tile's page w, then hd / 4 dims of O^T over all keys: the output needs
 // no join between warps, and P^T crosses between them as operand fragments (by
 // 8x8 transposes in registers, then shared memory).  K's next tile is copied
-// while this one's V is multiplied, and V's while the next scores are made, so
-// one buffer each is enough.  The terms of fp32 queries and probabilities and
+// while this one's V is multiplied, and V's while the next scores are made: one
+// buffer each, and three CTAs an SM (two buffers and two CTAs: 45 -> 56 us at
+// 256 slots of about 120 rows and 5 nodes).  The terms of fp32 queries and probabilities and
 // the lagging maximum are those of the wide form.
 constexpr int kTnWarps = 4, kTnThreads = kTnWarps * 32, kTnK = 64;
 
@@ -796,9 +817,14 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
             asm volatile("cp.async.wait_group 1;" ::: "memory");
             __syncthreads();  // K, Q and the parents are there
             if (tail && th < NT * 8) s_mask[th] = th < rows ? tree_mask(s_up, th >> a.lg) : 0;  // read past the next barrier
-            float s[NT][4];
+            // the small terms in a sum of their own: an accumulator is cut, not
+            // rounded, with every product added, so it should take few
+            float s[NT][4], s1[NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+            for (int nt = 0; nt < NT; nt++) {
+                s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+                s1[nt][0] = s1[nt][1] = s1[nt][2] = s1[nt][3] = 0.f;
+            }
             if (r0 + warp * 16 < end) {
                 const int kr = warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
                 const uint32_t sk = kv_smem(bk) + kr * ROW;
@@ -807,11 +833,11 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
                     uint32_t ka[4];
                     ldm4(ka, sk + (((2 * k + (lane >> 4)) ^ (kr & 7)) << 4));
 #pragma unroll
-                    for (int i = QT - 1; i >= 0; i--)  // small terms first
+                    for (int i = QT - 1; i >= 0; i--)
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
                             const uint2 b = qf[((i * KS + k) * NT + nt) * 32 + lane];
-                            mma_16816(s[nt], ka, b.x, b.y);
+                            mma_16816(i ? s1[nt] : s[nt], ka, b.x, b.y);
                         }
                 }
             }
@@ -830,7 +856,7 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
                     }
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        float x = s[nt][2 * h + j] * sl2;
+                        float x = (s[nt][2 * h + j] + s1[nt][2 * h + j]) * sl2;
                         if (!((see >> (g + h * 8)) & 1)) x = -INFINITY;
                         s[nt][2 * h + j] = x;
                         grow |= x > m[nt][j] + 8.f;
@@ -900,22 +926,35 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
             }
             const int vr = (lane & 7) + (lane >> 4) * 8;
             const uint32_t sv = kv_smem(bv) + vr * ROW;
+            // the tile's sum by itself, small terms first, then added to O: sums
+            // in registers round, the products' accumulators cut
+            float u[MT][NT][4];
 #pragma unroll
-            for (int ks = 0; ks < kTnK / 16; ks++) {
-                if (r0 + ks * 16 >= end) break;
-                uint32_t va[MT][4];
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++)
-                    ldm4t(va[mt], sv + ks * 16 * ROW + (((2 * (warp * MT + mt) + ((lane >> 3) & 1)) ^ (vr & 7)) << 4));
+                for (int mt = 0; mt < MT; mt++) u[mt][nt][0] = u[mt][nt][1] = u[mt][nt][2] = u[mt][nt][3] = 0.f;
 #pragma unroll
-                for (int i = PT - 1; i >= 0; i--)
+            for (int i = PT - 1; i >= 0; i--)
+#pragma unroll
+                for (int ks = 0; ks < kTnK / 16; ks++) {
+                    if (r0 + ks * 16 >= end) break;
+                    uint32_t va[MT][4];
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+                        ldm4t(va[mt], sv + ks * 16 * ROW + (((2 * (warp * MT + mt) + ((lane >> 3) & 1)) ^ (vr & 7)) << 4));
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
                         const uint2 b = pf[((i * 4 + ks) * NT + nt) * 32 + lane];
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++) mma_16816(o[mt][nt], va[mt], b.x, b.y);
+                        for (int mt = 0; mt < MT; mt++) mma_16816(u[mt][nt], va[mt], b.x, b.y);
                     }
-            }
+                }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) o[mt][nt][j] += u[mt][nt][j];
             __syncthreads();  // P and V have been read
             copy(1);
         }
