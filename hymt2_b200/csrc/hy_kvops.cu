@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constan
 
 // grid (layers * slots * kv heads, row blocks): a warp copies K (lanes 0-15)
 // and V (lanes 16-31) of one kept row, 16 bytes a lane (hd 64: 8).
-constexpr int kGatherRows = 64;
+constexpr int kGatherRows = 128;
 __global__ void __launch_bounds__(256) evict_gather(const __grid_constant__ EvictArgs a) {
     const int idx = blockIdx.x, kvh = idx % a.v.kvh, s = (idx / a.v.kvh) % a.v.slots, layer = idx / (a.v.kvh * a.v.slots);
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;

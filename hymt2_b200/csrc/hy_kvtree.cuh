@@ -423,6 +423,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             const int half = HD == 128 ? lane >> 4 : 0, c = (lane & 15) * 4;  // dims half * 64 + c ..
             const bool on = HD == 128 || lane < 16;
             const T *src = (const T *)a.q + (long long)(x.t0 + node0) * a.q_ld + (long long)x.kvh * a.G * HD + half * 64 + c;
+            // (fp32: all sixteen of a warp's rows at once took 77 us against 73 at 32 x 30 nodes)
             constexpr int B = sizeof(T) == 4 ? 8 : 16;
             for (int r0 = warp; r0 < rows; r0 += 8 * B) {
                 float4 q[B];
