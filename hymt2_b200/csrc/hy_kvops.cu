@@ -40,7 +40,7 @@ bool make_view(const hyc_kv_view *v, KvView &o, const char **why) {
     else if (!aligned16(v->kv)) *why = "the cache must be 16-byte aligned";
     else if (v->page_max > (1 << 26) || v->kv_heads > 65535 || v->layers > 65535) *why = "cache view too large";
     else if ((long long)v->layers * v->npages * 2 * kPageRows > 0x7fffffffLL ||
-             (double)v->layers * v->slots * v->kv_heads * (v->page_max / 8 + 1) > 2147483647.0)
+             (double)v->layers * v->slots * v->kv_heads * (v->page_max / 4 + 4) > 2147483647.0)
         *why = "cache view too large";
     if (*why) return false;
     o.kv = v->kv;
@@ -459,9 +459,9 @@ HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer
     if (max_nodes < 1 || max_nodes > kTreeMax) return op_fail(err, err_cap, -1, "max_nodes must be 1 .. 64");
     if (!d_len || !d_off || !d_parent || !d_q || !d_out || !d_ws) return op_fail(err, err_cap, -1, "null argument");
     const int el = q_bf16 ? 2 : 4;
-    if (!aligned16(d_q) || !aligned16(d_out) || !aligned16(d_ws) || (q_ld * el) % 16 || (out_ld * el) % 16 ||
+    if (!aligned16(d_q) || !aligned16(d_out) || ((uintptr_t)d_ws & 255) || (q_ld * el) % 16 || (out_ld * el) % 16 ||
         q_ld < (long long)heads * a.v.hd || out_ld < (long long)heads * a.v.hd)
-        return op_fail(err, err_cap, -1, "q, out and the scratch must be 16-byte aligned with rows of heads * hdim or more");
+        return op_fail(err, err_cap, -1, "q and out must be 16-byte aligned with rows of heads * hdim or more, the scratch 256-byte aligned");
     a.layer = layer;
     a.heads = heads;
     a.max_nodes = max_nodes;
@@ -478,6 +478,7 @@ HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer
     if (sms < 1) return op_fail(err, err_cap, -3, "no usable CUDA device");
     const TreeWs ws = tree_ws(a.v, a.G, max_nodes, sms);
     if (ws_bytes < ws.bytes) return op_fail(err, err_cap, -1, "scratch too small");
+    a.out32 = ((uintptr_t)d_out & 31) == 0 && (out_ld * el) % 32 == 0;
     a.roots = (int4 *)d_ws;
     a.lg = lg2(a.G);
     a.part_ml = (float2 *)((char *)d_ws + ws.ml);

@@ -21,12 +21,13 @@ struct TreeArgs {
     long long out_ld;
     float *lse;
     // split columns: the pieces' (max, sum) and unnormalised outputs, and for
-    // each range the column that starts in it and goes on in the next one as
-    // {slot, KV head, first tile, tiles per range}; slot < 0: none
+    // each range the column whose first tile it has and which goes on in the next
+    // one as {slot, KV head, first place, places per range}; slot < 0: none
     int4 *roots;
     float2 *part_ml;
     float *part_o;
-    int lg;  // log2 G
+    int lg;      // log2 G
+    bool out32;  // every output row is 32-byte aligned
     int ranges, row_blocks, min_tiles;
 };
 
@@ -34,13 +35,19 @@ __device__ __forceinline__ void st_row4(float *p, float a, float b, float c, flo
 __device__ __forceinline__ void st_row4(__nv_bfloat16 *p, float a, float b, float c, float d) {
     *(uint2 *)p = make_uint2(pack_bf16(a, b), pack_bf16(c, d));
 }
-// Eight values of a row, 32 (bf16: 16) bytes a lane.
-__device__ __forceinline__ void st_row8(float *p, const float *v, float f) {
-    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0] * f), "f"(v[1] * f), "f"(v[2] * f),
-                 "f"(v[3] * f), "f"(v[4] * f), "f"(v[5] * f), "f"(v[6] * f), "f"(v[7] * f)
-                 : "memory");
+// Eight values of a row, 32 (bf16: 16) bytes a lane; fp32 rows that are only
+// 16-byte aligned (wide false) take two stores.
+__device__ __forceinline__ void st_row8(float *p, const float *v, float f, bool wide) {
+    if (wide) {
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0] * f), "f"(v[1] * f), "f"(v[2] * f),
+                     "f"(v[3] * f), "f"(v[4] * f), "f"(v[5] * f), "f"(v[6] * f), "f"(v[7] * f)
+                     : "memory");
+    } else {
+        st_row4(p, v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+        st_row4(p + 4, v[4] * f, v[5] * f, v[6] * f, v[7] * f);
+    }
 }
-__device__ __forceinline__ void st_row8(__nv_bfloat16 *p, const float *v, float f) {
+__device__ __forceinline__ void st_row8(__nv_bfloat16 *p, const float *v, float f, bool) {
     *(uint4 *)p = make_uint4(pack_bf16(v[0] * f, v[1] * f), pack_bf16(v[2] * f, v[3] * f), pack_bf16(v[4] * f, v[5] * f),
                              pack_bf16(v[6] * f, v[7] * f));
 }
@@ -52,18 +59,29 @@ __device__ __forceinline__ float4 ld_row4(const __nv_bfloat16 *p) {
 }
 
 // Work is cut into tiles of TK cached rows of one (slot, KV head) column, in
-// slot order, and into `ranges` runs of equal length, one per CTA (and row
-// block): every SM gets the same share whatever the lengths are.  A column
-// that ends up in several ranges leaves (max, sum, out) pieces which
-// tree_merge joins.
+// slot order, and into `ranges` runs of equal cost, one per CTA: every SM gets
+// the same share whatever the lengths are.  Starting a column costs about as
+// much as tree_lead tiles, which stand before it in the count and hold no work
+// (without them CTAs with three short columns ended last: 74 -> 61 us at 32
+// slots of 300 to 3000 rows; in the narrow form, where several CTAs share an
+// SM, one or two places took 49.5 us against 47.5 at 256 slots).  A column that ends up in several ranges leaves
+// (max, sum, out) pieces which tree_merge joins.
+template <int TK>
+__host__ __device__ constexpr int tree_lead() { return TK == 128 ? 3 : 0; }
+
 template <int TK>
 struct TreeWalk {
-    int slot, rem, left, g, g0;       // next tile: slot, index within the slot's tiles; tiles left; global index, first
+    static constexpr int LEAD = tree_lead<TK>();
+    int slot, rem, left, g, g0;       // next place: slot, index within the slot's; places left; global index, first
     int L, t0, n, T, at;              // the slot whose numbers are loaded
-    // the segment: tiles a .. b - 1 of column (slot, kvh)
-    int s_slot, s_kvh, s_a, s_b, s_g;
+    // the segment: tiles a .. b - 1 of column (slot, kvh), which starts at place s_c; the segment's own at s_g
+    int s_slot, s_kvh, s_a, s_b, s_g, s_c;
 
     __device__ __forceinline__ static int tiles(int L, int n, int cap) { return n > 0 ? (min(L + n, cap) + TK - 1) / TK : 0; }
+    __device__ __forceinline__ static int places(int L, int n, int cap) {
+        const int t = tiles(L, n, cap);
+        return t > 0 ? t + LEAD : 0;
+    }
     __device__ __forceinline__ bool next(const TreeArgs &a, int first_node) {
         while (left > 0) {
             if (slot >= a.v.slots) return false;
@@ -72,21 +90,23 @@ struct TreeWalk {
                 T = tiles(L, n, a.v.page_max * kPageRows);
                 at = slot;
             }
-            if (rem >= T * a.v.kvh) {
+            const int V = T + LEAD;
+            if (T == 0 || rem >= V * a.v.kvh) {
                 slot++;
                 rem = 0;
                 continue;
             }
+            const int kvh = rem / V, x = rem - kvh * V, c = min(V - x, left);
             s_slot = slot;
-            s_kvh = rem / T;
-            s_a = rem % T;
-            s_b = min(T, s_a + left);
+            s_kvh = kvh;
+            s_a = max(0, x - LEAD);
+            s_b = max(0, x + c - LEAD);
             s_g = g;
-            const int c = s_b - s_a;
+            s_c = g - x;
             left -= c;
             rem += c;
             g += c;
-            if (first_node < n) return true;
+            if (first_node < n && s_b > s_a) return true;
         }
         return false;
     }
@@ -102,7 +122,7 @@ __device__ __forceinline__ void tree_plan(const TreeArgs &a, int range, int *s_s
     for (int s = b0; s < b1; s++) {
         int L, t0, n;
         tree_span(a.v, a.len, a.off, a.max_nodes, s, L, t0, n);
-        sum += TreeWalk<TK>::tiles(L, n, cap) * a.v.kvh;
+        sum += TreeWalk<TK>::places(L, n, cap) * a.v.kvh;
     }
     int incl = sum;
 #pragma unroll
@@ -120,7 +140,7 @@ __device__ __forceinline__ void tree_plan(const TreeArgs &a, int range, int *s_s
     const int C = max((total + a.ranges - 1) / a.ranges, a.min_tiles);
     if (th < NR) {
         const long long g0 = (long long)(range + th) * C;
-        s_start[4 * th + 2] = (int)max(0LL, min((long long)C, total - g0));  // tiles of this range
+        s_start[4 * th + 2] = (int)max(0LL, min((long long)C, total - g0));  // places of this range
         s_start[4 * th + 3] = C;
     }
 #pragma unroll
@@ -131,7 +151,7 @@ __device__ __forceinline__ void tree_plan(const TreeArgs &a, int range, int *s_s
         for (int s = b0; s < b1; s++) {
             int L, t0, n;
             tree_span(a.v, a.len, a.off, a.max_nodes, s, L, t0, n);
-            const int c = TreeWalk<TK>::tiles(L, n, cap) * a.v.kvh;
+            const int c = TreeWalk<TK>::places(L, n, cap) * a.v.kvh;
             if (g0 < at + c) {
                 s_start[4 * i] = s;
                 s_start[4 * i + 1] = (int)g0 - at;
@@ -161,7 +181,7 @@ __device__ __forceinline__ int tree_parent(const TreeArgs &a, int t0, int n, int
 }
 // One segment of a walk, as the softmax warps share it.
 struct TreeSeg {
-    int have, slot, kvh, a, b, g, piece, L, t0, n, T;
+    int have, slot, kvh, a, b, c, piece, L, t0, n, T;
 };
 // Bits of the nodes that node i sees: itself and its ancestors up to the root
 // or to a padding node.  Parents lie below their nodes, so the walk ends.
@@ -457,7 +477,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             x.kvh = v.s_kvh;
             x.a = v.s_a;
             x.b = v.s_b;
-            x.g = v.s_g;
+            x.c = v.s_c;
             x.piece = v.s_g != v.g0;
             x.L = v.L;
             x.t0 = v.t0;
@@ -628,7 +648,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                         const float inv = l == 0.f ? 0.f : 1.0f / l;
                         T *dst = (T *)a.out + (long long)tok * a.out_ld + (long long)head * HD + h * W;
 #pragma unroll
-                        for (int d = 0; d < W; d += 8) st_row8(dst + d, o + d, inv);
+                        for (int d = 0; d < W; d += 8) st_row8(dst + d, o + d, inv, a.out32);
                         if (a.lse && h == 0)
                             a.lse[(long long)tok * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
                     } else {
@@ -636,11 +656,11 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                         if (h == 0) a.part_ml[(size_t)piece * 128 + th] = make_float2(m, l);
                         float *po = a.part_o + (size_t)piece * 128 * HD + h * W * 128 + th * 8;
 #pragma unroll
-                        for (int d = 0; d < W; d += 8) st_row8(po + d * 128, o + d, 1.f);
+                        for (int d = 0; d < W; d += 8) st_row8(po + d * 128, o + d, 1.f, true);
                     }
                 }
             }
-            if (range_root && cur.a == 0 && !whole) a.roots[range] = make_int4(cur.slot, cur.kvh, cur.g, s_start[3]);
+            if (range_root && cur.a == 0 && !whole) a.roots[range] = make_int4(cur.slot, cur.kvh, cur.c, s_start[3]);
             bar_sync(1, kTtSoft);
             seg++;
         }
@@ -1029,7 +1049,7 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
                     if (g == 0 && warp == 0) a.part_ml[piece * (NT * 8) + row] = make_float2(m[nt][j], L);
                 }
             }
-        if (th == 0 && wc.s_a == 0 && !whole) a.roots[range] = make_int4(wc.s_slot, wc.s_kvh, wc.s_g, s_start[3]);
+        if (th == 0 && wc.s_a == 0 && !whole) a.roots[range] = make_int4(wc.s_slot, wc.s_kvh, wc.s_c, s_start[3]);
         __syncthreads();
         if (th == 0) s_bad = 0;
     }
@@ -1051,7 +1071,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constan
     constexpr int D = HD / 32, W = kMergeThreads / 32;
     __shared__ int s_scan[W];
     __shared__ float s_part[W][HD], s_m[W], s_l[W];
-    __shared__ int4 s_col[W], s_at[W];  // a row's {slot, KV head, first tile, tiles per range}, {row, first token, tiles, -}
+    __shared__ int4 s_col[W], s_at[W];  // a row's {slot, KV head, first place, places per range}, {row, first token, tiles, -}
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // rows of the columns that start in this thread's ranges (one column a range at most)
@@ -1107,7 +1127,8 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constan
         const int d0 = lane * D;
         if (on) {
             const int4 root = s_col[mine], me = s_at[mine];
-            const int r = me.x, C = root.w, p0 = root.z / C + part, p1 = (root.z + me.z - 1) / C;
+            const int r = me.x, C = root.w, lead = tree_lead<TK>();
+            const int p0 = (root.z + lead) / C + part, p1 = (root.z + lead + me.z - 1) / C;
             constexpr int B = 4;
             for (int q0 = p0; q0 <= p1; q0 += B * wpr) {  // four pieces in flight
                 float v[B][D];

@@ -8,7 +8,8 @@ them (`evict`).  No counterpart in the reference, whose loop decodes one token
 per step (src/model.c:943-954) over a cache that only grows (:804-808).
 
 All work runs on torch's current stream of the cache's device and nothing
-synchronises.  Shapes, types and strides are checked here and by the library
+synchronises.  tree_attention's scratch is one per stream (a captured call's own, unless its stream has
+one: then a replay must not run beside calls on that stream).  Shapes, types and strides are checked here and by the library
 (`BackendError`); what the arrays hold is not read back: lengths, offsets and
 parents are bounded on the device as the header states.
 """
@@ -118,7 +119,9 @@ class PagedKV:
         if ws is None:
             need = self._lib.hyc_tree_attention_ws(self._ref, heads, max_nodes)
             buf = torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
-            ws = self._ws[(stream, heads, max_nodes)] = (buf, buf.data_ptr(), buf.numel())
+            ws = (buf, buf.data_ptr(), buf.numel())
+            if not torch.cuda.is_current_stream_capturing():  # a graph keeps a scratch of its own
+                self._ws[(stream, heads, max_nodes)] = ws
         self._call(self._lib.hyc_tree_attention, stream, self._ref, layer, heads, max_nodes, ln, of, pa, q.data_ptr(), old,
                    bf16, hd ** -0.5 if scale is None else scale, out.data_ptr(), old_out, lse.data_ptr(), ws[1], ws[2])
         return out, lse

@@ -383,7 +383,8 @@ HYC_API int hyc_attention_decode_noalloc(void *stream, int heads, int kv_heads, 
  *
  * Drafted trees: slot s holds d_len[s] cached rows and drafts the nodes
  * d_off[s] .. d_off[s + 1] - 1 (d_off[0] = 0, at most max_nodes <= 64 a slot,
- * none is fine), whose K and V stand in rows d_len[s] + i.  d_parent[t] is
+ * none is fine), whose K and V stand in rows d_len[s] + i; the token arrays
+ * hold d_off[slots] tokens.  d_parent[t] is
  * the node's parent within its tree, below the node itself (-1, or any number
  * that is not below it: none; -2: a padding node, which sees nothing and is
  * nobody's ancestor).  Rows past a slot's page table do not exist. */
@@ -400,7 +401,7 @@ typedef struct hyc_kv_view {
  * d_out likewise with out_ld and the same type; d_lse (optional) is [tokens]
  * [heads] fp32.  A node that sees no row gets zeros and -inf.  heads /
  * kv_heads in {1, 2, 4, 8}.  d_ws is scratch of at least
- * hyc_tree_attention_ws bytes, 16-byte aligned, used by this call alone until
+ * hyc_tree_attention_ws bytes, 256-byte aligned, used by this call alone until
  * it has run; its contents need no preparation.  K or V of rows that a node
  * does not see never reach its output, whatever they hold. */
 HYC_API int hyc_kvops_timeouts(void);
@@ -431,7 +432,8 @@ HYC_API int hyc_tree_commit(void *stream, const hyc_kv_view *cache, int max_node
  * Query j < n = d_nq[s] (at most max_q <= 64) is token d_sel[s * max_q + j]
  * of d_q, fp32 or bf16, q_ld elements from token to token and q_layer from
  * layer to layer, and of d_lse [layers][lse_layer elements] as [tokens]
- * [heads].  A negative d_sel is left out.  d_acc holds acc_rows rows per (l,
+ * [heads].  A negative d_sel, and a query whose lse is -inf (it saw nothing),
+ * is left out; what d_sel names must exist.  d_acc holds acc_rows rows per (l,
  * s, h), rows from acc_rows on are not accumulated.  The order of the sums
  * is fixed: the same inputs give the same bits. */
 HYC_API int hyc_cache_weights(void *stream, const hyc_kv_view *cache, int heads, int max_q, const int *d_len,

@@ -251,6 +251,60 @@ def test_tree_attention_same_bits_twice_other_stream_graph_and_out():
     assert torch.equal(out, first) and torch.equal(lse, lse1)
 
 
+@pytest.mark.parametrize("n", [1, 6, 40])
+def test_tree_attention_long_sums_do_not_drift(n):
+    """fp32 outputs over 20000 rows: no error that grows with the rows.  Queries, keys and probabilities keep 24 bits and
+    a tile's sum is cut eight times at most at its full size, by 2^-24 of it on average half: 2^-22; scores' errors (as
+    2^-24 of a sum of 128 products of size one, times the score's scale) stay below that.  Bound: 2^-20, where cutting
+    every sum would leave over 2^-16."""
+    import torch
+    from hymt2_b200.kvcache import PagedKV
+    torch.manual_seed(3)
+    S, L, kvh, G, hd = 6, 20000, 2, 4, 128
+    page_max = (L + n + 15) // 16
+    kv = torch.randn(1, S * page_max, 2, 16, kvh, hd, device="cuda").to(torch.bfloat16)
+    pages = torch.randperm(S * page_max, device="cuda").to(torch.int32).view(S, page_max)
+    q = torch.randn(S * n, kvh * G, hd, device="cuda")
+    off = gpu(np.arange(S + 1, dtype=np.int32) * n)
+    par = np.tile(np.arange(-1, n - 1), S).astype(np.int32)
+    out, lse = PagedKV(kv, pages).tree_attention(q, gpu(np.full(S, L, np.int32)), off, gpu(par), n)
+    for s in (0, S - 1):
+        x = kv[0, pages[s].long()].double()  # [pages][2][16][kvh][hd]
+        k, v = (x[:, i].flatten(0, 1)[:L + n] for i in range(2))
+        hide = torch.arange(L + n, device="cuda")[None] > L + torch.arange(n, device="cuda")[:, None]
+        for h in range(kvh * G):
+            y = (q[s * n:(s + 1) * n, h].double() @ k[:, h // G].T * hd ** -0.5).masked_fill(hide, -torch.inf)
+            want = torch.softmax(y, -1) @ v[:, h // G]
+            got = out[s * n:(s + 1) * n, h].double()
+            assert float((got - want).norm() / want.norm()) < 2.0 ** -20
+            assert float((lse[s * n:(s + 1) * n, h].double() - torch.logsumexp(y, -1)).abs().max()) < 2.0 ** -18
+
+
+def test_no_wait_has_given_up():
+    from hymt2_b200.device import load_library
+    assert load_library().hyc_kvops_timeouts() == 0
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n,L", [(3, 900), (40, 200), (40, 3000)])
+def test_tree_attention_rows_of_16_byte_alignment(n, L, bf16):
+    """Queries and outputs whose rows start at odd multiples of 16 bytes (split and unsplit columns, both forms)."""
+    import torch
+    rng = np.random.default_rng(n + L)
+    kvh, G, hd = 2, 4, 128
+    kv, pages = make_cache(rng, 1, kvh, hd, [L + n])
+    par, w = random_tree(rng, n), kvh * G * hd
+    dt = torch.bfloat16 if bf16 else torch.float32
+    step = 8 if bf16 else 4  # 16 bytes
+    q = torch.from_numpy(rng.standard_normal((n, w)).astype(np.float32)).to(dt)
+    want, wlse = run_tree(kv, pages, 0, [L], [par], gpu(q).view(n, kvh * G, hd), n)
+    room_q, room_o = (torch.zeros(n * (w + step) + step, dtype=dt, device="cuda")[step:].view(n, w + step)[:, :w] for _ in range(2))
+    room_q.copy_(q)
+    assert room_q.data_ptr() % 32 == 16 and room_o.data_ptr() % 32 == 16
+    got, lse = run_tree(kv, pages, 0, [L], [par], room_q.view(n, kvh * G, hd), n, out=room_o.view(n, kvh * G, hd))
+    assert np.array_equal(got, want) and np.array_equal(lse, wlse)
+
+
 def test_operators_past_32_bit_offsets():
     """A cache of over 2^32 elements, used at its far end."""
     import torch
