@@ -489,13 +489,18 @@ HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer
     const dim3 mgrid(4 * sms);
     if (ws.narrow) {
         a.min_tiles = kNarrowTiles;
+        // short slots (and columns enough): a column to a CTA, no pieces and no
+        // second kernel
+        const int cap = (a.v.page_max * kPageRows + kTnK - 1) / kTnK;
+        a.whole = cap <= 2 || (cap <= 4 && a.v.slots * a.v.kvh >= sms);
         // as many CTAs as an SM holds (ranges are equal shares, so all of them
         // should run at once), by shared memory and the kernel's register bound
 #define HY_NT(T_, HD_, NT_)                                                                                             \
     if (ws.rows == 8 * NT_) {                                                                                           \
         a.ranges = sms * std::min(kNarrowCtas, (int)(227 * 1024 / (tn_smem<T_, HD_, NT_>() + 2048)));                             \
         e = go(tree_attn_mma<T_, HD_, NT_>, dim3(a.ranges), dim3(kTnThreads), tn_smem<T_, HD_, NT_>(), stream, false, a); \
-        if (e == cudaSuccess) e = go(tree_merge<T_, HD_, kTnK>, mgrid, dim3(kMergeThreads), 0, stream, true, a, ws.rows); \
+        if (e == cudaSuccess && !a.whole)                                                                               \
+            e = go(tree_merge<T_, HD_, kTnK>, mgrid, dim3(kMergeThreads), 0, stream, true, a, ws.rows);                 \
     }
 #define HY_TREE(T_, HD_) HY_NT(T_, HD_, 1) HY_NT(T_, HD_, 2) HY_NT(T_, HD_, 3) HY_NT(T_, HD_, 4)
         if (q_bf16 && a.v.hd == 64) { HY_TREE(__nv_bfloat16, 64) }

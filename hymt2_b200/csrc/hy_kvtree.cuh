@@ -28,6 +28,7 @@ struct TreeArgs {
     float *part_o;
     int lg;      // log2 G
     bool out32;  // every output row is 32-byte aligned
+    bool whole;  // narrow form: whole columns to each range
     int ranges, row_blocks, min_tiles;
 };
 
@@ -81,6 +82,20 @@ struct TreeWalk {
     __device__ __forceinline__ static int places(int L, int n, int cap) {
         const int t = tiles(L, n, cap);
         return t > 0 ? t + LEAD : 0;
+    }
+    // Whole columns instead (a.whole): range r takes columns r, r + ranges, ..., g being the next one.
+    __device__ __forceinline__ bool next_whole(const TreeArgs &a) {
+        while (g < a.v.slots * a.v.kvh) {
+            s_slot = g / a.v.kvh;
+            s_kvh = g - s_slot * a.v.kvh;
+            g += a.ranges;
+            tree_span(a.v, a.len, a.off, a.max_nodes, s_slot, L, t0, n);
+            T = tiles(L, n, a.v.page_max * kPageRows);
+            s_a = 0;
+            s_b = T;
+            if (T > 0) return true;
+        }
+        return false;
     }
     __device__ __forceinline__ bool next(const TreeArgs &a, int first_node) {
         while (left > 0) {
@@ -735,15 +750,20 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
     const int th = threadIdx.x, warp = th >> 5, lane = th & 31, g = lane >> 2, tq = lane & 3, range = blockIdx.x;
     pdl_trigger();
     pdl_wait();
-    tree_plan<kTnK, 1>(a, range, s_scan, s_start);
-    if (th == 0) {
-        a.roots[range] = make_int4(-1, 0, 0, 0);
-        s_bad = 0;
+    TreeWalk<kTnK> wi;
+    if (a.whole) {
+        wi.g = range;
+    } else {
+        tree_plan<kTnK, 1>(a, range, s_scan, s_start);
+        wi = tree_walk<kTnK>(s_start, range);
+        if (th == 0) a.roots[range] = make_int4(-1, 0, 0, 0);
     }
+    if (th == 0) s_bad = 0;  // first used after the barriers of the first tile
+    const auto step = [&](TreeWalk<kTnK> &w) { return a.whole ? w.next_whole(a) : w.next(a, 0); };
     const int cap = a.v.page_max * kPageRows;
     const float sl2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);
-    TreeWalk<kTnK> wi = tree_walk<kTnK>(s_start, range), wc = wi;
-    bool more = wi.next(a, 0);
+    TreeWalk<kTnK> wc = wi;
+    bool more = step(wi);
     int it = more ? wi.s_a : 0;  // the tile to copy next, of column wi
     const uint16_t *src[kTnK / kPageRows];  // its pages' K rows of this thread (first row and chunk), null: no page
     const int cc = th % CH, cr = th / CH;   // this thread's chunk of a row, and its first row of a copy step's
@@ -775,7 +795,7 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
     pages();
     copy(0);
     copy(1);
-    while (wc.next(a, 0)) {
+    while (step(wc)) {
         const int rows = wc.n << a.lg, end = min(wc.L + wc.n, cap);
         // parents, and the queries as B fragments: lane (g, t) holds row g, dims 2t, 2t + 1, 2t + 8, 2t + 9 of 16
         if (th < kTreeMax) s_up[th] = (int8_t)tree_parent(a, wc.t0, wc.n, th);
@@ -831,7 +851,7 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
             const int r0 = t * kTnK;
             const bool tail = r0 + kTnK > wc.L;
             if (++it == wi.s_b) {  // the copies' next tile, and its pages on their way
-                more = wi.next(a, 0);
+                more = step(wi);
                 it = wi.s_a;
             }
             pages();
