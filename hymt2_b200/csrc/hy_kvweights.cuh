@@ -273,36 +273,44 @@ __global__ void __launch_bounds__(kWtThreads, 1) cache_weights_tc(const __grid_c
                     if (lane == 0) s_counts[qb] = ok;
                 }
                 uint8_t *dst0 = sq + qb * qbuf_b;
-                const int half = HD == 128 ? lane >> 4 : 0, c = (lane & 15) * 4;
-                const T *src0 = (const T *)a.q + w.s_layer * a.q_layer + (long long)w.s_kvh * a.G * HD + half * 64 + c;
-                constexpr int B = 4;
-                for (int r0 = wl; r0 < N; r0 += 4 * B) {  // a warp to a row, four rows in flight (eight: 74 -> 95 us at 31 queries)
-                    float4 q[B];
+                if constexpr (sizeof(T) == 2) {
+                    // bf16 rows as they are, 16 bytes a copy, all in flight
+                    constexpr int CH = HD / 8;
+                    const T *src0 = (const T *)a.q + w.s_layer * a.q_layer + (long long)w.s_kvh * a.G * HD;
+                    for (int e = th; e < N * CH; e += 128) {
+                        const int r = e / CH, c = e % CH, t = s_tok[r];
+                        const uint32_t dst = kv_smem(dst0 + (c >> 3) * half_b + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
+                                     "l"(src0 + (t >= 0 ? t * a.q_ld + ((q0 + r) & (a.G - 1)) * HD + c * 8 : 0)), "r"(t >= 0 ? 16 : 0)
+                                     : "memory");
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                } else {
+                    const int half = HD == 128 ? lane >> 4 : 0, c = (lane & 15) * 4;
+                    const T *src0 = (const T *)a.q + w.s_layer * a.q_layer + (long long)w.s_kvh * a.G * HD + half * 64 + c;
+                    constexpr int B = 4;
+                    for (int r0 = wl; r0 < N; r0 += 4 * B) {  // a warp to a row, four rows in flight (eight: 74 -> 95 us at 31 queries)
+                        float4 q[B];
 #pragma unroll
-                    for (int i = 0; i < B; i++) {
-                        const int r = r0 + 4 * i, t = r < N ? s_tok[r] : -1;
-                        q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (t >= 0 && (HD == 128 || lane < 16)) {
-                            const T *src = src0 + t * a.q_ld + ((q0 + r) & (a.G - 1)) * HD;
-                            if constexpr (sizeof(T) == 4) {
+                        for (int i = 0; i < B; i++) {
+                            const int r = r0 + 4 * i, t = r < N ? s_tok[r] : -1;
+                            q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (t >= 0 && (HD == 128 || lane < 16)) {
+                                const T *src = src0 + t * a.q_ld + ((q0 + r) & (a.G - 1)) * HD;
                                 q[i] = *(const float4 *)src;
-                            } else {
-                                const uint2 u = *(const uint2 *)src;
-                                q[i] = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u),
-                                                   __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
                             }
                         }
-                    }
 #pragma unroll
-                    for (int i = 0; i < B; i++) {
-                        const int r = r0 + 4 * i;
-                        if (r < N && (HD == 128 || lane < 16)) {
-                            uint32_t lo[QT], hi[QT];
-                            split_bf16<QT>(q[i].x, q[i].y, lo);
-                            split_bf16<QT>(q[i].z, q[i].w, hi);
-                            uint8_t *dst = dst0 + half * half_b + r * 128 + ((((c >> 3) ^ (r & 7)) << 4) | ((c & 4) << 1));
+                        for (int i = 0; i < B; i++) {
+                            const int r = r0 + 4 * i;
+                            if (r < N && (HD == 128 || lane < 16)) {
+                                uint32_t lo[QT], hi[QT];
+                                split_bf16<QT>(q[i].x, q[i].y, lo);
+                                split_bf16<QT>(q[i].z, q[i].w, hi);
+                                uint8_t *dst = dst0 + half * half_b + r * 128 + ((((c >> 3) ^ (r & 7)) << 4) | ((c & 4) << 1));
 #pragma unroll
-                            for (int x = 0; x < QT; x++) *(uint2 *)(dst + x * term_b) = make_uint2(lo[x], hi[x]);
+                                for (int x = 0; x < QT; x++) *(uint2 *)(dst + x * term_b) = make_uint2(lo[x], hi[x]);
+                            }
                         }
                     }
                 }
