@@ -59,7 +59,9 @@ bool make_view(const hyc_kv_view *v, KvView &o, const char **why) {
 
 int lg2(int G) { return G == 1 ? 0 : G == 2 ? 1 : G == 4 ? 2 : 3; }
 
-// Rows (nodes x heads of a group) up to which a tree takes the narrow form,
+// Rows (nodes x heads of a group) up to which a tree takes the narrow form
+// (its own limit: four 8-row columns of registers; at 20 rows over 256 short
+// slots it took 53 us where the wide form took 67),
 // the least tiles of one of its ranges, and its most CTAs an SM.
 constexpr int kNarrowRows = 32, kNarrowTiles = 1, kNarrowCtas = 3;
 
@@ -146,6 +148,8 @@ struct CommitArgs {
 // thread c owns 16 bytes of a K or V row and moves the path's rows in order.
 // Row j of the path comes from row path[j] >= j, so a row is read before
 // anything is written over it.  CTAs of layer 0 write the outcome.
+// Bound by latency: a few dependent loads, then one row after the other (32
+// layers x 128 slots 10 us, one slot 6 us of kernel time).
 __global__ void __launch_bounds__(128) tree_commit(const __grid_constant__ CommitArgs a) {
     __shared__ int s_path[kTreeMax], s_n, s_last;
     const int s = blockIdx.x, layer = blockIdx.y, lane = threadIdx.x & 31;
@@ -233,8 +237,9 @@ __device__ __forceinline__ uint32_t weight_key(float v) {
 // and 10 bits: the first one's bins hold the sign, the exponent and two more
 // bits, so that weights of a few magnitudes spread over many bins (by bytes,
 // nearly all fell into three, and their shared-memory additions into one
-// another: 47 us for 768 columns of 6100 rows).  A warp whose keys all fall
-// into one bin adds them once.
+// another).  A warp whose keys all fall into one bin adds them once.  768
+// columns of up to 6100 rows take 38 us, 128 of 4096 rows 12 us: passes over
+// rows that the L1 holds, one latency after the other.
 constexpr int kSelBins = 2048;
 __global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constant__ EvictArgs a) {
     __shared__ unsigned hist[kSelBins], wsum[2][kSelThreads / 32];
@@ -367,7 +372,11 @@ __global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constan
 }
 
 // grid (layers * slots * kv heads, row blocks): a warp copies K (lanes 0-15)
-// and V (lanes 16-31) of one kept row, 16 bytes a lane (hd 64: 8).
+// and V (lanes 16-31) of one kept row, 16 bytes a lane (hd 64: 8).  1.15 GB (24
+// slots x 8 layers, 1500 rows kept) take 197 us, 5.9 TB/s.  Four rows in flight
+// a warp took 274 us with the selection against 239 (the rows' places in memory
+// then spread), selection and copy in one kernel 251, the last rows' copy beside
+// the selection 282.
 constexpr int kGatherRows = 128;
 __global__ void __launch_bounds__(256) evict_gather(const __grid_constant__ EvictArgs a) {
     const int idx = blockIdx.x, kvh = idx % a.v.kvh, s = (idx / a.v.kvh) % a.v.slots, layer = idx / (a.v.kvh * a.v.slots);
@@ -490,7 +499,8 @@ HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer
     if (ws.narrow) {
         a.min_tiles = kNarrowTiles;
         // short slots (and columns enough): a column to a CTA, no pieces and no
-        // second kernel
+        // second kernel (256 slots of 192 rows 47.4 -> 45.8 us; one of 64 rows
+        // 15.5 -> 13.7, the host's launch); longer slots would leave SMs idle
         const int cap = (a.v.page_max * kPageRows + kTnK - 1) / kTnK;
         a.whole = cap <= 2 || (cap <= 4 && a.v.slots * a.v.kvh >= sms);
         // as many CTAs as an SM holds (ranges are equal shares, so all of them
