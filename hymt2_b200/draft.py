@@ -54,12 +54,12 @@ class DraftStats:
 
 
 def generate(dm, prompts, max_new: int, draft=None, stop=(), budget: int = 0, sinks: int = 4, recent: int = 32,
-             window: int = 16):
+             window: int = 16, slack: int = 32):
     """Greedy ids for a few prompts at once, one slot each (dm.batch_prepare and dm.tree_prepare done before).
 
-    draft(ids) -> (tokens, parents): a tree whose node 0 is ids[-1].  budget > 0 bounds every slot's cache; the last
-    `window` prompt tokens then go through a tree pass, so that their queries' weights are counted.  Returns (ids per
-    prompt, DraftStats)."""
+    draft(ids) -> (tokens, parents): a tree whose node 0 is ids[-1].  budget > 0 bounds every slot's cache: it is cut
+    back to budget rows when it has over `slack` more (a cut copies what stays).  The last `window` prompt tokens then
+    go through a tree pass, so that their queries' weights are counted.  Returns (ids per prompt, DraftStats)."""
     draft = draft or PromptLookup()
     stop, n = set(int(t) for t in stop), len(prompts)
     ids = [[int(t) for t in p] for p in prompts]
@@ -79,7 +79,7 @@ def generate(dm, prompts, max_new: int, draft=None, stop=(), budget: int = 0, si
     out: list[list[int]] = [[] for _ in range(n)]
     live = [s for s in range(n) if max_new > 0]
     while live:
-        if budget and max(dm.tree_state(s)[0] for s in live) > budget:
+        if budget and max(dm.tree_state(s)[0] for s in live) > budget + slack:
             dm.tree_evict(budget, sinks, recent)
             stats.evictions += 1
         trees = {}
@@ -125,6 +125,7 @@ def main(argv=None) -> None:
     rng = np.random.default_rng(7)
     phrase = rng.integers(0, min(1000, dm.vocab_out), 24)
     prompt = np.where(rng.random(a.prompt) < 0.05, rng.integers(0, min(1000, dm.vocab_out), a.prompt), np.resize(phrase, a.prompt))
+    generate(dm, [prompt[:64].tolist()], 2, PromptLookup(nodes=a.nodes), budget=a.budget)  # first uses lay weights out
     t = time.perf_counter()
     out, st = generate(dm, [prompt.tolist()], a.new, PromptLookup(nodes=a.nodes), budget=a.budget)
     dt = time.perf_counter() - t
