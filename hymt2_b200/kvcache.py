@@ -100,14 +100,14 @@ class PagedKV:
         old = st[0] if nt > 1 else heads * hd
         old_out = heads * hd
         if out is None:
-            out = q.new_empty((nt, heads, hd))
+            out = q.new_empty(nt, heads, hd)
         elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != self._dev or out.stride(2) != 1 or \
                 out.stride(1) != hd:
             raise ValueError("out must be shaped and typed like q with contiguous tokens")
         elif nt > 1:
             old_out = out.stride(0)
         if lse is None:
-            lse = q.new_empty((nt, heads), dtype=torch.float32)
+            lse = q.new_empty(nt, heads, dtype=torch.float32) if bf16 else q.new_empty(nt, heads)
         else:
             self._floats("lse", lse, (nt, heads))
         ln, of = self._ints("lens", lens, (self.slots,)), self._ints("offsets", offsets, (self.slots + 1,))
@@ -136,11 +136,10 @@ class PagedKV:
         args = (self._ints("lens", lens, one), self._ints("offsets", offsets, (self.slots + 1,)), self._ints("parent", parent, nt),
                 self._ints("tokens", tokens, nt), self._ints("next_tokens", next_tokens, nt),
                 None if forced is None else self._ints("forced", forced, one))
-        n = lens.new_empty((3, self.slots))
-        path = lens.new_empty((self.slots, max(max_nodes, 0)))
-        p, step = n.data_ptr(), 4 * self.slots
-        self._call(self._lib.hyc_tree_commit, self._stream(), self._ref, max_nodes, *args, p, p + step, path.data_ptr(), p + 2 * step)
-        new_lens, accepted, bonus = n.unbind()
+        new_lens, accepted, bonus = lens.new_empty(self.slots), lens.new_empty(self.slots), lens.new_empty(self.slots)
+        path = lens.new_empty(self.slots, max(max_nodes, 0))
+        self._call(self._lib.hyc_tree_commit, self._stream(), self._ref, max_nodes, *args, new_lens.data_ptr(),
+                   accepted.data_ptr(), path.data_ptr(), bonus.data_ptr())
         return new_lens, accepted, path, bonus
 
     def add_weights(self, acc: torch.Tensor, q: torch.Tensor, lse: torch.Tensor, lens: torch.Tensor,
@@ -175,8 +174,8 @@ class PagedKV:
         w = self._floats("acc", acc, (self.layers, self.slots, self.kv_heads, acc.shape[3]))
         ln = self._ints("lens", lens, (self.slots,))
         out = lens.new_empty(self.slots)
-        kept = lens.new_empty((self.layers, self.slots, self.kv_heads, budget))
-        kw = acc.new_empty((self.layers, self.slots, self.kv_heads, budget))
+        kept = lens.new_empty(self.layers, self.slots, self.kv_heads, budget)
+        kw = acc.new_empty(self.layers, self.slots, self.kv_heads, budget)
         self._call(self._lib.hyc_cache_evict, self._stream(), self._ref, dst._ref, ln, w, acc.shape[3], budget, sinks, recent,
                    out.data_ptr(), kept.data_ptr(), kw.data_ptr())
         return out, kept, kw
