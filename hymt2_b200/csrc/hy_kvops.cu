@@ -61,9 +61,8 @@ int lg2(int G) { return G == 1 ? 0 : G == 2 ? 1 : G == 4 ? 2 : 3; }
 
 // Rows (nodes x heads of a group) up to which a tree takes the narrow form
 // (its own limit: four 8-row columns of registers; at 20 rows over 256 short
-// slots it took 53 us where the wide form took 67),
-// the least tiles of one of its ranges, and its most CTAs an SM.
-constexpr int kNarrowRows = 32, kNarrowTiles = 1, kNarrowCtas = 3;
+// slots it took 53 us where the wide form took 67), and its most CTAs an SM.
+constexpr int kNarrowRows = 32, kNarrowCtas = 3;
 
 bool group_ok(int heads, int kvh, int &G) {
     if (heads < 1 || heads % kvh) return false;
@@ -497,7 +496,6 @@ HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer
     cudaError_t e = cudaErrorInvalidValue;
     const dim3 mgrid(4 * sms);
     if (ws.narrow) {
-        a.min_tiles = kNarrowTiles;
         // short slots (and columns enough): a column to a CTA, no pieces and no
         // second kernel (256 slots of 192 rows 47.4 -> 45.8 us; one of 64 rows
         // 15.5 -> 13.7, the host's launch); longer slots would leave SMs idle
@@ -521,7 +519,6 @@ HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer
 #undef HY_NT
         return done(e, err, err_cap);
     }
-    a.min_tiles = 1;
     CUtensorMap map;
     if (!page_map(a.v, &map)) return op_fail(err, err_cap, -3, "cuTensorMapEncodeTiled failed");
     const dim3 grid(ws.ranges * ws.row_blocks);

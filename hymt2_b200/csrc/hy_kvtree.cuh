@@ -29,7 +29,7 @@ struct TreeArgs {
     int lg;      // log2 G
     bool out32;  // every output row is 32-byte aligned
     bool whole;  // narrow form: whole columns to each range
-    int ranges, row_blocks, min_tiles;
+    int ranges, row_blocks;
 };
 
 __device__ __forceinline__ void st_row4(float *p, float a, float b, float c, float d) { *(float4 *)p = make_float4(a, b, c, d); }
@@ -152,7 +152,7 @@ __device__ __forceinline__ void tree_plan(const TreeArgs &a, int range, int *s_s
         if (i < w) before += s_scan[i];
         total += s_scan[i];
     }
-    const int C = max((total + a.ranges - 1) / a.ranges, a.min_tiles);
+    const int C = max((total + a.ranges - 1) / a.ranges, 1);
     if (th < NR) {
         const long long g0 = (long long)(range + th) * C;
         s_start[4 * th + 2] = (int)max(0LL, min((long long)C, total - g0));  // places of this range
@@ -346,111 +346,111 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
     const bool range_root = rb == 0 && threadIdx.x == 0;  // the thread that notes the range's split column
     if (range_root) a.roots[range] = make_int4(-1, 0, 0, 0);
     if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTtRegsFeed));
-    if (warp == 8) {
-        // eight pages a tile, K then V; a page that does not exist is read past
-        // the end of the map, which fills zeros
-        const int y0 = a.layer * a.v.npages * 2 * kPageRows, yend = a.v.layers * a.v.npages * 2 * kPageRows;
-        int pos = 0;
-        RingPos at;
-        while (w.next(a, node0)) {
-            const int pages = (min(w.L + w.n, cap) + kPageRows - 1) / kPageRows;
-            // the segment's queries towards L2: the softmax warps load them when
-            // the segment before has used its own
-            for (int i = lane; i < (min(NB, w.n - node0) << a.lg) * (HD * (int)sizeof(T) / 128); i += 32) {
-                const int e = i * (128 / (int)sizeof(T)), r = e / HD;
-                const T *q = (const T *)a.q + (long long)(w.t0 + node0 + (r >> a.lg)) * a.q_ld +
-                             (long long)(w.s_kvh * a.G + (r & (a.G - 1))) * HD + e % HD;
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
-            }
-            for (int t = w.s_a; t < w.s_b; t++) {
-                const int j = t * (kTtK / kPageRows) + (lane & 7);
-                const int pg = j < pages ? __ldg(a.v.pages + (size_t)w.s_slot * a.v.page_max + j) : -1;
-                const int y = pg < 0 || pg >= a.v.npages ? yend : y0 + pg * 2 * kPageRows;
-                for (int kv = 0; kv < 2; kv++, pos++, at.next(NST)) {
-                    const int st = at.st;
-                    mb_wait(&empty[st], at.use ^ 1, &s_stop);  // passes on a stage's first use
-                    if (__any_sync(0xffffffffu, *(volatile int *)&s_stop)) break;
-                    int yj[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) yj[i] = __shfl_sync(0xffffffffu, y == yend ? yend : y + kv * kPageRows, i);
-                    if (elect()) {
-                        mb_expect(&full[st], STB);
-#pragma unroll
-                        for (int i = 0; i < 8; i++)
-#pragma unroll
-                            for (int h = 0; h < NH; h++)
-                                tma_box(ring + (size_t)st * STB + h * 16384 + i * 2048, &map, w.s_kvh * HD + h * 64, yj[i], &full[st]);
-                    }
-                    __syncwarp();
-                }
-            }
-        }
-        // copies in flight land before the kernel ends, also after a wait gave up
-        for (int p = max(0, pos - NST); p < pos; p++) {
-            int none = 0;  // never set: the wait itself is bounded
-            mb_wait(&full[p % NST], (p / NST) & 1, &none);
-        }
-    } else if (warp == 9) {
-        {
-            constexpr uint32_t iqk = um_idesc(128, kTtK, false), ipv = um_idesc(128, HD, true);
-            const uint32_t ring0 = __shfl_sync(0xffffffffu, kv_smem(ring), 0), q0 = um_desc_lo(__shfl_sync(0xffffffffu, kv_smem(sq), 0), 16);
-            int it = 0, seg = 0;  // tiles and segments done
-            RingPos at_k, at_v;   // K and V of the next tiles
-            at_v.next(NST);
-            // O += P(i) . V(i), or O = ...; the segment's first one also waits for the last segment's O to be read
-            auto pv = [&](int i, bool first) {
-                const int st = at_v.st;
-                mb_wait(&pfull[i & 1], (i >> 1) & 1, &s_stop);
-                mb_wait(&full[st], at_v.use, &s_stop);
-                at_v.next(NST, 2);
-                if (first && seg > 0) mb_wait(&ofree, (seg - 1) & 1, &s_stop);
-                um_fence_after();
-                const bool fresh = s_fresh[i & 1];
-                const uint32_t vb = um_desc_lo(ring0 + st * STB, 16384), p0 = tmem + kTtS + (i & 1) * 128, px = tmem + kTtX + (i & 1) * 64;
-                if (elect()) {
-#pragma unroll
-                    for (int x = PT - 1; x >= 0; x--)  // small terms first
-#pragma unroll
-                        for (int k = 0; k < kTtK / 16; k++)
-                            um_mma_ts(tmem + kTtO, (x == 2 ? px : p0 + x * 64) + k * 8, vb + k * (2048 / 16), ipv,
-                                      x == PT - 1 && k == 0 ? !fresh : true);
-                    um_commit(&empty[st]);
-                    um_commit(&odone[i & 1]);
-                }
-                __syncwarp();
-            };
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTtRegsFeed));
+        if (warp == 8) {
+            // eight pages a tile, K then V; a page that does not exist is read past
+            // the end of the map, which fills zeros
+            const int y0 = a.layer * a.v.npages * 2 * kPageRows, yend = a.v.layers * a.v.npages * 2 * kPageRows;
+            int pos = 0;
+            RingPos at;
             while (w.next(a, node0)) {
-                for (int t = w.s_a; t < w.s_b; t++, it++) {
-                    const int st = at_k.st;
-                    if (t == w.s_a) mb_wait(&qfull, seg & 1, &s_stop);
-                    mb_wait(&full[st], at_k.use, &s_stop);
-                    at_k.next(NST, 2);
+                const int pages = (min(w.L + w.n, cap) + kPageRows - 1) / kPageRows;
+                // the segment's queries towards L2: the softmax warps load them when
+                // the segment before has used its own
+                for (int i = lane; i < (min(NB, w.n - node0) << a.lg) * (HD * (int)sizeof(T) / 128); i += 32) {
+                    const int e = i * (128 / (int)sizeof(T)), r = e / HD;
+                    const T *q = (const T *)a.q + (long long)(w.t0 + node0 + (r >> a.lg)) * a.q_ld +
+                                 (long long)(w.s_kvh * a.G + (r & (a.G - 1))) * HD + e % HD;
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+                }
+                for (int t = w.s_a; t < w.s_b; t++) {
+                    const int j = t * (kTtK / kPageRows) + (lane & 7);
+                    const int pg = j < pages ? __ldg(a.v.pages + (size_t)w.s_slot * a.v.page_max + j) : -1;
+                    const int y = pg < 0 || pg >= a.v.npages ? yend : y0 + pg * 2 * kPageRows;
+                    for (int kv = 0; kv < 2; kv++, pos++, at.next(NST)) {
+                        const int st = at.st;
+                        mb_wait(&empty[st], at.use ^ 1, &s_stop);  // passes on a stage's first use
+                        if (__any_sync(0xffffffffu, *(volatile int *)&s_stop)) break;
+                        int yj[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) yj[i] = __shfl_sync(0xffffffffu, y == yend ? yend : y + kv * kPageRows, i);
+                        if (elect()) {
+                            mb_expect(&full[st], STB);
+#pragma unroll
+                            for (int i = 0; i < 8; i++)
+#pragma unroll
+                                for (int h = 0; h < NH; h++)
+                                    tma_box(ring + (size_t)st * STB + h * 16384 + i * 2048, &map, w.s_kvh * HD + h * 64, yj[i], &full[st]);
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+            // copies in flight land before the kernel ends, also after a wait gave up
+            for (int p = max(0, pos - NST); p < pos; p++) {
+                int none = 0;  // never set: the wait itself is bounded
+                mb_wait(&full[p % NST], (p / NST) & 1, &none);
+            }
+        } else if (warp == 9) {
+            {
+                constexpr uint32_t iqk = um_idesc(128, kTtK, false), ipv = um_idesc(128, HD, true);
+                const uint32_t ring0 = __shfl_sync(0xffffffffu, kv_smem(ring), 0), q0 = um_desc_lo(__shfl_sync(0xffffffffu, kv_smem(sq), 0), 16);
+                int it = 0, seg = 0;  // tiles and segments done
+                RingPos at_k, at_v;   // K and V of the next tiles
+                at_v.next(NST);
+                // O += P(i) . V(i), or O = ...; the segment's first one also waits for the last segment's O to be read
+                auto pv = [&](int i, bool first) {
+                    const int st = at_v.st;
+                    mb_wait(&pfull[i & 1], (i >> 1) & 1, &s_stop);
+                    mb_wait(&full[st], at_v.use, &s_stop);
+                    at_v.next(NST, 2);
+                    if (first && seg > 0) mb_wait(&ofree, (seg - 1) & 1, &s_stop);
                     um_fence_after();
-                    const uint32_t kb = um_desc_lo(ring0 + st * STB, 16), s0 = tmem + kTtS + (it & 1) * 128;
+                    const bool fresh = s_fresh[i & 1];
+                    const uint32_t vb = um_desc_lo(ring0 + st * STB, 16384), p0 = tmem + kTtS + (i & 1) * 128, px = tmem + kTtX + (i & 1) * 64;
                     if (elect()) {
 #pragma unroll
-                        for (int x = QT - 1; x >= 0; x--)
+                        for (int x = PT - 1; x >= 0; x--)  // small terms first
 #pragma unroll
-                            for (int k = 0; k < HD / 16; k++) {
-                                um_mma(s0, q0 + (x * QTB + (k >> 2) * QH + (k & 3) * 32) / 16, kb + ((k >> 2) * 16384 + (k & 3) * 32) / 16, iqk,
-                                       !(x == QT - 1 && k == 0));
-                            }
+                            for (int k = 0; k < kTtK / 16; k++)
+                                um_mma_ts(tmem + kTtO, (x == 2 ? px : p0 + x * 64) + k * 8, vb + k * (2048 / 16), ipv,
+                                          x == PT - 1 && k == 0 ? !fresh : true);
                         um_commit(&empty[st]);
-                        um_commit(&sfull[it & 1]);
+                        um_commit(&odone[i & 1]);
                     }
                     __syncwarp();
-                    if (t > w.s_a) pv(it - 1, t - 1 == w.s_a);
+                };
+                while (w.next(a, node0)) {
+                    for (int t = w.s_a; t < w.s_b; t++, it++) {
+                        const int st = at_k.st;
+                        if (t == w.s_a) mb_wait(&qfull, seg & 1, &s_stop);
+                        mb_wait(&full[st], at_k.use, &s_stop);
+                        at_k.next(NST, 2);
+                        um_fence_after();
+                        const uint32_t kb = um_desc_lo(ring0 + st * STB, 16), s0 = tmem + kTtS + (it & 1) * 128;
+                        if (elect()) {
+#pragma unroll
+                            for (int x = QT - 1; x >= 0; x--)
+#pragma unroll
+                                for (int k = 0; k < HD / 16; k++) {
+                                    um_mma(s0, q0 + (x * QTB + (k >> 2) * QH + (k & 3) * 32) / 16, kb + ((k >> 2) * 16384 + (k & 3) * 32) / 16, iqk,
+                                           !(x == QT - 1 && k == 0));
+                                }
+                            um_commit(&empty[st]);
+                            um_commit(&sfull[it & 1]);
+                        }
+                        __syncwarp();
+                        if (t > w.s_a) pv(it - 1, t - 1 == w.s_a);
+                    }
+                    pv(it - 1, w.s_b - 1 == w.s_a);
+                    seg++;
                 }
-                pv(it - 1, w.s_b - 1 == w.s_a);
-                seg++;
+                if (elect()) um_commit(&fin);
+                __syncwarp();
+                int none = 0;
+                mb_wait(&fin, 0, &none);
             }
-            if (elect()) um_commit(&fin);
-            __syncwarp();
-            int none = 0;
-            mb_wait(&fin, 0, &none);
         }
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTtRegsSoft));
         const int th = threadIdx.x & 127, h = warp >> 2;  // row, and half of its keys and dims

@@ -162,7 +162,7 @@ __device__ __forceinline__ void um_mma_ts(uint32_t d, uint32_t a, uint32_t blo, 
         "r"(a), "r"(blo), "r"(idesc), "r"((int)acc), "r"(kUmDescHi)
         : "memory");
 }
-// 32 lanes x 32 columns of 32-bit words from / 16 columns to this warp's lane quarter.
+// 32 lanes x 32 or 16 columns of 32-bit words from, or 16 to, this warp's lane quarter.
 __device__ __forceinline__ void um_ld32(uint32_t t, float *r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
@@ -180,15 +180,6 @@ __device__ __forceinline__ void um_ld16(uint32_t t, float *r) {
         : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
           "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
         : "r"(t)
-        : "memory");
-}
-__device__ __forceinline__ void um_st32(uint32_t t, const float *r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]),
-        "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]), "f"(r[10]), "f"(r[11]), "f"(r[12]), "f"(r[13]),
-        "f"(r[14]), "f"(r[15]), "f"(r[16]), "f"(r[17]), "f"(r[18]), "f"(r[19]), "f"(r[20]), "f"(r[21]), "f"(r[22]),
-        "f"(r[23]), "f"(r[24]), "f"(r[25]), "f"(r[26]), "f"(r[27]), "f"(r[28]), "f"(r[29]), "f"(r[30]), "f"(r[31]), "r"(t)
         : "memory");
 }
 __device__ __forceinline__ void um_st16(uint32_t t, const uint32_t *r) {
