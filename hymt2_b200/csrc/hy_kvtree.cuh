@@ -647,9 +647,12 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             // every S of the segment is done, so the next one's Q may go in
             // while the last P . V runs
             if (s_seg[(seg + 1) & 1].have) load_q(s_seg[(seg + 1) & 1]);
-            s_half[h][th] = l;
+            // the halves' sums, each in the word that this thread itself read the
+            // other half's last maximum from (the word of its own maximum may
+            // still be read by the other half, which no barrier has held since)
+            s_half[h ^ 1][th] = l;
             bar_sync(1, kTtSoft);  // and s_bad is complete
-            l = h ? s_half[0][th] + l : l + s_half[1][th];
+            l = h ? s_half[1][th] + l : l + s_half[0][th];
             const unsigned long long bad = s_bad[seg & 1][h] & mask;
             if (th == 0) s_bad[(seg + 1) & 1][h] = 0;
             const bool whole = cur.a == 0 && t1 == cur.T;
