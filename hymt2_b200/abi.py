@@ -131,8 +131,11 @@ SIGNATURES = {
     "hyc_kvops_timeouts": (I, []),
     "hyc_tree_attention_ws": (Z, [KV, I, I]),
     "hyc_tree_attention": (I, [P, KV, I, I, I, P, P, P, P, LL, I, F, P, LL, P, P, Z, C.c_char_p, I]),
+    "hyc_tree_attention_n": (I, [P, KV, I, I, I, I, P, P, P, P, LL, I, F, P, LL, P, P, Z, C.c_char_p, I]),
     "hyc_tree_commit": (I, [P, KV, I, P, P, P, P, P, P, P, P, P, P, C.c_char_p, I]),
+    "hyc_tree_commit_n": (I, [P, KV, I, I, P, P, P, P, P, P, P, P, P, P, C.c_char_p, I]),
     "hyc_cache_weights": (I, [P, KV, I, I, P, P, P, P, LL, LL, I, P, LL, F, P, I, C.c_char_p, I]),
+    "hyc_cache_weights_n": (I, [P, KV, I, I, I, P, P, P, P, LL, LL, I, P, LL, F, P, I, C.c_char_p, I]),
     "hyc_cache_evict": (I, [P, KV, KV, P, P, I, I, I, I, P, P, P, C.c_char_p, I]),
     "hyc_attention_test": (I, [P, I, I, I, I, I, I, F, P, P, P, P, P, P, P, P]),
 }

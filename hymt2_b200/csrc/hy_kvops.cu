@@ -11,6 +11,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -51,6 +52,7 @@ bool make_view(const hyc_kv_view *v, KvView &o, const char **why) {
     o.hd = v->hdim;
     o.slots = v->slots;
     o.page_max = v->page_max;
+    o.tokens = INT_MAX;
     o.kvd = v->kv_heads * v->hdim;
     o.page_stride = 2LL * kPageRows * o.kvd;
     o.layer_stride = o.npages * o.page_stride;
@@ -455,13 +457,15 @@ HYC_API size_t hyc_tree_attention_ws(const hyc_kv_view *cache, int heads, int ma
     return tree_ws(v, G, max_nodes, sms > 0 ? sms : 148).bytes;
 }
 
-HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer, int heads, int max_nodes,
-                               const int *d_len, const int *d_off, const int *d_parent, const void *d_q,
-                               long long q_ld, int q_bf16, float scale, void *d_out, long long out_ld, float *d_lse,
-                               void *d_ws, size_t ws_bytes, char *err, int err_cap) {
+HYC_API int hyc_tree_attention_n(void *stream, const hyc_kv_view *cache, int layer, int heads, int max_nodes, int tokens,
+                                 const int *d_len, const int *d_off, const int *d_parent, const void *d_q,
+                                 long long q_ld, int q_bf16, float scale, void *d_out, long long out_ld, float *d_lse,
+                                 void *d_ws, size_t ws_bytes, char *err, int err_cap) {
     TreeArgs a;
     const char *why;
     if (!make_view(cache, a.v, &why)) return op_fail(err, err_cap, -1, why);
+    if (tokens < 0) return op_fail(err, err_cap, -1, "tokens must not be negative");
+    a.v.tokens = tokens;
     if (!group_ok(heads, a.v.kvh, a.G)) return op_fail(err, err_cap, -1, "heads / kv_heads must be 1, 2, 4 or 8");
     if (layer < 0 || layer >= a.v.layers) return op_fail(err, err_cap, -1, "no such layer");
     if (max_nodes < 1 || max_nodes > kTreeMax) return op_fail(err, err_cap, -1, "max_nodes must be 1 .. 64");
@@ -537,13 +541,23 @@ HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer
     return done(e, err, err_cap);
 }
 
-HYC_API int hyc_tree_commit(void *stream, const hyc_kv_view *cache, int max_nodes, const int *d_len,
-                            const int *d_off, const int *d_parent, const int *d_tokens, const int *d_next,
-                            const int *d_forced, int *d_len_out, int *d_naccept, int *d_path, int *d_bonus,
-                            char *err, int err_cap) {
+HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer, int heads, int max_nodes,
+                               const int *d_len, const int *d_off, const int *d_parent, const void *d_q,
+                               long long q_ld, int q_bf16, float scale, void *d_out, long long out_ld, float *d_lse,
+                               void *d_ws, size_t ws_bytes, char *err, int err_cap) {
+    return hyc_tree_attention_n(stream, cache, layer, heads, max_nodes, INT_MAX, d_len, d_off, d_parent, d_q, q_ld, q_bf16,
+                                scale, d_out, out_ld, d_lse, d_ws, ws_bytes, err, err_cap);
+}
+
+HYC_API int hyc_tree_commit_n(void *stream, const hyc_kv_view *cache, int max_nodes, int tokens, const int *d_len,
+                              const int *d_off, const int *d_parent, const int *d_tokens, const int *d_next,
+                              const int *d_forced, int *d_len_out, int *d_naccept, int *d_path, int *d_bonus,
+                              char *err, int err_cap) {
     CommitArgs a;
     const char *why;
     if (!make_view(cache, a.v, &why)) return op_fail(err, err_cap, -1, why);
+    if (tokens < 0) return op_fail(err, err_cap, -1, "tokens must not be negative");
+    a.v.tokens = tokens;
     if (max_nodes < 1 || max_nodes > kTreeMax) return op_fail(err, err_cap, -1, "max_nodes must be 1 .. 64");
     if (!d_len || !d_off || !d_parent || !d_tokens || !d_next || !d_len_out || !d_naccept || !d_path || !d_bonus)
         return op_fail(err, err_cap, -1, "null argument");
@@ -562,13 +576,23 @@ HYC_API int hyc_tree_commit(void *stream, const hyc_kv_view *cache, int max_node
     return done(go(tree_commit, dim3(a.v.slots, a.v.layers), dim3(128), 0, stream, false, a), err, err_cap);
 }
 
-HYC_API int hyc_cache_weights(void *stream, const hyc_kv_view *cache, int heads, int max_q, const int *d_len,
-                              const int *d_nq, const int *d_sel, const void *d_q, long long q_ld, long long q_layer,
-                              int q_bf16, const float *d_lse, long long lse_layer, float scale, float *d_acc,
-                              int acc_rows, char *err, int err_cap) {
+HYC_API int hyc_tree_commit(void *stream, const hyc_kv_view *cache, int max_nodes, const int *d_len,
+                            const int *d_off, const int *d_parent, const int *d_tokens, const int *d_next,
+                            const int *d_forced, int *d_len_out, int *d_naccept, int *d_path, int *d_bonus,
+                            char *err, int err_cap) {
+    return hyc_tree_commit_n(stream, cache, max_nodes, INT_MAX, d_len, d_off, d_parent, d_tokens, d_next, d_forced, d_len_out,
+                             d_naccept, d_path, d_bonus, err, err_cap);
+}
+
+HYC_API int hyc_cache_weights_n(void *stream, const hyc_kv_view *cache, int heads, int max_q, int tokens, const int *d_len,
+                                const int *d_nq, const int *d_sel, const void *d_q, long long q_ld, long long q_layer,
+                                int q_bf16, const float *d_lse, long long lse_layer, float scale, float *d_acc,
+                                int acc_rows, char *err, int err_cap) {
     WeightArgs a;
     const char *why;
     if (!make_view(cache, a.v, &why)) return op_fail(err, err_cap, -1, why);
+    if (tokens < 0) return op_fail(err, err_cap, -1, "tokens must not be negative");
+    a.v.tokens = tokens;
     if (!group_ok(heads, a.v.kvh, a.G)) return op_fail(err, err_cap, -1, "heads / kv_heads must be 1, 2, 4 or 8");
     if (max_q < 1 || max_q > kTreeMax) return op_fail(err, err_cap, -1, "max_q must be 1 .. 64");
     if (!d_len || !d_nq || !d_sel || !d_q || !d_lse || !d_acc || acc_rows < 1)
@@ -610,6 +634,14 @@ HYC_API int hyc_cache_weights(void *stream, const hyc_kv_view *cache, int heads,
         e = q_bf16 ? go(cache_weights_tc<__nv_bfloat16, 128>, grid, block, smem, stream, false, a, map)
                    : go(cache_weights_tc<float, 128>, grid, block, smem, stream, false, a, map);
     return done(e, err, err_cap);
+}
+
+HYC_API int hyc_cache_weights(void *stream, const hyc_kv_view *cache, int heads, int max_q, const int *d_len,
+                              const int *d_nq, const int *d_sel, const void *d_q, long long q_ld, long long q_layer,
+                              int q_bf16, const float *d_lse, long long lse_layer, float scale, float *d_acc,
+                              int acc_rows, char *err, int err_cap) {
+    return hyc_cache_weights_n(stream, cache, heads, max_q, INT_MAX, d_len, d_nq, d_sel, d_q, q_ld, q_layer, q_bf16, d_lse,
+                               lse_layer, scale, d_acc, acc_rows, err, err_cap);
 }
 
 HYC_API int hyc_cache_evict(void *stream, const hyc_kv_view *cache, const hyc_kv_view *dst, const int *d_len,

@@ -21,6 +21,7 @@ struct KvView {
     uint16_t *kv;
     const int *pages;
     int layers, npages, kvh, hd, slots, page_max, kvd;
+    int tokens;  // of the token arrays
     long long page_stride, layer_stride;  // elements
 
     // Page of row r of a slot, -1 when there is none.
@@ -35,13 +36,15 @@ struct KvView {
     }
 };
 
-// Slot s's cached rows and nodes, bounded by its page table and max_nodes.
+// Slot s's cached rows and nodes, bounded by its page table, max_nodes and the
+// token arrays: nodes of tokens that are not there do not exist.
 __device__ __forceinline__ void tree_span(const KvView &v, const int *len, const int *off, int max_nodes, int s, int &L,
                                           int &t0, int &n) {
     const int cap = v.page_max * kPageRows;
     L = min(max(__ldg(len + s), 0), cap);
     t0 = __ldg(off + s);
-    n = min(max(__ldg(off + s + 1) - t0, 0), max_nodes);
+    const int t1 = min(__ldg(off + s + 1), v.tokens);
+    n = t0 >= 0 && t1 > t0 ? min(t1 - t0, max_nodes) : 0;
 }
 
 // Waits that gave up (2 s): counted here, read by hyc_kvops_timeouts.

@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) cache_weights_tc(const __grid_c
                 const int th = threadIdx.x - 18 * 32;  // a row's token, log-sum-exp and bound
                 if (th < N) {
                     const int j = (q0 + th) >> a.lg, head = w.s_kvh * a.G + ((q0 + th) & (a.G - 1));
-                    const int t = th < rows ? __ldg(a.sel + (size_t)w.s_slot * a.max_q + j) : -1;
+                    const int sel = th < rows ? __ldg(a.sel + (size_t)w.s_slot * a.max_q + j) : -1, t = sel < a.v.tokens ? sel : -1;
                     // a query that is left out, or saw nothing (-inf), sees no row
                     const float e = t >= 0 ? a.lse[w.s_layer * a.lse_layer + (long long)t * a.heads + head] : -INFINITY;
                     s_lse[qb][th] = e * -1.4426950408889634f;

@@ -114,9 +114,9 @@ bool tree_attention(HyCtx *c, const Fwd &f, const AttnArgs &aa, int li, int nt, 
     if (!stored) return false;
     const int S = b.slots;
     const hyc_kv_view v = tree_view(c, f.kv);
-    if (hyc_tree_attention(c->st, &v, li, c->heads, t.max_nodes, t.d_len(), t.d_int + S, t.d_int + 3 * S + 1, aa.qkv, aa.qkv_ld, 0,
-                           aa.scale, aa.ao, aa.qdim, t.lse ? t.lse + (size_t)li * b.max_tokens * c->heads : nullptr, t.ws,
-                           t.ws_bytes, c->err, sizeof c->err) != 0) {
+    if (hyc_tree_attention_n(c->st, &v, li, c->heads, t.max_nodes, nt, t.d_len(), t.d_int + S, t.d_int + 3 * S + 1, aa.qkv,
+                             aa.qkv_ld, 0, aa.scale, aa.ao, aa.qdim, t.lse ? t.lse + (size_t)li * b.max_tokens * c->heads : nullptr,
+                             t.ws, t.ws_bytes, c->err, sizeof c->err) != 0) {
         c->broken = true;
         return false;
     }
@@ -161,14 +161,14 @@ bool tree_run(HyCtx *c, const int *tokens, const int *parent, const int *off, co
     if (!ran) return false;
     const hyc_kv_view v = tree_view(c, b.kv);
     int *out = t.d_int + t.in_ints;
-    bool ok = hyc_tree_commit(c->st, &v, t.max_nodes, t.d_len(), t.d_int + S, t.d_int + 3 * S + 1, b.tok(), b.d_ids,
-                              t.d_int + 2 * S + 1, out, out + S, out + 3 * S, out + 2 * S, c->err, sizeof c->err) == 0;
+    bool ok = hyc_tree_commit_n(c->st, &v, t.max_nodes, nt, t.d_len(), t.d_int + S, t.d_int + 3 * S + 1, b.tok(), b.d_ids,
+                                t.d_int + 2 * S + 1, out, out + S, out + 3 * S, out + 2 * S, c->err, sizeof c->err) == 0;
     c->launches++;
     if (ok && t.weights) {
         const int ld = c->qd + 2 * c->kvd;
-        ok = hyc_cache_weights(c->st, &v, c->heads, t.max_nodes, t.d_len(), out + S, out + 3 * S, t.qkv, ld, (long long)T * ld, 0,
-                               t.lse, (long long)T * c->heads, 1.0f / sqrtf((float)c->hd), t.acc, tree_rows(b), c->err,
-                               sizeof c->err) == 0;
+        ok = hyc_cache_weights_n(c->st, &v, c->heads, t.max_nodes, nt, t.d_len(), out + S, out + 3 * S, t.qkv, ld,
+                                 (long long)T * ld, 0, t.lse, (long long)T * c->heads, 1.0f / sqrtf((float)c->hd), t.acc,
+                                 tree_rows(b), c->err, sizeof c->err) == 0;
         c->launches++;
     }
     if (!ok) {

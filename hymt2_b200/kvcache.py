@@ -10,8 +10,9 @@ per step (src/model.c:943-954) over a cache that only grows (:804-808).
 All work runs on torch's current stream of the cache's device and nothing
 synchronises.  tree_attention's scratch is one per stream (a captured call's own, unless its stream has
 one: then a replay must not run beside calls on that stream).  Shapes, types and strides are checked here and by the library
-(`BackendError`); what the arrays hold is not read back: lengths, offsets and
-parents are bounded on the device as the header states.
+(`BackendError`); what the arrays hold is not read back: lengths, offsets,
+parents and selected tokens are bounded on the device as the header states (its
+forms that take the number of tokens).
 """
 from __future__ import annotations
 
@@ -122,8 +123,8 @@ class PagedKV:
             ws = (buf, buf.data_ptr(), buf.numel())
             if not torch.cuda.is_current_stream_capturing():  # a graph keeps a scratch of its own
                 self._ws[(stream, heads, max_nodes)] = ws
-        self._call(self._lib.hyc_tree_attention, stream, self._ref, layer, heads, max_nodes, ln, of, pa, q.data_ptr(), old,
-                   bf16, hd ** -0.5 if scale is None else scale, out.data_ptr(), old_out, lse.data_ptr(), ws[1], ws[2])
+        self._call(self._lib.hyc_tree_attention_n, stream, self._ref, layer, heads, max_nodes, nt, ln, of, pa, q.data_ptr(),
+                   old, bf16, hd ** -0.5 if scale is None else scale, out.data_ptr(), old_out, lse.data_ptr(), ws[1], ws[2])
         return out, lse
 
     def tree_commit(self, lens: torch.Tensor, offsets: torch.Tensor, parent: torch.Tensor, tokens: torch.Tensor,
@@ -138,7 +139,7 @@ class PagedKV:
                 None if forced is None else self._ints("forced", forced, one))
         new_lens, accepted, bonus = lens.new_empty(self.slots), lens.new_empty(self.slots), lens.new_empty(self.slots)
         path = lens.new_empty(self.slots, max(max_nodes, 0))
-        self._call(self._lib.hyc_tree_commit, self._stream(), self._ref, max_nodes, *args, new_lens.data_ptr(),
+        self._call(self._lib.hyc_tree_commit_n, self._stream(), self._ref, max_nodes, nt[0], *args, new_lens.data_ptr(),
                    accepted.data_ptr(), path.data_ptr(), bonus.data_ptr())
         return new_lens, accepted, path, bonus
 
@@ -161,7 +162,7 @@ class PagedKV:
         se = self._ints("sel", sel, (self.slots, sel.shape[1]))
         if nt == 0:
             return
-        self._call(self._lib.hyc_cache_weights, self._stream(), self._ref, heads, sel.shape[1], ln, nq, se, q.data_ptr(),
+        self._call(self._lib.hyc_cache_weights_n, self._stream(), self._ref, heads, sel.shape[1], nt, ln, nq, se, q.data_ptr(),
                    st[1] if nt > 1 else heads * hd, st[0] if self.layers > 1 else 0, bf16, e, nt * heads,
                    hd ** -0.5 if scale is None else scale, w, acc.shape[3])
 

@@ -384,7 +384,10 @@ HYC_API int hyc_attention_decode_noalloc(void *stream, int heads, int kv_heads, 
  * Drafted trees: slot s holds d_len[s] cached rows and drafts the nodes
  * d_off[s] .. d_off[s + 1] - 1 (d_off[0] = 0, at most max_nodes <= 64 a slot,
  * none is fine), whose K and V stand in rows d_len[s] + i; the token arrays
- * hold d_off[slots] tokens.  d_parent[t] is
+ * hold d_off[slots] tokens.  A caller that does not know what d_off (or d_sel
+ * below) holds names the arrays' length instead, in the forms that end in _n:
+ * nodes of token numbers outside 0 .. tokens - 1 do not exist, such queries
+ * are left out, and no array is touched past its end.  d_parent[t] is
  * the node's parent within its tree, below the node itself (-1, or any number
  * that is not below it: none; -2: a padding node, which sees nothing and is
  * nobody's ancestor).  Rows past a slot's page table do not exist. */
@@ -410,6 +413,10 @@ HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer
                                const int *d_len, const int *d_off, const int *d_parent, const void *d_q,
                                long long q_ld, int q_bf16, float scale, void *d_out, long long out_ld, float *d_lse,
                                void *d_ws, size_t ws_bytes, char *err, int err_cap);
+HYC_API int hyc_tree_attention_n(void *stream, const hyc_kv_view *cache, int layer, int heads, int max_nodes, int tokens,
+                                 const int *d_len, const int *d_off, const int *d_parent, const void *d_q,
+                                 long long q_ld, int q_bf16, float scale, void *d_out, long long out_ld, float *d_lse,
+                                 void *d_ws, size_t ws_bytes, char *err, int err_cap);
 
 /* Greedy acceptance: the path starts at node 0 (the token the sequence ends
  * with) and goes on to the first child whose token is d_next[t], the token
@@ -424,6 +431,10 @@ HYC_API int hyc_tree_commit(void *stream, const hyc_kv_view *cache, int max_node
                             const int *d_off, const int *d_parent, const int *d_tokens, const int *d_next,
                             const int *d_forced, int *d_len_out, int *d_naccept, int *d_path, int *d_bonus,
                             char *err, int err_cap);
+HYC_API int hyc_tree_commit_n(void *stream, const hyc_kv_view *cache, int max_nodes, int tokens, const int *d_len,
+                              const int *d_off, const int *d_parent, const int *d_tokens, const int *d_next,
+                              const int *d_forced, int *d_len_out, int *d_naccept, int *d_path, int *d_bonus,
+                              char *err, int err_cap);
 
 /* Accumulated attention weights: for layer l, KV head h and row r of slot s,
  *   d_acc[l][s][h][r] += sum over the slot's queries j and the head's group
@@ -440,6 +451,10 @@ HYC_API int hyc_cache_weights(void *stream, const hyc_kv_view *cache, int heads,
                               const int *d_nq, const int *d_sel, const void *d_q, long long q_ld, long long q_layer,
                               int q_bf16, const float *d_lse, long long lse_layer, float scale, float *d_acc,
                               int acc_rows, char *err, int err_cap);
+HYC_API int hyc_cache_weights_n(void *stream, const hyc_kv_view *cache, int heads, int max_q, int tokens, const int *d_len,
+                                const int *d_nq, const int *d_sel, const void *d_q, long long q_ld, long long q_layer,
+                                int q_bf16, const float *d_lse, long long lse_layer, float scale, float *d_acc,
+                                int acc_rows, char *err, int err_cap);
 
 /* Eviction: for every layer and KV head of slot s with n = d_len[s] rows,
  * keeps all rows when n <= budget, else the first `sinks`, the last `recent`
