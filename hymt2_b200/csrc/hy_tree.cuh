@@ -132,9 +132,12 @@ bool tree_run(HyCtx *c, const int *tokens, const int *parent, const int *off, co
     REQ(c, off[0] == 0 && nt >= 1 && nt <= T && nt <= b.max_out, "more nodes than the batch's tokens or head rows");
     int *h_len = t.h_int, *h_off = t.h_int + S, *h_forced = h_off + S + 1, *h_par = h_forced + S, *h_row = h_par + T;
     int *tok = b.h_in, *slot = b.h_in + T, *pos = b.h_in + 2 * T, *rows = b.h_in + 3 * T;
+    // all offsets before any of them is used: in between two that hold, one may lie past the arrays
+    for (int s = 0; s < S; s++)
+        REQ(c, off[s + 1] >= off[s] && off[s + 1] <= nt && off[s + 1] - off[s] <= t.max_nodes,
+            "a slot's offsets fall, or its tree has more than max_nodes nodes");
     for (int s = 0; s < S; s++) {
         const int n = off[s + 1] - off[s];
-        REQ(c, n >= 0 && n <= t.max_nodes, "a slot's offsets fall, or its tree has more than max_nodes nodes");
         REQ(c, n == 0 || t.len[s] + n <= b.slot_ctx, "a tree does not fit its slot's context");
         for (int i = 0; i < n; i++) {
             const int k = off[s] + i, p = parent[k];
