@@ -351,7 +351,14 @@ class DeviceModel:
         """One pass over a tree of drafted tokens for each slot.
 
         trees: {slot: (tokens, parents)}, node 0 the token the slot's sequence ends with (parent -1); forced: the
-        slots whose nodes are a given chain, all kept.  Returns {slot: (kept tokens, the model's next token)}."""
+        slots whose nodes are a given chain, all kept.  slots: those of batch_prepare.  Returns {slot: (kept tokens, the
+        model's next token)}."""
+        if slots != self.batch_slots:
+            raise ValueError(f"the batch state has {self.batch_slots} slots")
+        if not trees or not all(0 <= s < slots for s in (*trees, *(forced or ()))):
+            raise ValueError(f"trees and forced name slots 0 .. {slots - 1}, at least one")
+        if any(len(tk) != len(pa) for tk, pa in trees.values()):
+            raise ValueError("a tree has as many parents as tokens")
         off = np.zeros(slots + 1, dtype=np.int32)
         for s, (tk, _) in trees.items():
             off[s + 1] = len(tk)
@@ -359,8 +366,6 @@ class DeviceModel:
         order = sorted(trees)
         tk = np.concatenate([np.asarray(trees[s][0], dtype=np.int32) for s in order])
         pa = np.concatenate([np.asarray(trees[s][1], dtype=np.int32) for s in order])
-        if len(tk) != len(pa):
-            raise ValueError("a tree has as many parents as tokens")
         fo = np.zeros(slots, dtype=np.int32)
         fo[list(forced or ())] = 1
         acc, nxt = np.zeros(slots, dtype=np.int32), np.zeros(slots, dtype=np.int32)
