@@ -660,6 +660,11 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             um_fence_before();
             mb_arrive(&ofree);
             if (active) {
+                // a node that saw nothing: its products with the cached rows are
+                // zeros only where those rows are finite
+                if (l == 0.f)
+#pragma unroll
+                    for (int d = 0; d < W; d++) o[d] = 0.f;
                 if (th < rows) {
                     const int tok = cur.t0 + node, head = cur.kvh * a.G + (th & (a.G - 1));
                     if (bad && l > 0.f) {
@@ -1065,6 +1070,9 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
                 if (row >= rows) continue;
                 const int tok = wc.t0 + (row >> a.lg), head = wc.s_kvh * a.G + (row & (a.G - 1));
                 const float L = (s_mx[0][row] + s_mx[1][row]) + (s_mx[2][row] + s_mx[3][row]);
+                if (L == 0.f)  // a node that saw nothing: 0 times a cached row is not 0 where that is not finite
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) o[mt][nt][j] = o[mt][nt][2 + j] = 0.f;
                 if (whole) {
                     const float inv = L == 0.f ? 0.f : 1.0f / L;
                     T *dst = (T *)a.out + (long long)tok * a.out_ld + (long long)head * HD + warp * MT * 16 + g;

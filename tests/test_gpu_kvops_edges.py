@@ -102,3 +102,30 @@ def test_weights_of_tokens_that_are_not_there(bf16):
         cache.add_weights(acc, q, lse, lens, nq, gpu(np.array([[0, gone, 5, 2], [gone, 1, 3, gone]], np.int32)))
         got.append(acc)
     assert bool((got[0] != 1).any()) and all(torch.equal(got[0], a) for a in got[1:])
+
+
+# ---------------------------------------------------------------- infinities and NaN in cached rows
+
+def spoil(kv, pages, slot, r, what, value, dims=slice(None), layer=0):
+    """K (what 0) or V (1) of a row, in some dims of every KV head."""
+    kv[layer, int(pages[slot, r // PAGE]), what, r % PAGE, :, dims] = value
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("G,n,L", [(4, 5, 40), (4, 5, 3000), (8, 13, 40), (8, 13, 3000), (4, 50, 3000)])
+def test_padding_nodes_over_spoiled_rows(G, n, L, hd, bf16, bad):
+    """A node that sees no row gets zeros and -inf whatever the slot's cached rows hold (columns of one tile and split
+    ones, both forms)."""
+    import torch
+    rng = np.random.default_rng(L + n + hd)
+    lens, trees = [L, 33], [random_tree(rng, n, pad=2), random_tree(rng, n)]
+    kv, pages = make_cache(rng, 1, 2, hd, [L + n, 33 + n])
+    for r in (0, L // 2, L - 1):
+        spoil(kv, pages, 0, r, 0, bad, slice(3, 5))
+        spoil(kv, pages, 0, r, 1, bad)
+    q = gpu(torch.from_numpy(rng.standard_normal((2 * n, 2 * G, hd)).astype(np.float32)).to(torch.bfloat16 if bf16 else torch.float32))
+    out, lse = run_tree(kv, pages, 0, lens, trees, q, n)
+    assert (out[n - 2:n] == 0).all() and (lse[n - 2:n] == -np.inf).all()
+    assert np.isfinite(out[n:]).all() and np.isfinite(lse[n:]).all()
