@@ -129,6 +129,7 @@ SIGNATURES = {
     "hyc_tree_evict": (I, [P, I, I, I]),
     "hyc_tree_state": (I, [P, I, P, P, P]),
     "hyc_kvops_timeouts": (I, []),
+    "hyc_kvops_wait_probe": (I, [C.c_ulonglong]),
     "hyc_tree_attention_ws": (Z, [KV, I, I]),
     "hyc_tree_attention": (I, [P, KV, I, I, I, P, P, P, P, LL, I, F, P, LL, P, P, Z, C.c_char_p, I]),
     "hyc_tree_attention_n": (I, [P, KV, I, I, I, I, P, P, P, P, LL, I, F, P, LL, P, P, Z, C.c_char_p, I]),

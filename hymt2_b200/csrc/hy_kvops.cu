@@ -397,6 +397,18 @@ __global__ void __launch_bounds__(256) evict_gather(const __grid_constant__ Evic
     }
 }
 
+// Failure-detection probe: the kernels' wait on a phase that nothing
+// completes, for limit_ns.  It gives up, is counted, and the kernel returns.
+__global__ void kv_wait_probe(unsigned long long limit_ns) {
+    __shared__ __align__(8) uint64_t bar;
+    __shared__ int stop;
+    if (threadIdx.x == 0) {
+        stop = 0;
+        mb_init(&bar, 1);
+        mb_wait(&bar, 0, &stop, limit_ns);
+    }
+}
+
 template <typename... KArgs, typename... Args>
 cudaError_t go(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, void *stream, bool pdl, Args &&...args) {
     cudaLaunchConfig_t cfg = {};
@@ -446,6 +458,19 @@ extern "C" {
 HYC_API int hyc_kvops_timeouts(void) {
     unsigned n = 0;
     return cudaMemcpyFromSymbol(&n, g_kv_timeouts, sizeof n) == cudaSuccess ? (int)n : -1;
+}
+
+HYC_API int hyc_kvops_wait_probe(unsigned long long limit_ns) {
+    if (limit_ns == 0 || limit_ns > 1000000000ull) return -1;
+    kv_wait_probe<<<1, 32>>>(limit_ns);
+    return cudaGetLastError() == cudaSuccess && cudaDeviceSynchronize() == cudaSuccess ? 0 : -1;
+}
+
+// The count behind the stream's work so far, into pinned memory: for the batch
+// engine, which looks at it with every pass's outcome.
+int hyk_kvops_timeouts_async(void *stream, unsigned *host) {
+    const cudaError_t e = cudaMemcpyFromSymbolAsync(host, g_kv_timeouts, sizeof *host, 0, cudaMemcpyDeviceToHost, (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : -1;
 }
 
 HYC_API size_t hyc_tree_attention_ws(const hyc_kv_view *cache, int heads, int max_nodes) {

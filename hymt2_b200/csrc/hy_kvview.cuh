@@ -76,12 +76,12 @@ __device__ __forceinline__ bool mb_try(uint64_t *b, unsigned parity) {
 // Waits for a phase for at most 2 s.  A wait that gives up sets the CTA's
 // *stop word, after which every wait returns at once: all threads still go
 // through the same steps, with whatever data is there, and the kernel ends.
-__device__ __forceinline__ void mb_wait(uint64_t *b, unsigned parity, int *stop) {
+__device__ __forceinline__ void mb_wait(uint64_t *b, unsigned parity, int *stop, unsigned long long limit = kKvWaitNs) {
     if (mb_try(b, parity)) return;
     const unsigned long long t0 = gtimer();
     while (!mb_try(b, parity)) {
         if (*(volatile int *)stop) return;
-        if (gtimer() - t0 > kKvWaitNs) {
+        if (gtimer() - t0 > limit) {
             *(volatile int *)stop = 1;
             atomicAdd(&g_kv_timeouts, 1u);
             return;

@@ -15,13 +15,17 @@
 // eviction keeps the heaviest rows (hyc_cache_evict): a slot's rows are then
 // no longer its positions, so the two are counted apart.
 
+extern "C" int hyk_kvops_timeouts_async(void *stream, unsigned *host);  // hy_kvops.cu
+
 struct TreeState {
     int max_nodes = 0;
     bool weights = false;
     std::vector<int> len, pos;  // rows and next position of each slot
+    unsigned gave_up = 0;       // waits of the operators' kernels that had given up before
     // device ints, staged from pinned memory in one copy: len [S] | off [S + 1] |
     // forced [S] | parent [T] | row [T], then the outcome: len_out [S] |
-    // accepted [S] | bonus [S] | path [S][max_nodes]
+    // accepted [S] | bonus [S] | path [S][max_nodes]; and, on the host alone, the count
+    // of waits that have given up
     int *d_int = nullptr, *h_int = nullptr;
     size_t in_ints = 0, ints = 0;
     float *qkv = nullptr, *lse = nullptr, *acc = nullptr;  // [L][T][q | k | v], [L][T][heads], [L][S][kvh][rows]
@@ -59,6 +63,20 @@ hyc_kv_view tree_view(const HyCtx *c, uint16_t *kv) {
     return v;
 }
 
+// The count of waits that have given up, with the stream's work done: noted, or
+// compared with what it was (an operator that gave up has ended with wrong
+// outputs).
+bool tree_waits(HyCtx *c, TreeState &t, bool note) {
+    unsigned *now = (unsigned *)(t.h_int + t.ints);
+    if (hyk_kvops_timeouts_async(c->st, now) != 0) return fail(c, "kvops timeouts", cudaGetLastError());
+    CK(c, cudaStreamSynchronize(c->st));
+    if (note) t.gave_up = *now;
+    if (*now == t.gave_up) return true;
+    c->broken = true;
+    snprintf(c->err, sizeof c->err, "operators on the KV cache: a wait inside a kernel timed out");
+    return false;
+}
+
 bool tree_prepare(HyCtx *c, int max_nodes, bool weights) {
     Batch &b = *c->bat;
     REQ(c, max_nodes >= 1 && max_nodes <= 64, "a tree has 1 .. 64 nodes");
@@ -74,7 +92,8 @@ bool tree_prepare(HyCtx *c, int max_nodes, bool weights) {
     t->in_ints = 3 * S + 1 + 2 * T;
     t->ints = t->in_ints + 3 * S + S * max_nodes;
     CK(c, cudaMalloc(&t->d_int, t->ints * 4));
-    CK(c, cudaMallocHost(&t->h_int, t->ints * 4));
+    CK(c, cudaMallocHost(&t->h_int, (t->ints + 1) * 4));
+    if (!tree_waits(c, *t, true)) return false;
     const hyc_kv_view v = tree_view(c, b.kv);
     t->ws_bytes = hyc_tree_attention_ws(&v, c->heads, max_nodes);
     REQ(c, t->ws_bytes > 0, "unsupported head geometry");
@@ -179,8 +198,7 @@ bool tree_run(HyCtx *c, const int *tokens, const int *parent, const int *off, co
         return false;
     }
     CK(c, cudaMemcpyAsync(t.h_int + t.in_ints, out, (t.ints - t.in_ints) * 4, cudaMemcpyDeviceToHost, c->st));
-    CK(c, cudaStreamSynchronize(c->st));
-    if (!tc_status(c)) return false;
+    if (!tree_waits(c, t, false) || !tc_status(c)) return false;
     for (int s = 0; s < S; s++) {
         t.len[s] = t.h_int[t.in_ints + s];
         t.pos[s] += t.h_int[t.in_ints + S + s];

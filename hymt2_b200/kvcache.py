@@ -8,7 +8,7 @@ them (`evict`).  No counterpart in the reference, whose loop decodes one token
 per step (src/model.c:943-954) over a cache that only grows (:804-808).
 
 All work runs on torch's current stream of the cache's device and nothing
-synchronises.  tree_attention's scratch is one per stream (a captured call's own, unless its stream has
+synchronises (but `check_waits`).  tree_attention's scratch is one per stream (a captured call's own, unless its stream has
 one: then a replay must not run beside calls on that stream).  Shapes, types and strides are checked here and by the library
 (`BackendError`); what the arrays hold is not read back: lengths, offsets,
 parents and selected tokens are bounded on the device as the header states (its
@@ -85,6 +85,14 @@ class PagedKV:
 
     def _stream(self) -> int:
         return _raw_stream(self._dev)
+
+    def check_waits(self) -> None:
+        """Waits for the device and raises BackendError when a wait inside one of these kernels has given up on it since
+        the library was loaded: outputs since then may be wrong."""
+        with torch.cuda.device(self._dev):
+            n = self._lib.hyc_kvops_timeouts()
+        if n != 0:
+            raise BackendError(f"operators on the KV cache: {n} waits inside a kernel timed out" if n > 0 else "device error")
 
     def tree_attention(self, q: torch.Tensor, lens: torch.Tensor, offsets: torch.Tensor, parent: torch.Tensor,
                        max_nodes: int, layer: int = 0, scale: float | None = None, out: torch.Tensor | None = None,

@@ -379,7 +379,11 @@ HYC_API int hyc_attention_decode_noalloc(void *stream, int heads, int kv_heads, 
  * Kernels that wait inside (for copies and tensor-core products) do so for at
  * most 2 s a wait and then end with wrong outputs; hyc_kvops_timeouts returns
  * how many waits have given up on the current device since the library was
- * loaded (0 unless something is broken; it synchronises), -1 on an error.
+ * loaded (0 unless something is broken; it synchronises), -1 on an error.  A
+ * handle's own passes (hyc_tree_forward) look at the count themselves and
+ * fail.  hyc_kvops_wait_probe shows it without a fault: one such wait on a
+ * phase that nothing completes, for limit_ns (<= 1 s), which gives up and is
+ * counted; 0 or -1.
  *
  * Drafted trees: slot s holds d_len[s] cached rows and drafts the nodes
  * d_off[s] .. d_off[s + 1] - 1 (d_off[0] = 0, at most max_nodes <= 64 a slot,
@@ -408,6 +412,7 @@ typedef struct hyc_kv_view {
  * it has run; its contents need no preparation.  K or V of rows that a node
  * does not see never reach its output, whatever they hold. */
 HYC_API int hyc_kvops_timeouts(void);
+HYC_API int hyc_kvops_wait_probe(unsigned long long limit_ns);
 HYC_API size_t hyc_tree_attention_ws(const hyc_kv_view *cache, int heads, int max_nodes);
 HYC_API int hyc_tree_attention(void *stream, const hyc_kv_view *cache, int layer, int heads, int max_nodes,
                                const int *d_len, const int *d_off, const int *d_parent, const void *d_q,
