@@ -6,6 +6,9 @@
 // one problem are the (node, head) pairs of a slot and KV head: 4 hd bytes of
 // cache a row r against 4 hd flops for each of them.
 #pragma once
+#include <cfloat>
+#include <cmath>
+
 #include "hy_kvview.cuh"
 
 namespace {
@@ -206,30 +209,75 @@ __device__ __forceinline__ unsigned long long tree_mask(const int8_t *s_up, int 
     return m;
 }
 
-// p_r v_r of drafted rows whose V is not finite (in dims d0 .. d0 + HD / 2 -
-// 1), for one (node, head): the matrix product leaves such rows out, and the
-// nodes that see them add them here, in the order of the rows.
+// The factor 2^x of a part that holds something: never 0, so that an infinite
+// V keeps its sign where its probability is too small for fp32.
+__device__ __forceinline__ float ex2_part(float x) {
+    const float f = ex2(x);
+    return f < FLT_MIN ? FLT_MIN : f;
+}
+
+// One (node, head) row over the rows r0 .. r1 - 1 that its node sees (mask: of
+// the drafted ones), by a whole warp in plain fp32 arithmetic, in place of a
+// row whose sum or output is not finite or which sees a V that is not.  The
+// products split fp32 numbers into bf16 terms, and infinity times a term that
+// is 0 or of the other sign is NaN where infinity times the number is not.
+// Scores of -inf drop their rows; with one of +inf or NaN the output is NaN.
+// The result goes to the output (ml null) or to a piece, dim d of which stands
+// at po[d / 8 * step + d % 8].
 template <typename T, int HD>
-__device__ __noinline__ void tree_add_bad(const TreeArgs &a, int slot, int kvh, int L, int t, int head, int d0,
-                                          unsigned long long bad, float sl2, float m, float *o) {
-    while (bad) {
-        const int j = __ffsll((long long)bad) - 1;
-        bad &= bad - 1;
-        const int pg = a.v.page(slot, L + j);
-        if (pg < 0) continue;
-        const uint16_t *k = a.v.kv + a.v.row(a.layer, pg, L + j) + kvh * HD, *v = k + kPageRows * a.v.kvd;
-        const T *q = (const T *)a.q + (long long)t * a.q_ld + (long long)head * HD;
-        float x = 0.f;
-        for (int d = 0; d < HD; d += 4) {
-            const float4 qq = ld_row4(q + d);
-            x = fmaf(qq.x, bf16_bits_to_f32(k[d]), x);
-            x = fmaf(qq.y, bf16_bits_to_f32(k[d + 1]), x);
-            x = fmaf(qq.z, bf16_bits_to_f32(k[d + 2]), x);
-            x = fmaf(qq.w, bf16_bits_to_f32(k[d + 3]), x);
-        }
-        const float p = ex2((a.scale < 0.f ? -x : x) * sl2 - m);
-        for (int d = 0; d < HD / 2; d++) o[d] = fmaf(p, bf16_bits_to_f32(v[d0 + d]), o[d]);
+__device__ __noinline__ void tree_redo(const TreeArgs &a, int slot, int kvh, int L, unsigned long long mask, int r0, int r1, int tok,
+                                       int head, float sl2, float2 *ml, float *po, int step) {
+    constexpr int D = HD / 32, B = 4;  // dims of a lane; rows in flight
+    const int lane = threadIdx.x & 31, d0 = lane * D;
+    float q[D], o[D], m = -INFINITY, l = 0.f;
+    bool nan = false;
+#pragma unroll
+    for (int d = 0; d < D; d++) {
+        q[d] = (float)((const T *)a.q)[(long long)tok * a.q_ld + (long long)head * HD + d0 + d];
+        if (a.scale < 0.f) q[d] = -q[d];
+        o[d] = 0.f;
     }
+    const uint16_t *base = a.v.kv + a.layer * a.v.layer_stride + kvh * HD + d0;
+    for (int r = r0; r < r1; r += B) {
+        float k[B][D], v[B][D];
+#pragma unroll
+        for (int i = 0; i < B; i++) {
+            const int pg = r + i < r1 ? a.v.page(slot, r + i) : -1;
+            const uint16_t *row = base + a.v.row(0, max(pg, 0), r + i);
+#pragma unroll
+            for (int d = 0; d < D; d++) {
+                k[i][d] = pg < 0 ? 0.f : bf16_bits_to_f32(row[d]);
+                v[i][d] = pg < 0 ? 0.f : bf16_bits_to_f32(row[kPageRows * a.v.kvd + d]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < B; i++) {
+            if (r + i >= r1 || (r + i >= L && !((mask >> (r + i - L)) & 1))) continue;
+            float x = 0.f;
+#pragma unroll
+            for (int d = 0; d < D; d++) x = fmaf(q[d], k[i][d], x);
+            x = warp_sum(x) * sl2;
+            if (x == -INFINITY) continue;
+            nan |= x != x;
+            const float mn = fmaxf(m, x), f = m == mn ? 1.f : m == -INFINITY ? 0.f : ex2_part(m - mn), p = ex2_part(x - mn);
+            m = mn;
+            l = fmaf(l, f, p);
+#pragma unroll
+            for (int d = 0; d < D; d++) o[d] = fmaf(p, v[i][d], o[d] * f);
+        }
+    }
+    if (m == INFINITY && !nan) l = 1.f;  // lse = +inf
+    if (ml) {
+        if (lane == 0) *ml = make_float2(m, l);
+#pragma unroll
+        for (int d = 0; d < D; d++) po[(d0 + d) / 8 * step + (d0 + d) % 8] = o[d];
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    T *dst = (T *)a.out + (long long)tok * a.out_ld + (long long)head * HD + d0;
+#pragma unroll
+    for (int d = 0; d < D; d++) dst[d] = (T)(o[d] * inv);
+    if (a.lse && lane == 0) a.lse[(long long)tok * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // ---------------------------------------------------------------- wide trees: tcgen05
@@ -619,8 +667,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                 if (tail) {
                     // V rows that no node sees become zeros (a product with a
                     // probability of 0 must be 0), and so do halves of drafted
-                    // rows that are not finite, which the nodes that see them
-                    // add at the end
+                    // rows that are not finite: the nodes that see them are
+                    // done again at the end
                     const int pos = 2 * it + 1, st = pos % NST, r = r0 + th;
                     mb_wait(&full[st], (pos / NST) & 1, &s_stop);
                     if (r >= L) {
@@ -647,34 +695,33 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
             // every S of the segment is done, so the next one's Q may go in
             // while the last P . V runs
             if (s_seg[(seg + 1) & 1].have) load_q(s_seg[(seg + 1) & 1]);
+            flush();
+            um_fence_before();
+            mb_arrive(&ofree);
+            float odd = 0.f;  // not 0: an output is not finite
+#pragma unroll
+            for (int d = 0; d < W; d++) odd = fmaf(o[d], 0.f, odd);
+            if (odd != 0.f) l = NAN;
             // the halves' sums, each in the word that this thread itself read the
             // other half's last maximum from (the word of its own maximum may
             // still be read by the other half, which no barrier has held since)
             s_half[h ^ 1][th] = l;
             bar_sync(1, kTtSoft);  // and s_bad is complete
             l = h ? s_half[1][th] + l : l + s_half[0][th];
-            const unsigned long long bad = s_bad[seg & 1][h] & mask;
+            const unsigned long long bad = (s_bad[seg & 1][0] | s_bad[seg & 1][1]) & mask;
             if (th == 0) s_bad[(seg + 1) & 1][h] = 0;
             const bool whole = cur.a == 0 && t1 == cur.T;
-            flush();
-            um_fence_before();
-            mb_arrive(&ofree);
             if (active) {
+                const int piece = (2 * range + cur.piece) * a.row_blocks + rb;
+                const bool redo = th < rows && live && (l != l || bad);
                 // a node that saw nothing: its products with the cached rows are
                 // zeros only where those rows are finite
-                if (l == 0.f)
+                if (l == 0.f || !live)
 #pragma unroll
                     for (int d = 0; d < W; d++) o[d] = 0.f;
-                if (th < rows) {
+                if (!live) l = 0.f;
+                if (th < rows && !redo) {
                     const int tok = cur.t0 + node, head = cur.kvh * a.G + (th & (a.G - 1));
-                    if (bad && l > 0.f) {
-                        float x[W];  // its address is taken: o stays in registers
-#pragma unroll
-                        for (int d = 0; d < W; d++) x[d] = o[d];
-                        tree_add_bad<T, HD>(a, cur.slot, cur.kvh, L, tok, head, h * W, bad, sl2, m, x);
-#pragma unroll
-                        for (int d = 0; d < W; d++) o[d] = x[d];
-                    }
                     if (whole) {
                         const float inv = l == 0.f ? 0.f : 1.0f / l;
                         T *dst = (T *)a.out + (long long)tok * a.out_ld + (long long)head * HD + h * W;
@@ -683,12 +730,18 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                         if (a.lse && h == 0)
                             a.lse[(long long)tok * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
                     } else {
-                        const int piece = (2 * range + cur.piece) * a.row_blocks + rb;
                         if (h == 0) a.part_ml[(size_t)piece * 128 + th] = make_float2(m, l);
                         float *po = a.part_o + (size_t)piece * 128 * HD + h * W * 128 + th * 8;
 #pragma unroll
                         for (int d = 0; d < W; d += 8) st_row8(po + d * 128, o + d, 1.f, true);
                     }
+                }
+                for (unsigned who = __ballot_sync(0xffffffffu, redo && h == 0); who; who &= who - 1) {  // rare
+                    const int row = (warp & 3) * 32 + __ffs(who) - 1, nd = node0 + (row >> a.lg);
+                    unsigned long long see = tree_mask(s_up, nd);
+                    tree_redo<T, HD>(a, cur.slot, cur.kvh, L, see, cur.a * kTtK, min(t1 * kTtK, end), cur.t0 + nd,
+                                     cur.kvh * a.G + (row & (a.G - 1)), sl2, whole ? nullptr : a.part_ml + (size_t)piece * 128 + row,
+                                     a.part_o + (size_t)piece * 128 * HD + row * 8, 1024);
                 }
             }
             if (range_root && cur.a == 0 && !whole) a.roots[range] = make_int4(cur.slot, cur.kvh, cur.c, s_start[3]);
@@ -764,6 +817,7 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
     __shared__ int s_scan[kTnWarps], s_start[4];
     __shared__ int8_t s_up[kTreeMax];
     __shared__ float s_mx[kTnWarps][NT * 8];
+    __shared__ unsigned s_redo;  // rows with outputs that are not finite
     __shared__ unsigned long long s_bad, s_mask[NT * 8];  // s_mask: what a query row's node sees of its tree
     uint8_t *bk = dsm, *bv = dsm + kTnK * ROW;
     uint2 *qf = (uint2 *)(bv + kTnK * ROW);    // Q fragments [term][16 dims][8 rows][lane]
@@ -779,7 +833,10 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
         wi = tree_walk<kTnK>(s_start, range);
         if (th == 0) a.roots[range] = make_int4(-1, 0, 0, 0);
     }
-    if (th == 0) s_bad = 0;  // first used after the barriers of the first tile
+    if (th == 0) {  // first used after the barriers of the first tile
+        s_bad = 0;
+        s_redo = 0;
+    }
     const auto step = [&](TreeWalk<kTnK> &w) { return a.whole ? w.next_whole(a) : w.next(a, 0); };
     const int cap = a.v.page_max * kPageRows;
     const float sl2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);
@@ -969,7 +1026,7 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
             __syncthreads();  // P and V are there
             if (tail) {
                 // drafted rows whose V is not finite become zeros; the nodes
-                // that see them add them at the end
+                // that see them are done again at the end
                 for (int r = max(wc.L - r0, 0) + warp; r < min(end - r0, kTnK); r += kTnWarps) {
                     bool x = false;
                     uint4 *p = (uint4 *)(bv + r * ROW + (lane % CH) * 16);
@@ -1028,38 +1085,19 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
 #pragma unroll
                 for (int w = 4; w < 32; w <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], w);
                 if (g == 0) s_mx[warp][nt * 8 + 2 * tq + j] = l[nt][j];
+                float odd = 0.f;  // not 0: an output is not finite (with a sum that is not, all are not)
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) odd = fmaf(o[mt][nt][j], 0.f, fmaf(o[mt][nt][2 + j], 0.f, odd));
+                if (odd != 0.f) atomicOr(&s_redo, 1u << (nt * 8 + 2 * tq + j));
             }
         __syncthreads();
-        for (unsigned long long bad = s_bad; bad; bad &= bad - 1) {  // rare: p_r v_r of the rows left out above
-            const int j = __ffsll((long long)bad) - 1, pg = a.v.page(wc.s_slot, wc.L + j);
-            if (pg < 0) continue;
-            const uint16_t *kr = a.v.kv + a.v.row(a.layer, pg, wc.L + j) + wc.s_kvh * HD, *vr = kr + kPageRows * a.v.kvd;
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-                for (int c = 0; c < 8 && nt * 8 + c < rows; c++) {
-                    const int row = nt * 8 + c;
-                    if (!((tree_mask(s_up, row >> a.lg) >> j) & 1)) continue;
-                    const T *q = (const T *)a.q + (long long)(wc.t0 + (row >> a.lg)) * a.q_ld +
-                                 (long long)(wc.s_kvh * a.G + (row & (a.G - 1))) * HD;
-                    float x = 0.f;
-                    for (int d = lane; d < HD; d += 32) x = fmaf((float)q[d], bf16_bits_to_f32(kr[d]), x);
-                    x = warp_sum(x);
-                    if ((c >> 1) != tq) continue;
-                    const float p = ex2((a.scale < 0.f ? -x : x) * sl2 - (c & 1 ? m[nt][1] : m[nt][0]));
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        const int d = (warp * MT + mt) * 16 + g;
-                        const float v0 = p * bf16_bits_to_f32(vr[d]), v1 = p * bf16_bits_to_f32(vr[d + 8]);
-                        if (c & 1) {
-                            o[mt][nt][1] += v0;
-                            o[mt][nt][3] += v1;
-                        } else {
-                            o[mt][nt][0] += v0;
-                            o[mt][nt][2] += v1;
-                        }
-                    }
-                }
-        }
+        const unsigned odd_rows = s_redo;
+        const unsigned long long bad = s_bad;
+        // whether a row is done again: it is one of those, or its node sees a drafted row that was left out above
+        const auto redo = [&](int row) {
+            const unsigned long long see = tree_mask(s_up, row >> a.lg);
+            return see && (((odd_rows >> row) & 1) || (see & bad));
+        };
         const bool whole = wc.s_a == 0 && wc.s_b == wc.T;
         const size_t piece = (size_t)2 * range + (wc.s_g != wc.g0);
 #pragma unroll
@@ -1067,7 +1105,7 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int row = nt * 8 + 2 * tq + j;
-                if (row >= rows) continue;
+                if (row >= rows || ((odd_rows || bad) && redo(row))) continue;
                 const int tok = wc.t0 + (row >> a.lg), head = wc.s_kvh * a.G + (row & (a.G - 1));
                 const float L = (s_mx[0][row] + s_mx[1][row]) + (s_mx[2][row] + s_mx[3][row]);
                 if (L == 0.f)  // a node that saw nothing: 0 times a cached row is not 0 where that is not finite
@@ -1093,9 +1131,20 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
                     if (g == 0 && warp == 0) a.part_ml[piece * (NT * 8) + row] = make_float2(m[nt][j], L);
                 }
             }
+        if (odd_rows || bad)  // rare
+            for (int row = warp; row < rows; row += kTnWarps) {
+                if (!redo(row)) continue;
+                const size_t at = piece * (NT * 8) + row;
+                tree_redo<T, HD>(a, wc.s_slot, wc.s_kvh, wc.L, tree_mask(s_up, row >> a.lg), wc.s_a * kTnK, min(wc.s_b * kTnK, end),
+                                 wc.t0 + (row >> a.lg), wc.s_kvh * a.G + (row & (a.G - 1)), sl2, whole ? nullptr : a.part_ml + at,
+                                 a.part_o + at * HD, 8);
+            }
         if (th == 0 && wc.s_a == 0 && !whole) a.roots[range] = make_int4(wc.s_slot, wc.s_kvh, wc.s_c, s_start[3]);
         __syncthreads();
-        if (th == 0) s_bad = 0;
+        if (th == 0) {
+            s_bad = 0;
+            s_redo = 0;
+        }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -1200,14 +1249,14 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constan
 #pragma unroll
                 for (int i = 0; i < B; i++)
                     if (ml[i].y != 0.f) mn = fmaxf(mn, ml[i].x);
-                const float old = M == -INFINITY ? 0.f : ex2(M - mn);
+                const float old = M == mn ? 1.f : M == -INFINITY ? 0.f : ex2_part(M - mn);
                 M = mn;
                 S *= old;
 #pragma unroll
                 for (int d = 0; d < D; d++) o[d] *= old;
 #pragma unroll
                 for (int i = 0; i < B; i++) {
-                    const float f = ml[i].y == 0.f ? 0.f : ex2(ml[i].x - M);  // 0: nothing seen in this piece
+                    const float f = ml[i].y == 0.f ? 0.f : ml[i].x == M ? 1.f : ex2_part(ml[i].x - M);  // 0: nothing seen in this piece
                     S = fmaf(ml[i].y, f, S);
 #pragma unroll
                     for (int d = 0; d < D; d++) o[d] = fmaf(v[i][d], f, o[d]);
@@ -1228,7 +1277,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constan
 #pragma unroll
                 for (int d = 0; d < D; d++) o[d] = 0.f;
                 for (int i = 0; i < wpr; i++) {
-                    const float l = s_l[warp + i], f = l == 0.f ? 0.f : ex2(s_m[warp + i] - M);
+                    const float l = s_l[warp + i], f = l == 0.f ? 0.f : s_m[warp + i] == M ? 1.f : ex2_part(s_m[warp + i] - M);
                     S = fmaf(l, f, S);
 #pragma unroll
                     for (int d = 0; d < D; d++) o[d] = fmaf(s_part[warp + i][d0 + d], f, o[d]);

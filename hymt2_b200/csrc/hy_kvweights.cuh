@@ -65,6 +65,27 @@ struct WeightWalk {
     }
 };
 
+// One row's sum over a block's queries (from query row q0 on) in plain fp32
+// arithmetic, in place of one that is not a number: the products split fp32
+// queries into bf16 terms, and an infinite key times terms of both signs, or
+// times one that is 0, is NaN where the key times the query is not.
+template <typename T, int HD>
+__device__ __noinline__ float weights_redo(const WeightArgs &a, int layer, int slot, int kvh, int r, int q0, int N, const float *lse,
+                                           const int *last, float sl2) {
+    const int pg = a.v.page(slot, r);
+    const uint16_t *k = a.v.kv + a.v.row(layer, max(pg, 0), r) + kvh * HD;
+    float sum = 0.f;
+    for (int c = 0; c < N; c++) {
+        if (r > last[c]) continue;  // also: past the block's queries, or left out
+        const int t = a.sel[(size_t)slot * a.max_q + ((q0 + c) >> a.lg)];
+        const T *q = (const T *)a.q + layer * a.q_layer + t * a.q_ld + (long long)(kvh * a.G + ((q0 + c) & (a.G - 1))) * HD;
+        float x = 0.f;
+        for (int d = 0; d < HD; d++) x = fmaf((float)q[d], pg < 0 ? 0.f : bf16_bits_to_f32(k[d]), x);
+        sum += ex2(fmaf(x, sl2, lse[c]));
+    }
+    return sum;
+}
+
 // On a B200, in calls one after the other: 3 fp32 queries over 32 layers x
 // 4096 rows, 4 KV heads (139 MB) 32 us, 4.3 TB/s, bound by K's bytes after 6 us
 // until the first queries are there; 31 bf16 queries over 16 slots of about
@@ -368,7 +389,11 @@ __global__ void __launch_bounds__(kWtThreads, 1) cache_weights_tc(const __grid_c
                     }
                     um_fence_before();
                     mb_arrive(&sempty[group]);
-                    if (r < w.end) acc[r] = sum + ((part[0].x + part[0].y) + (part[1].x + part[1].y));
+                    if (r < w.end) {
+                        float add = (part[0].x + part[0].y) + (part[1].x + part[1].y);
+                        if (add != add) add = weights_redo<T, HD>(a, w.s_layer, w.s_slot, w.s_kvh, r, q0, N, s_lse[qb], s_last[qb], sl2);
+                        acc[r] = sum + add;
+                    }
                 }
                 mb_arrive(&qempty[qb]);
             }

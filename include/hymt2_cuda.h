@@ -410,7 +410,11 @@ typedef struct hyc_kv_view {
  * kv_heads in {1, 2, 4, 8}.  d_ws is scratch of at least
  * hyc_tree_attention_ws bytes, 256-byte aligned, used by this call alone until
  * it has run; its contents need no preparation.  K or V of rows that a node
- * does not see never reach its output, whatever they hold. */
+ * does not see never reach its output, whatever they hold.  Infinities and
+ * NaN in what it sees have the formulas' effect: a score of -inf drops its
+ * row (all of them: zeros and -inf), one of +inf gives an output of NaN and an
+ * lse of +inf, an infinite V gives that infinity (those nodes are done again
+ * one by one, which takes longer). */
 HYC_API int hyc_kvops_timeouts(void);
 HYC_API int hyc_kvops_wait_probe(unsigned long long limit_ns);
 HYC_API size_t hyc_tree_attention_ws(const hyc_kv_view *cache, int heads, int max_nodes);
@@ -449,7 +453,8 @@ HYC_API int hyc_tree_commit_n(void *stream, const hyc_kv_view *cache, int max_no
  * of d_q, fp32 or bf16, q_ld elements from token to token and q_layer from
  * layer to layer, and of d_lse [layers][lse_layer elements] as [tokens]
  * [heads].  A negative d_sel, and a query whose lse is -inf (it saw nothing),
- * is left out; what d_sel names must exist.  d_acc holds acc_rows rows per (l,
+ * is left out; what d_sel names must exist.  A score of -inf adds nothing, one
+ * of +inf infinity.  d_acc holds acc_rows rows per (l,
  * s, h), rows from acc_rows on are not accumulated.  The order of the sums
  * is fixed: the same inputs give the same bits. */
 HYC_API int hyc_cache_weights(void *stream, const hyc_kv_view *cache, int heads, int max_q, const int *d_len,

@@ -129,3 +129,125 @@ def test_padding_nodes_over_spoiled_rows(G, n, L, hd, bf16, bad):
     out, lse = run_tree(kv, pages, 0, lens, trees, q, n)
     assert (out[n - 2:n] == 0).all() and (lse[n - 2:n] == -np.inf).all()
     assert np.isfinite(out[n:]).all() and np.isfinite(lse[n:]).all()
+
+
+def exact_tree(kv, pages, lens, trees, q, G, scale):
+    """plain_tree with what infinities and NaN do: rows of score -inf drop out, +inf or NaN makes the output NaN (lse +inf
+    or NaN), infinite V gives infinities."""
+    nt, heads, hd = q.shape
+    out, lse, tol, tlse = np.zeros((nt, heads, hd)), np.full((nt, heads), -np.inf), np.zeros((nt, heads, 1)), np.zeros((nt, heads))
+    t0 = 0
+    with np.errstate(invalid="ignore"):
+        for s, par in enumerate(trees):
+            k, v = rows_of(kv, pages, 0, s, lens[s] + len(par))
+            for i, see in enumerate(ancestors(par)):
+                seen = np.array(list(range(lens[s])) + [lens[s] + j for j in see], dtype=int)
+                if not see:
+                    continue
+                for h in range(heads):
+                    qq, t = q[t0 + i, h].astype(np.float64), t0 + i
+                    x = scale * (k[seen, h // G] * qq).sum(-1)
+                    rows, x = seen[x != -np.inf], x[x != -np.inf]
+                    if not len(rows):
+                        continue
+                    if not np.isfinite(x).all():
+                        out[t, h], lse[t, h] = np.nan, np.nan if np.isnan(x).any() else np.inf
+                        continue
+                    kk, vv = k[rows, h // G], v[rows, h // G]
+                    ex = scale * (np.abs(kk) @ np.abs(qq)).max() * hd * 2.0 ** -23
+                    m, p = x.max(), np.exp(x - x.max())
+                    lse[t, h] = m + np.log(p.sum())
+                    out[t, h] = (p[:, None] * vv).sum(0) / p.sum()
+                    tol[t, h] = (2.1 * ex + 2.0 ** -18) * np.abs(vv[np.isfinite(vv)]).max()
+                    tlse[t, h] = ex + 2.0 ** -18 + 2.0 ** -22 * abs(lse[t, h])
+            t0 += len(par)
+    return out, lse, tol, tlse
+
+
+def same(got, want, tol):
+    f = np.isfinite(want)
+    with np.errstate(invalid="ignore"):
+        ok = np.where(f, np.abs(got - np.where(f, want, 0)) <= tol, (got == want) | (np.isnan(got) & np.isnan(want)))
+    return ok.all(), np.argwhere(~ok)[:5].tolist()
+
+
+@pytest.mark.parametrize("case", ["v_inf", "v_two", "v_nan", "v_far", "k_inf", "k_all", "k_nan", "drafted", "q_inf"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("G,n,L", [(4, 5, 40), (4, 5, 2000), (8, 13, 40), (8, 13, 2000), (4, 40, 900)])
+def test_infinities_in_rows_that_are_seen(G, n, L, hd, bf16, case):
+    """The formulas' effect, dim by dim, in both forms, in columns of one tile and split ones."""
+    import torch
+    rng = np.random.default_rng(L + n + hd)
+    kvh, inf, nan = 2, float("inf"), float("nan")
+    lens, trees = [L, 33], [random_tree(rng, n, pad=1), random_tree(rng, n)]
+    kv, pages = make_cache(rng, 1, kvh, hd, [L + n, 33 + n])
+    q = torch.from_numpy(rng.standard_normal((2 * n, kvh * G, hd)).astype(np.float32)).to(torch.bfloat16 if bf16 else torch.float32)
+    if case == "v_inf":
+        spoil(kv, pages, 0, L // 3, 1, inf, slice(2, 4))
+        spoil(kv, pages, 0, L - 1, 1, -inf, slice(hd - 9, hd))
+    elif case == "v_two":   # both signs in one dim: NaN there
+        spoil(kv, pages, 0, 0, 1, inf, slice(0, 3))
+        spoil(kv, pages, 0, L - 1, 1, -inf, slice(2, 7))
+    elif case == "v_nan":
+        spoil(kv, pages, 0, 7, 1, nan, slice(1, 2))
+    elif case == "v_far":   # a row whose probability is below fp32's range
+        spoil(kv, pages, 0, 5, 1, -inf, slice(6, 7))
+        q = q * 40
+        q[..., 9] = 60
+        spoil(kv, pages, 0, 5, 0, -8.0, slice(9, 10))
+    elif case == "k_inf":   # scores of -inf and of +inf, as the query's sign has it
+        spoil(kv, pages, 0, 3, 0, inf, slice(11, 12))
+        spoil(kv, pages, 0, L - 2, 0, -inf, slice(20, 21))
+    elif case == "k_all":   # every row of the tree's: all scores -inf or all +inf in each head
+        for r in range(L + n):
+            spoil(kv, pages, 0, r, 0, inf, slice(11, 12))
+    elif case == "k_nan":
+        spoil(kv, pages, 0, L // 2, 0, nan, slice(0, 1))
+    elif case == "drafted":
+        spoil(kv, pages, 0, L, 1, inf, slice(5, 6))
+        spoil(kv, pages, 0, L + 1, 0, -inf, slice(8, 9))
+        spoil(kv, pages, 0, L + 2, 1, nan, slice(hd - 1, hd))
+    else:
+        q[1, 0, 4], q[n + 2, 3, 7] = inf, -inf
+    sc = hd ** -0.5
+    out, lse = run_tree(kv, pages, 0, lens, trees, gpu(q), n)
+    want, wlse, tol, tlse = exact_tree(kv, pages, lens, trees, q.double().numpy(), G, sc)
+    if bf16:
+        tol = tol + np.where(np.isfinite(want), np.abs(want), 0) * 2.0 ** -8
+    assert not np.isfinite(want).all() or case == "v_far"
+    ok, where = same(out, want, tol)
+    assert ok, where
+    ok, where = same(lse, wlse, tlse)
+    assert ok, where
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hd,maxq", [(128, 5), (64, 40)])
+def test_weights_of_infinite_keys(hd, maxq, bf16):
+    """A key of +-inf adds nothing where the score is -inf, and infinity where it is +inf; NaN stays in its row."""
+    import torch
+    from hymt2_b200.kvcache import PagedKV
+    rng = np.random.default_rng(hd)
+    L, kvh, G = 300, 2, 4
+    kv, pages = make_cache(rng, 1, kvh, hd, [L + maxq])
+    spoil(kv, pages, 0, 10, 0, float("inf"), slice(3, 4))
+    spoil(kv, pages, 0, L + 1, 0, -float("inf"), slice(5, 6))
+    spoil(kv, pages, 0, 200, 0, float("nan"), slice(0, 1))
+    q = torch.from_numpy(rng.standard_normal((1, maxq, kvh * G, hd)).astype(np.float32)).to(torch.bfloat16 if bf16 else torch.float32)
+    q[:, :, :G, 3] = -q[:, :, :G, 3].abs()  # the first head's group: scores of -inf only
+    lse = torch.full((1, maxq, kvh * G), 4.0)
+    acc = torch.zeros(1, 1, kvh, L + maxq, device="cuda")
+    PagedKV(gpu(kv), gpu(pages)).add_weights(acc, gpu(q), gpu(lse), gpu(np.array([L], np.int32)), gpu(np.array([maxq], np.int32)),
+                                             gpu(np.arange(maxq, dtype=np.int32)[None]))
+    got, (k, _) = acc[0, 0].double().cpu().numpy(), rows_of(kv, pages, 0, 0, L + maxq)
+    for h in range(kvh):
+        qq = q[0, :, h * G:(h + 1) * G].double().numpy()
+        with np.errstate(invalid="ignore"):
+            x = (k[:, h][:, None, None] * qq[None]).sum(-1) * hd ** -0.5
+        x = np.where(np.arange(L + maxq)[:, None, None] <= L + np.arange(maxq)[None, :, None], x, -np.inf)
+        want = np.exp(x - 4.0).sum((1, 2))
+        # a score's error: hd products of 2^-23 of their sum of sizes, under 200 here; sums of up to 160 terms
+        ok, where = same(got[h], want, np.where(np.isfinite(want), want, 0) * (200 * hd ** -0.5 * hd * 2.0 ** -23 + 2.0 ** -16))
+        assert ok, (h, where)
+    assert np.isfinite(got[0, 10]) and np.isinf(got[1, 10]) and np.isnan(got[:, 200]).all()
