@@ -1917,6 +1917,7 @@ HYC_API int hyc_batch_forward(void *impl, const int *tokens, const int *tok_slot
     memcpy(b.h_in + T, tok_slot, (size_t)nt * 4);
     memcpy(b.h_in + 2 * T, tok_pos, (size_t)nt * 4);
     if (nout > 0) memcpy(b.h_in + 3 * T, out_rows, (size_t)nout * 4);
+    for (int t = 0; t < nt; t++) tree_fed(b, tok_slot[t]);
     if (!batch_upload(c, nt, nout) || !batch_run(c, nt, nout, vo)) return -1;
     if (nout > 0) {
         if (cudaMemcpyAsync(b.h_ids, b.d_ids, (size_t)nout * 4, cudaMemcpyDeviceToHost, c->st) != cudaSuccess) return -1;
@@ -1939,6 +1940,7 @@ HYC_API int hyc_batch_kv_copy(void *impl, int src_slot, int dst_slot, int npos) 
     const Batch &b = *c->bat;
     if (src_slot < 0 || src_slot >= b.slots || dst_slot < 0 || dst_slot >= b.slots || npos < 0 || npos > b.slot_ctx)
         return -1;
+    tree_fed(*c->bat, dst_slot);
     return kv_copy(c, src_slot, dst_slot, npos) && cudaStreamSynchronize(c->st) == cudaSuccess ? 0 : -1;
 }
 
@@ -1974,6 +1976,7 @@ HYC_API int hyc_tree_open(void *impl, int slot, int rows) {
     if (slot < 0 || slot >= b.slots || rows < 0 || rows > b.slot_ctx) return -1;
     TreeState &t = *b.tree;
     t.len[(size_t)slot] = t.pos[(size_t)slot] = rows;
+    t.fed[(size_t)slot] = 0;
     if (t.acc) {  // no query of this sequence has been counted yet
         const size_t col = (size_t)c->kvh * tree_rows(b) * 4;
         if (cudaMemset2DAsync((char *)t.acc + slot * col, b.slots * col, 0, col, (size_t)c->L, c->st) != cudaSuccess) {

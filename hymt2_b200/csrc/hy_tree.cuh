@@ -21,6 +21,7 @@ struct TreeState {
     int max_nodes = 0;
     bool weights = false;
     std::vector<int> len, pos;  // rows and next position of each slot
+    std::vector<char> fed;      // it has been written from outside since it was opened: len says nothing of its rows
     unsigned gave_up = 0;       // waits of the operators' kernels that had given up before
     // device ints, staged from pinned memory in one copy: len [S] | off [S + 1] |
     // forced [S] | parent [T] | row [T], then the outcome: len_out [S] |
@@ -31,9 +32,9 @@ struct TreeState {
     float *qkv = nullptr, *lse = nullptr, *acc = nullptr;  // [L][T][q | k | v], [L][T][heads], [L][S][kvh][rows]
     void *ws = nullptr;
     size_t ws_bytes = 0;
-    uint16_t *kv2 = nullptr;  // eviction copies into it and the two change places (lazy)
-    int *kept = nullptr;
+    int *kept = nullptr;  // eviction: [L][S][kvh][evict_rows], and the kept rows' weights (lazy)
     float *acc2 = nullptr;
+    int evict_rows = 0;
     int *d_len() const { return d_int; }
 };
 
@@ -42,7 +43,7 @@ int tree_rows(const Batch &b) { return b.page_max * kPageRows; }
 void tree_free(Batch *b) {
     TreeState *t = b->tree;
     if (!t) return;
-    void *ptrs[] = {t->d_int, t->qkv, t->lse, t->acc, t->ws, t->kv2, t->kept, t->acc2};
+    void *ptrs[] = {t->d_int, t->qkv, t->lse, t->acc, t->ws, t->kept, t->acc2};
     for (void *p : ptrs) cudaFree(p);
     if (t->h_int) cudaFreeHost(t->h_int);
     delete t;
@@ -89,6 +90,7 @@ bool tree_prepare(HyCtx *c, int max_nodes, bool weights) {
     t->weights = weights;
     t->len.assign(S, 0);
     t->pos.assign(S, 0);
+    t->fed.assign(S, 0);
     t->in_ints = 3 * S + 1 + 2 * T;
     t->ints = t->in_ints + 3 * S + S * max_nodes;
     CK(c, cudaMalloc(&t->d_int, t->ints * 4));
@@ -200,6 +202,7 @@ bool tree_run(HyCtx *c, const int *tokens, const int *parent, const int *off, co
     CK(c, cudaMemcpyAsync(t.h_int + t.in_ints, out, (t.ints - t.in_ints) * 4, cudaMemcpyDeviceToHost, c->st));
     if (!tree_waits(c, t, false) || !tc_status(c)) return false;
     for (int s = 0; s < S; s++) {
+        if (off[s + 1] > off[s]) t.fed[s] = 0;
         t.len[s] = t.h_int[t.in_ints + s];
         t.pos[s] += t.h_int[t.in_ints + S + s];
     }
@@ -212,27 +215,40 @@ bool tree_evict(HyCtx *c, int budget, int sinks, int recent) {
     REQ(c, t.weights, "eviction needs accumulated weights (hyc_tree_prepare)");
     REQ(c, budget >= 1 && budget <= tree_rows(b) && sinks >= 0 && recent >= 0 && sinks <= budget - recent,
         "the budget must hold sinks + recent rows and fit a slot");
-    if (*std::max_element(t.len.begin(), t.len.end()) <= budget) return true;
     const size_t S = (size_t)b.slots, cols = (size_t)c->L * S * c->kvh, R = (size_t)tree_rows(b);
-    if (!t.kv2) {
-        CK(c, cudaMalloc(&t.kv2, b.kv_elems(c) * 2));
-        CK(c, cudaMemsetAsync(t.kv2, 0, b.kv_elems(c) * 2, c->st));
-        CK(c, cudaMalloc(&t.kept, cols * R * 4));
-        CK(c, cudaMalloc(&t.acc2, cols * R * 4));
+    // a fed slot goes in as one that is within the budget: nothing of it moves
+    bool any = false;
+    for (size_t s = 0; s < S; s++) {
+        any |= t.len[s] > budget && !t.fed[s];
+        t.h_int[s] = t.fed[s] ? std::min(t.len[s], budget) : t.len[s];
+    }
+    if (!any) return true;
+    if (t.evict_rows < budget) {
+        cudaFree(t.kept);
+        cudaFree(t.acc2);
+        t.kept = nullptr;
+        t.acc2 = nullptr;
+        t.evict_rows = 0;
+        CK(c, cudaMalloc(&t.kept, cols * budget * 4));
+        CK(c, cudaMalloc(&t.acc2, cols * budget * 4));
+        t.evict_rows = budget;
     }
     int *out = t.d_int + t.in_ints;
-    memcpy(t.h_int, t.len.data(), S * 4);
     CK(c, cudaMemcpyAsync(t.d_int, t.h_int, S * 4, cudaMemcpyHostToDevice, c->st));
-    const hyc_kv_view src = tree_view(c, b.kv), dst = tree_view(c, t.kv2);
-    if (hyc_cache_evict(c->st, &src, &dst, t.d_len(), t.acc, (int)R, budget, sinks, recent, out, t.kept, t.acc2, c->err,
+    const hyc_kv_view v = tree_view(c, b.kv);
+    if (hyc_cache_evict(c->st, &v, &v, t.d_len(), t.acc, (int)R, budget, sinks, recent, out, t.kept, t.acc2, c->err,
                         sizeof c->err) != 0) {
         c->broken = true;
         return false;
     }
     c->launches += 2;
     CK(c, cudaMemcpy2DAsync(t.acc, R * 4, t.acc2, (size_t)budget * 4, (size_t)budget * 4, cols, cudaMemcpyDeviceToDevice, c->st));
-    std::swap(b.kv, t.kv2);
     CK(c, cudaStreamSynchronize(c->st));
-    for (size_t s = 0; s < S; s++) t.len[s] = std::min(t.len[s], budget);
+    for (size_t s = 0; s < S; s++)
+        if (!t.fed[s]) t.len[s] = std::min(t.len[s], budget);
     return true;
+}
+
+void tree_fed(Batch &b, int slot) {
+    if (b.tree) b.tree->fed[(size_t)slot] = 1;
 }

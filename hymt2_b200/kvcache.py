@@ -177,7 +177,7 @@ class PagedKV:
     def evict(self, dst: "PagedKV", lens: torch.Tensor, acc: torch.Tensor, budget: int, sinks: int, recent: int):
         """(new lens, kept rows, their weights): the first `sinks`, the last `recent` and the heaviest other rows of
         every layer, slot and KV head, `budget` in all, copied in order into `dst`, whose pages hold none of this
-        cache's rows.  kept and weights are [layers][slots][kv_heads][budget], -1 and 0 behind a shorter slot."""
+        cache's rows, or which is this cache itself (its rows then move up within it).  kept and weights are [layers][slots][kv_heads][budget], -1 and 0 behind a shorter slot."""
         if acc.dim() != 4 or dst._dev != self._dev or budget < 1:
             raise ValueError("acc must be [layers][slots][kv_heads][rows], both caches on one device, budget positive")
         w = self._floats("acc", acc, (self.layers, self.slots, self.kv_heads, acc.shape[3]))

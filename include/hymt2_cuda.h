@@ -225,7 +225,9 @@ HYC_API int hyc_serve(void *impl, const int *prompts, const int *prompt_off, int
  * as a prompt's last tokens.  The ids are those of one-token steps.
  * hyc_tree_evict: every slot with more than budget rows keeps its first
  * `sinks`, last `recent` and, in each layer and KV head, its heaviest other
- * rows, budget in all; positions go on.
+ * rows, budget in all; positions go on.  All other rows stay as they are, and
+ * so does a slot that hyc_batch_forward or hyc_batch_kv_copy has written since
+ * it was opened: the next hyc_tree_open says what it holds.
  * hyc_tree_state: a slot's rows and next position, and (optional, where
  * weights are kept) its weights [layers][kv_heads][rows].
  * hyc_batch_kv_read reads the slot's rows.  All return 0 or -1
@@ -474,8 +476,10 @@ HYC_API int hyc_cache_weights_n(void *stream, const hyc_kv_view *cache, int head
  * slots and heads with room for budget rows a slot.  d_kept [layers][slots]
  * [kv_heads][budget] receives the kept rows (-1 behind them), d_acc_out,
  * shaped alike, their weights (0 behind them), d_len_out[s] = min(n, budget).
- * Pages of `dst` must not be pages of `cache` that a slot still reads, and no
- * page may serve two slots of `dst`.  acc_rows must cover every d_len. */
+ * `dst` may be `cache` itself (the same view): rows then move within it, and
+ * slots of budget rows or fewer are not touched.  Otherwise pages of `dst` must
+ * not be pages of `cache` that a slot still reads; and no page may serve two
+ * slots of `dst`.  acc_rows must cover every d_len. */
 HYC_API int hyc_cache_evict(void *stream, const hyc_kv_view *cache, const hyc_kv_view *dst, const int *d_len,
                             const float *d_acc, int acc_rows, int budget, int sinks, int recent, int *d_len_out,
                             int *d_kept, float *d_acc_out, char *err, int err_cap);

@@ -251,3 +251,35 @@ def test_weights_of_infinite_keys(hd, maxq, bf16):
         ok, where = same(got[h], want, np.where(np.isfinite(want), want, 0) * (200 * hd ** -0.5 * hd * 2.0 ** -23 + 2.0 ** -16))
         assert ok, (h, where)
     assert np.isfinite(got[0, 10]) and np.isinf(got[1, 10]) and np.isnan(got[:, 200]).all()
+
+
+# ---------------------------------------------------------------- eviction within one cache
+
+@pytest.mark.parametrize("hd,kvh", [(128, 2), (64, 3)])
+@pytest.mark.parametrize("budget,sinks,recent", [(1, 0, 0), (1, 0, 1), (63, 4, 8), (64, 0, 0), (65, 30, 34), (513, 3, 100), (2000, 4, 4)])
+def test_evict_within_the_cache(hd, kvh, budget, sinks, recent):
+    """The same rows, lists and weights as into another cache; slots within the budget, rows behind a slot's and pages of
+    no slot stay."""
+    import torch
+    from hymt2_b200.kvcache import PagedKV
+    rng = np.random.default_rng(budget + hd)
+    layers, lens = 2, [0, 1, budget, budget + 1, 700, 1030, 2047]
+    S, R = len(lens), 2064
+    kv, pages = make_cache(rng, layers, kvh, hd, [R] * S)
+    acc = gpu(np.round(np.exp(3 * rng.standard_normal((layers, S, kvh, R)))).astype(np.float32))
+    acc[1, 5] = acc[1, 5].flip(-1).cumsum(-1)   # one slot whose last rows are the heaviest
+    acc[0, 6] = acc[0, 6].cumsum(-1).flip(-1)   # and one whose first are
+    ln = gpu(np.array(lens, np.int32))
+    one, two = gpu(kv), gpu(kv)
+    page_max = -(-budget // PAGE)
+    dst, dpages = torch.zeros(layers, S * page_max, 2, PAGE, kvh, hd, dtype=torch.bfloat16, device="cuda"), np.arange(S * page_max).reshape(S, page_max)
+    want = PagedKV(one, gpu(pages)).evict(PagedKV(dst, gpu(dpages.astype(np.int32))), ln, acc, budget, sinks, recent)
+    cache = PagedKV(two, gpu(pages))
+    got = cache.evict(cache, ln, acc, budget, sinks, recent)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    full, moved, dst = kv.clone(), two.cpu(), dst.cpu()
+    for s in range(S):
+        if lens[s] > budget:
+            j = np.arange(budget)
+            full[:, pages[s, j // PAGE], :, j % PAGE] = dst[:, dpages[s, j // PAGE], :, j % PAGE]
+    assert torch.equal(moved, full)
