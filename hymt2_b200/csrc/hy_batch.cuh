@@ -111,6 +111,7 @@ __global__ void kv_copy_page(uint16_t *kv, size_t layer_stride, long long page_s
 // ---------------------------------------------------------------- host side
 
 void tree_free(Batch *b);
+void tree_close_all(Batch &b);
 void fwd_tree(HyCtx *c, Fwd &f);
 
 void batch_free(HyCtx *c) {
@@ -308,6 +309,7 @@ bool serve_run(HyCtx *c, const int *prompts, const int *off, int nreq, int max_n
     PagePool pool;
     pool.reset(b.npages);
     for (int i = 0; i < S * PM; i++) b.h_pages[i] = 0;  // rows of idle slots are never read
+    tree_close_all(b);  // the requests' rows take the place of the drafted sequences'
     bool table_dirty = true;
     // the page holding position pos of q, allocated (with any before it) on first use
     auto need_page = [&](ServeSeq &q, int pos) -> bool {

@@ -249,6 +249,13 @@ bool tree_evict(HyCtx *c, int budget, int sinks, int recent) {
     return true;
 }
 
+void tree_close_all(Batch &b) {
+    if (!b.tree) return;
+    b.tree->len.assign(b.tree->len.size(), 0);
+    b.tree->pos.assign(b.tree->pos.size(), 0);
+    b.tree->fed.assign(b.tree->fed.size(), 0);
+}
+
 void tree_fed(Batch &b, int slot) {
     if (b.tree) b.tree->fed[(size_t)slot] = 1;
 }

@@ -213,6 +213,7 @@ HYC_API int hyc_serve(void *impl, const int *prompts, const int *prompt_off, int
  * slots are empty.
  * hyc_tree_open: slot holds rows 0 .. rows - 1, filled by hyc_batch_forward at
  * positions 0 .. rows - 1, and goes on at position rows; its weights are zero.
+ * hyc_serve uses the same rows: after it all slots are empty.
  * hyc_tree_forward: one pass.  Slot s gets the nodes off[s] .. off[s + 1] - 1
  * (host arrays, off [slots + 1], off[0] = 0; no nodes leaves the slot as it
  * is): node 0 is the token its sequence ends with (parent -1), every other

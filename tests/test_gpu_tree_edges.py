@@ -111,3 +111,23 @@ def test_a_slot_goes_on_after_a_cut(backend, synth, model_dir):
         assert dm.tree_state(0)[0] == 20
     finally:
         dm.close()
+
+
+def test_the_server_empties_the_slots(backend, synth, model_dir):
+    """hyc_serve puts its requests' rows where the drafted sequences' were, so nothing of those is left to go on from."""
+    rng = np.random.default_rng(11)
+    ids = rng.integers(0, 900, 40).tolist()
+    dm = _open(backend, synth, model_dir, slots=2, weights=True)
+    try:
+        fresh = dm.tree_forward({0: ([ids[0]], [-1])}, 2)[0]
+        dm.tree_open(0, 0)
+        dm.batch_forward(ids[:-1], [0] * 39, list(range(39)), [])
+        dm.tree_open(0, 39)
+        dm.tree_forward({0: ([ids[-1]], [-1])}, 2)
+        assert dm.tree_state(0)[:2] == (40, 40)
+        dm.serve([rng.integers(0, 900, 20).tolist()], 4, 32)
+        assert [dm.tree_state(s)[:2] for s in (0, 1)] == [(0, 0)] * 2
+        assert dm.tree_forward({0: ([ids[0]], [-1])}, 2)[0] == fresh
+        assert np.allclose(dm.tree_state(0, weights=True)[2].sum(-1), dm.hp.heads // dm.hp.kv_heads, rtol=1e-4)
+    finally:
+        dm.close()
