@@ -58,7 +58,8 @@ def generate(dm, prompts, max_new: int, draft=None, stop=(), budget: int = 0, si
     """Greedy ids for a few prompts at once, one slot each (dm.batch_prepare and dm.tree_prepare done before).
 
     draft(ids) -> (tokens, parents): a tree whose node 0 is ids[-1].  budget > 0 bounds every slot's cache: it is cut
-    back to budget rows when it has over `slack` more (a cut copies what stays).  The last `window` prompt tokens then
+    back to budget rows when it has over `slack` more, or more and no room for the next tree (a cut copies what stays).
+    A slot that has no row or position left ends early, with the ids so far.  The last `window` prompt tokens then
     go through a tree pass, so that their queries' weights are counted.  Returns (ids per prompt, DraftStats)."""
     draft = draft or PromptLookup()
     stop, n = set(int(t) for t in stop), len(prompts)
@@ -79,15 +80,19 @@ def generate(dm, prompts, max_new: int, draft=None, stop=(), budget: int = 0, si
     out: list[list[int]] = [[] for _ in range(n)]
     live = [s for s in range(n) if max_new > 0]
     while live:
-        if budget and max(dm.tree_state(s)[0] for s in live) > budget + slack:
+        drafts = {s: draft(ids[s] + out[s]) for s in live}
+        state = {s: dm.tree_state(s) for s in live}
+        if budget and any(state[s][0] > min(budget + slack, max(budget, dm.batch_ctx - min(len(drafts[s][0]), dm.tree_nodes)))
+                          for s in live):
             dm.tree_evict(budget, sinks, recent)
             stats.evictions += 1
-        trees = {}
-        for s in live:  # as many nodes as the slot and the context have room for
-            rows, pos, _ = dm.tree_state(s)
-            room = max(1, min(dm.tree_nodes, dm.batch_ctx - rows, dm.ctx - pos))
-            tk, pa = draft(ids[s] + out[s])
-            trees[s] = tk[:room], pa[:room]
+            state = {s: dm.tree_state(s) for s in live}
+        # as many nodes as the slot and the context have room for
+        room = {s: min(dm.tree_nodes, dm.batch_ctx - state[s][0], dm.ctx - state[s][1]) for s in live}
+        live = [s for s in live if room[s] > 0]
+        if not live:
+            break
+        trees = {s: (drafts[s][0][:room[s]], drafts[s][1][:room[s]]) for s in live}
         got = dm.tree_forward(trees, dm.batch_slots)
         stats.passes += 1
         stats.nodes += sum(len(t) for t, _ in trees.values())
