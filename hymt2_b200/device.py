@@ -311,7 +311,7 @@ class DeviceModel:
         mo = slots if max_out is None else max_out
         if self.be.lib.hyc_batch_prepare(self.be.impl, slots, slot_ctx, max_tokens, mo) != 0:
             raise BackendError("batch_prepare: " + self.be.error())
-        self.batch_slots, self.batch_ctx, self.batch_tokens = slots, slot_ctx, max_tokens
+        self.batch_slots, self.batch_ctx, self.batch_tokens, self.batch_out = slots, slot_ctx, max_tokens, mo
         self.batch_vocab = self.g.tensors.get("output.weight", self.g.tensors["token_embd.weight"]).n
 
     def batch_forward(self, tokens, slots, positions, out_rows, want_logits: bool = False):

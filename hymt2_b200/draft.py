@@ -74,9 +74,15 @@ def generate(dm, prompts, max_new: int, draft=None, stop=(), budget: int = 0, si
     for s in range(n):
         dm.tree_open(s, keep[s])
     if budget:
-        chains = {s: (p[keep[s]:-1], list(range(-1, len(p) - keep[s] - 2))) for s, p in enumerate(ids) if keep[s] < len(p) - 1}
-        if chains:
-            dm.tree_forward(chains, dm.batch_slots, forced=chains)
+        chain = {s: p[keep[s]:-1] for s, p in enumerate(ids)}
+        while any(chain.values()):  # in passes of as many nodes as a tree and a pass may have
+            part, left = {}, min(dm.batch_tokens, dm.batch_out)
+            for s, c in chain.items():
+                m = min(len(c), dm.tree_nodes, left)
+                if m > 0:
+                    part[s] = c[:m], list(range(-1, m - 1))
+                    chain[s], left = c[m:], left - m
+            dm.tree_forward(part, dm.batch_slots, forced=part)
     out: list[list[int]] = [[] for _ in range(n)]
     live = [s for s in range(n) if max_new > 0]
     while live:

@@ -103,3 +103,22 @@ def test_a_slot_without_room_ends_early(kw, most, draft):
     want = [plain(PROMPT, 100), plain(PROMPT[:20], 100)]
     assert [len(o) for o in out] == [most - 50 + 1, most - 20 + 1]   # the last row's token too
     assert all(o == w[:len(o)] for o, w in zip(out, want))
+
+
+@pytest.mark.parametrize("nodes", [1, 3, 8, 15])
+@pytest.mark.parametrize("window", [0, 1, 7, 16, 100])
+def test_a_window_wider_than_a_tree(nodes, window):
+    """The prompt's last tokens go in as chains of as many nodes as a tree has, each query counted once."""
+    dm = Engine(nodes=nodes)
+    out, _ = generate(dm, [PROMPT], 5, budget=60, window=window)
+    assert out == [plain(PROMPT, 5)]
+    assert dm.counted[0] == min(window, len(PROMPT) - 1) + dm.pos[0] - (len(PROMPT) - 1)
+
+
+@pytest.mark.parametrize("max_tokens,max_out", [(64, 64), (64, 17), (6, 6)])
+def test_windows_of_more_tokens_than_a_pass(max_tokens, max_out):
+    dm = Engine(slots=6, max_tokens=max_tokens, max_out=max_out)
+    prompts = [PROMPT[i:] for i in range(6)]
+    out, _ = generate(dm, prompts, 1, lambda ids: ([ids[-1]], [-1]), budget=60)
+    assert out == [plain(p, 1) for p in prompts]
+    assert all(c >= 16 for c in dm.counted)
