@@ -44,6 +44,17 @@ class PromptLookup:
         return tokens, parents
 
 
+def _shares(want: list[int], most: int) -> list[int]:
+    """Of `most` nodes, what each gets: an equal share, or what it wants where that is less, and what those leave in turn."""
+    got = [min(w, most // len(want)) for w in want]
+    left = most - sum(got)
+    for i, w in enumerate(want):
+        more = min(w - got[i], left)
+        got[i] += more
+        left -= more
+    return got
+
+
 @dataclass
 class DraftStats:
     passes: int = 0
@@ -59,8 +70,9 @@ def generate(dm, prompts, max_new: int, draft=None, stop=(), budget: int = 0, si
 
     draft(ids) -> (tokens, parents): a tree whose node 0 is ids[-1].  budget > 0 bounds every slot's cache: it is cut
     back to budget rows when it has over `slack` more, or more and no room for the next tree (a cut copies what stays).
-    A slot that has no row or position left ends early, with the ids so far.  The last `window` prompt tokens then
-    go through a tree pass, so that their queries' weights are counted.  Returns (ids per prompt, DraftStats)."""
+    The last `window` prompt tokens then go through tree passes, so that their queries' weights are counted.  The slots
+    share a pass's tokens; one that has no row or position left ends early, with the ids so far.  Returns (ids per
+    prompt, DraftStats)."""
     draft = draft or PromptLookup()
     stop, n = set(int(t) for t in stop), len(prompts)
     ids = [[int(t) for t in p] for p in prompts]
@@ -98,11 +110,13 @@ def generate(dm, prompts, max_new: int, draft=None, stop=(), budget: int = 0, si
         live = [s for s in live if room[s] > 0]
         if not live:
             break
-        trees = {s: (drafts[s][0][:room[s]], drafts[s][1][:room[s]]) for s in live}
+        share = _shares([min(room[s], len(drafts[s][0])) for s in live], min(dm.batch_tokens, dm.batch_out))
+        trees = {s: (drafts[s][0][:m], drafts[s][1][:m]) for s, m in zip(live, share) if m > 0}
+        live = [s for s in live if s not in trees] + list(trees)  # who had to wait is first in the next pass
         got = dm.tree_forward(trees, dm.batch_slots)
         stats.passes += 1
         stats.nodes += sum(len(t) for t, _ in trees.values())
-        for s in list(live):
+        for s in trees:
             path, nxt = got[s]
             for t in path[1:] + [nxt]:
                 if t in stop:

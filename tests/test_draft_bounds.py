@@ -122,3 +122,14 @@ def test_windows_of_more_tokens_than_a_pass(max_tokens, max_out):
     out, _ = generate(dm, prompts, 1, lambda ids: ([ids[-1]], [-1]), budget=60)
     assert out == [plain(p, 1) for p in prompts]
     assert all(c >= 16 for c in dm.counted)
+
+
+@pytest.mark.parametrize("draft", DRAFTS)
+@pytest.mark.parametrize("slots,max_tokens,max_out", [(16, 128, 128), (5, 64, 20), (6, 6, 6), (6, 5, 5), (6, 64, 4), (3, 1, 1)])
+def test_trees_of_more_nodes_than_a_pass(slots, max_tokens, max_out, draft):
+    """The live slots share a pass's tokens; where there are fewer tokens than slots, slots take turns."""
+    dm = Engine(slots=slots, max_tokens=max_tokens, max_out=max_out, slot_ctx=128)
+    prompts = [PROMPT[i:] for i in range(slots)]
+    out, st = generate(dm, prompts, 20, draft, budget=100)
+    assert out == [plain(p, 20) for p in prompts]
+    assert st.nodes <= st.passes * min(max_tokens, max_out)
