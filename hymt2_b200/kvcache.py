@@ -142,8 +142,10 @@ class PagedKV:
         The path runs from node 0 to the first child whose token is next_tokens of the node before, and so on; its
         rows move up to rows lens[s] .. in every layer.  Slots with forced[s] != 0 take all their nodes."""
         nt, one = (tokens.shape[0],), (self.slots,)
-        args = (self._ints("lens", lens, one), self._ints("offsets", offsets, (self.slots + 1,)), self._ints("parent", parent, nt),
-                self._ints("tokens", tokens, nt), self._ints("next_tokens", next_tokens, nt),
+        none = self._view.kv  # no token: the library wants pointers, and reads nothing through them
+        args = (self._ints("lens", lens, one), self._ints("offsets", offsets, (self.slots + 1,)),
+                self._ints("parent", parent, nt) or none, self._ints("tokens", tokens, nt) or none,
+                self._ints("next_tokens", next_tokens, nt) or none,
                 None if forced is None else self._ints("forced", forced, one))
         new_lens, accepted, bonus = lens.new_empty(self.slots), lens.new_empty(self.slots), lens.new_empty(self.slots)
         path = lens.new_empty(self.slots, max(max_nodes, 0))
@@ -168,10 +170,11 @@ class PagedKV:
         w = self._floats("acc", acc, (self.layers, self.slots, self.kv_heads, acc.shape[3]))
         ln, nq = self._ints("lens", lens, (self.slots,)), self._ints("n_query", n_query, (self.slots,))
         se = self._ints("sel", sel, (self.slots, sel.shape[1]))
-        if nt == 0:
+        if sel.shape[1] == 0:
             return
-        self._call(self._lib.hyc_cache_weights_n, self._stream(), self._ref, heads, sel.shape[1], nt, ln, nq, se, q.data_ptr(),
-                   st[1] if nt > 1 else heads * hd, st[0] if self.layers > 1 else 0, bf16, e, nt * heads,
+        none = self._view.kv  # no token: the library wants pointers, and reads nothing through them
+        self._call(self._lib.hyc_cache_weights_n, self._stream(), self._ref, heads, sel.shape[1], nt, ln, nq, se,
+                   q.data_ptr() or none, st[1] if nt > 1 else heads * hd, st[0] if self.layers > 1 else 0, bf16, e or none, nt * heads,
                    hd ** -0.5 if scale is None else scale, w, acc.shape[3])
 
     def evict(self, dst: "PagedKV", lens: torch.Tensor, acc: torch.Tensor, budget: int, sinks: int, recent: int):

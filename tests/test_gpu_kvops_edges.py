@@ -283,3 +283,37 @@ def test_evict_within_the_cache(hd, kvh, budget, sinks, recent):
             j = np.arange(budget)
             full[:, pages[s, j // PAGE], :, j % PAGE] = dst[:, dpages[s, j // PAGE], :, j % PAGE]
     assert torch.equal(moved, full)
+
+
+# ---------------------------------------------------------------- calls without tokens or queries
+
+def test_commit_without_tokens():
+    """No slot drafts anything: every length stays, nothing is accepted or moved."""
+    import torch
+    from hymt2_b200.kvcache import PagedKV
+    rng = np.random.default_rng(3)
+    kv, pages = make_cache(rng, 2, 1, 64, [40, 40])
+    d, none = gpu(kv), torch.empty(0, dtype=torch.int32, device="cuda")
+    lens = gpu(np.array([7, 0], np.int32))
+    for forced in (None, gpu(np.array([1, 0], np.int32))):
+        ln, n, path, bonus = PagedKV(d, gpu(pages)).tree_commit(lens, gpu(np.zeros(3, np.int32)), none, none, none, 4, forced=forced)
+        assert ln.tolist() == [7, 0] and n.tolist() == [0, 0] and bonus.tolist() == [-1, -1] and bool((path == -1).all())
+    assert torch.equal(d.cpu(), kv)
+
+
+def test_weights_without_queries_or_tokens():
+    import torch
+    from hymt2_b200.kvcache import PagedKV
+    rng = np.random.default_rng(3)
+    kv, pages = make_cache(rng, 1, 2, 64, [40, 40])
+    cache, lens = PagedKV(gpu(kv), gpu(pages)), gpu(np.array([7, 20], np.int32))
+    acc = torch.ones(1, 2, 2, 48, device="cuda")
+    q, lse = torch.randn(1, 3, 4, 64, device="cuda"), torch.zeros(1, 3, 4, device="cuda")
+    zero = gpu(np.zeros(2, np.int32))
+    cache.add_weights(acc, q, lse, lens, zero, gpu(np.zeros((2, 0), np.int32)))
+    cache.add_weights(acc, q, lse, lens, zero, gpu(np.zeros((2, 5), np.int32)))
+    cache.add_weights(acc, q[:, :0], lse[:, :0], lens, zero, gpu(np.zeros((2, 5), np.int32)))
+    assert bool((acc == 1).all())
+    # queries that are not there are left out; their rows start from zero like any
+    cache.add_weights(acc, q[:, :0], lse[:, :0], lens, gpu(np.array([2, 0], np.int32)), gpu(np.zeros((2, 5), np.int32)))
+    assert bool((acc[0, 0, :, 7:9] == 0).all()) and float(acc.sum()) == 2 * 2 * 48 - 4
