@@ -8,8 +8,9 @@ them (`evict`).  No counterpart in the reference, whose loop decodes one token
 per step (src/model.c:943-954) over a cache that only grows (:804-808).
 
 All work runs on torch's current stream of the cache's device and nothing
-synchronises (but `check_waits`).  tree_attention's scratch is one per stream (a captured call's own, unless its stream has
-one: then a replay must not run beside calls on that stream).  Shapes, types and strides are checked here and by the library
+synchronises (but `check_waits`).  tree_attention's scratch is one buffer a
+stream, of the largest call so far; a captured call has one of its own, in its
+graph's memory.  Shapes, types and strides are checked here and by the library
 (`BackendError`); what the arrays hold is not read back: lengths, offsets,
 parents and selected tokens are bounded on the device as the header states (its
 forms that take the number of tokens).
@@ -26,9 +27,11 @@ from .device import BackendError, load_library
 PAGE_ROWS = 16
 TREE_MAX = 64  # nodes of one tree
 
-# The raw handle of a device's current stream without a Stream object around it, where torch has that call.
+# The raw handle of a device's current stream without a Stream object around it, and whether it is being captured, where
+# torch has those calls.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_is_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
 
 
 class PagedKV:
@@ -54,6 +57,8 @@ class PagedKV:
         self._lib = load_library()
         self._err = C.create_string_buffer(256)
         self._ws: dict = {}  # scratch of tree_attention: one per stream, so that calls on two never share it
+        self._fit: dict = {}  # (stream, heads, max_nodes) for which the stream's is known to be large enough
+        self._none = kv.data_ptr()  # in place of an empty array: the library wants pointers, and reads nothing through these
 
     def _ints(self, name: str, t: torch.Tensor, shape: tuple) -> int:
         if t.dtype is not torch.int32 or t.shape != shape or t.get_device() != self._dev or not t.is_contiguous():
@@ -85,6 +90,25 @@ class PagedKV:
 
     def _stream(self) -> int:
         return _raw_stream(self._dev)
+
+    def _capturing(self) -> bool:
+        if torch.cuda.current_device() == self._dev:
+            return _is_capturing()
+        with torch.cuda.device(self._dev):
+            return _is_capturing()
+
+    def _scratch(self, stream: int, heads: int, max_nodes: int) -> tuple:
+        need = max(self._lib.hyc_tree_attention_ws(self._ref, heads, max_nodes), 16)
+        ws = None if self._capturing() else self._ws.get(stream)
+        if ws is None or ws[2] < need:
+            buf = torch.empty(need, dtype=torch.uint8, device=self.device)
+            ws = (buf, buf.data_ptr(), need)
+            if self._capturing():
+                return ws
+            self._ws[stream] = ws
+            self._fit = {k: v for k, v in self._fit.items() if k[0] != stream}
+        self._fit[stream, heads, max_nodes] = ws
+        return ws
 
     def check_waits(self) -> None:
         """Waits for the device and raises BackendError when a wait inside one of these kernels has given up on it since
@@ -124,13 +148,9 @@ class PagedKV:
         if nt == 0:
             return out, lse
         stream = self._stream()
-        ws = self._ws.get((stream, heads, max_nodes))
+        ws = None if (_is_capturing() if self._only else self._capturing()) else self._fit.get((stream, heads, max_nodes))
         if ws is None:
-            need = self._lib.hyc_tree_attention_ws(self._ref, heads, max_nodes)
-            buf = torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
-            ws = (buf, buf.data_ptr(), buf.numel())
-            if not torch.cuda.is_current_stream_capturing():  # a graph keeps a scratch of its own
-                self._ws[(stream, heads, max_nodes)] = ws
+            ws = self._scratch(stream, heads, max_nodes)
         self._call(self._lib.hyc_tree_attention_n, stream, self._ref, layer, heads, max_nodes, nt, ln, of, pa, q.data_ptr(),
                    old, bf16, hd ** -0.5 if scale is None else scale, out.data_ptr(), old_out, lse.data_ptr(), ws[1], ws[2])
         return out, lse
@@ -142,10 +162,9 @@ class PagedKV:
         The path runs from node 0 to the first child whose token is next_tokens of the node before, and so on; its
         rows move up to rows lens[s] .. in every layer.  Slots with forced[s] != 0 take all their nodes."""
         nt, one = (tokens.shape[0],), (self.slots,)
-        none = self._view.kv  # no token: the library wants pointers, and reads nothing through them
         args = (self._ints("lens", lens, one), self._ints("offsets", offsets, (self.slots + 1,)),
-                self._ints("parent", parent, nt) or none, self._ints("tokens", tokens, nt) or none,
-                self._ints("next_tokens", next_tokens, nt) or none,
+                self._ints("parent", parent, nt) or self._none, self._ints("tokens", tokens, nt) or self._none,
+                self._ints("next_tokens", next_tokens, nt) or self._none,
                 None if forced is None else self._ints("forced", forced, one))
         new_lens, accepted, bonus = lens.new_empty(self.slots), lens.new_empty(self.slots), lens.new_empty(self.slots)
         path = lens.new_empty(self.slots, max(max_nodes, 0))
@@ -172,15 +191,15 @@ class PagedKV:
         se = self._ints("sel", sel, (self.slots, sel.shape[1]))
         if sel.shape[1] == 0:
             return
-        none = self._view.kv  # no token: the library wants pointers, and reads nothing through them
         self._call(self._lib.hyc_cache_weights_n, self._stream(), self._ref, heads, sel.shape[1], nt, ln, nq, se,
-                   q.data_ptr() or none, st[1] if nt > 1 else heads * hd, st[0] if self.layers > 1 else 0, bf16, e or none, nt * heads,
-                   hd ** -0.5 if scale is None else scale, w, acc.shape[3])
+                   q.data_ptr() or self._none, st[1] if nt > 1 else heads * hd, st[0] if self.layers > 1 else 0, bf16,
+                   e or self._none, nt * heads, hd ** -0.5 if scale is None else scale, w, acc.shape[3])
 
     def evict(self, dst: "PagedKV", lens: torch.Tensor, acc: torch.Tensor, budget: int, sinks: int, recent: int):
         """(new lens, kept rows, their weights): the first `sinks`, the last `recent` and the heaviest other rows of
         every layer, slot and KV head, `budget` in all, copied in order into `dst`, whose pages hold none of this
-        cache's rows, or which is this cache itself (its rows then move up within it).  kept and weights are [layers][slots][kv_heads][budget], -1 and 0 behind a shorter slot."""
+        cache's rows, or which is this cache itself (its rows then move up within it).  kept and weights are
+        [layers][slots][kv_heads][budget], -1 and 0 behind a shorter slot."""
         if acc.dim() != 4 or dst._dev != self._dev or budget < 1:
             raise ValueError("acc must be [layers][slots][kv_heads][rows], both caches on one device, budget positive")
         w = self._floats("acc", acc, (self.layers, self.slots, self.kv_heads, acc.shape[3]))

@@ -317,3 +317,73 @@ def test_weights_without_queries_or_tokens():
     # queries that are not there are left out; their rows start from zero like any
     cache.add_weights(acc, q[:, :0], lse[:, :0], lens, gpu(np.array([2, 0], np.int32)), gpu(np.zeros((2, 5), np.int32)))
     assert bool((acc[0, 0, :, 7:9] == 0).all()) and float(acc.sum()) == 2 * 2 * 48 - 4
+
+
+# ---------------------------------------------------------------- scratch
+
+def _long_trees(n=12):
+    from hymt2_b200.kvcache import PagedKV
+    import torch
+    rng = np.random.default_rng(2)
+    lens, trees = [900, 2, 333], [random_tree(rng, x) for x in (n, n, 1)]
+    kv, pages = make_cache(rng, 1, 4, 128, [950, 50, 400])
+    args = (torch.randn(2 * n + 1, 16, 128, device="cuda"), gpu(np.array(lens, np.int32)), gpu(np.array([0, n, 2 * n, 2 * n + 1], np.int32)),
+            gpu(np.concatenate(trees)))
+    return PagedKV(gpu(kv), gpu(pages)), args
+
+
+@pytest.mark.parametrize("n", [3, 40])
+def test_a_captured_call_has_a_scratch_of_its_own(n):
+    """Warmed up and captured on one side stream: replays use none of that stream's scratch, two graphs none of each
+    other's, and they outlive the handle."""
+    import torch
+    cache, args = _long_trees(n)
+    want = cache.tree_attention(*args, n)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(3):
+            cache.tree_attention(*args, n)
+    s.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            graphs.append((g, cache.tree_attention(*args, n)))
+    held = [ws[0] for ws in cache._ws.values()]
+    for buf in held:
+        buf.fill_(0x55)
+    torch.cuda.synchronize()
+    for g, _ in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(bool((buf == 0x55).all()) for buf in held)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):  # side by side
+        for st, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for _, out in graphs for o, w in zip(out, want))
+    kv, pages = cache.kv, cache.pages  # the graphs' inputs stay, their handle goes
+    del cache, held, buf
+    torch.cuda.empty_cache()
+    for g, out in graphs:
+        out[0].zero_()
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for _, out in graphs for o, w in zip(out, want)) and kv.is_cuda and pages.is_cuda
+
+
+def test_one_scratch_for_all_widths():
+    import torch
+    cache, args = _long_trees(12)
+    want = cache.tree_attention(*args, 12)
+    for n in list(range(12, 65)) + [12, 64, 12]:
+        out = cache.tree_attention(*args, n)[0]
+        assert float((out - want[0]).abs().max()) < 1e-4   # other splits and forms of the same sums
+    assert len(cache._ws) == 1
+    need = [cache._lib.hyc_tree_attention_ws(cache._ref, 16, n) for n in range(12, 65)]
+    assert next(iter(cache._ws.values()))[0].numel() == max(need)
+    assert all(ws is next(iter(cache._ws.values())) for ws in cache._fit.values())
+    torch.cuda.synchronize()
