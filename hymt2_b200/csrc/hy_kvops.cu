@@ -553,6 +553,7 @@ HYC_API int hyc_tree_attention_n(void *stream, const hyc_kv_view *cache, int lay
     if (layer < 0 || layer >= a.v.layers) return op_fail(err, err_cap, -1, "no such layer");
     if (max_nodes < 1 || max_nodes > kTreeMax) return op_fail(err, err_cap, -1, "max_nodes must be 1 .. 64");
     if (!d_len || !d_off || !d_parent || !d_q || !d_out || !d_ws) return op_fail(err, err_cap, -1, "null argument");
+    if (!std::isfinite(scale)) return op_fail(err, err_cap, -1, "scale must be finite");
     const int el = q_bf16 ? 2 : 4;
     if (!aligned16(d_q) || !aligned16(d_out) || ((uintptr_t)d_ws & 255) || (q_ld * el) % 16 || (out_ld * el) % 16 ||
         q_ld < (long long)heads * a.v.hd || out_ld < (long long)heads * a.v.hd)
@@ -680,6 +681,7 @@ HYC_API int hyc_cache_weights_n(void *stream, const hyc_kv_view *cache, int head
     if (max_q < 1 || max_q > kTreeMax) return op_fail(err, err_cap, -1, "max_q must be 1 .. 64");
     if (!d_len || !d_nq || !d_sel || !d_q || !d_lse || !d_acc || acc_rows < 1)
         return op_fail(err, err_cap, -1, "null argument");
+    if (!std::isfinite(scale)) return op_fail(err, err_cap, -1, "scale must be finite");
     const int el = q_bf16 ? 2 : 4;
     if (!aligned16(d_q) || (q_ld * el) % 16 || (q_layer * el) % 16 || q_ld < (long long)heads * a.v.hd)
         return op_fail(err, err_cap, -1, "q must be 16-byte aligned with rows of heads * hdim or more");

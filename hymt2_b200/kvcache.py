@@ -75,7 +75,7 @@ class PagedKV:
         bf16 = q.dtype is torch.bfloat16
         if not bf16 and q.dtype is not torch.float32 or q.get_device() != self._dev:
             raise ValueError(f"q must be float32 or bfloat16 on {self.device}")
-        if hd != self.hdim or heads % self.kv_heads or stride[-1] != 1 or stride[-2] != hd:
+        if hd != self.hdim or heads % self.kv_heads or stride[-1] != 1 or (stride[-2] != hd and heads > 1):
             raise ValueError("q must be [..., heads, hdim] with contiguous tokens, heads a multiple of kv_heads")
         return bf16
 
@@ -135,7 +135,7 @@ class PagedKV:
         if out is None:
             out = q.new_empty(nt, heads, hd)
         elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != self._dev or out.stride(2) != 1 or \
-                out.stride(1) != hd:
+                (out.stride(1) != hd and heads > 1):
             raise ValueError("out must be shaped and typed like q with contiguous tokens")
         elif nt > 1:
             old_out = out.stride(0)

@@ -387,3 +387,42 @@ def test_one_scratch_for_all_widths():
     assert next(iter(cache._ws.values()))[0].numel() == max(need)
     assert all(ws is next(iter(cache._ws.values())) for ws in cache._fit.values())
     torch.cuda.synchronize()
+
+
+def test_queries_of_one_head():
+    """One head has no stride of its own: any that torch carries for it will do."""
+    import torch
+    from hymt2_b200.kvcache import PagedKV
+    rng = np.random.default_rng(4)
+    kv, pages = make_cache(rng, 2, 1, 64, [60])
+    cache, n = PagedKV(gpu(kv), gpu(pages)), 5
+    lens, off, par = gpu(np.array([50], np.int32)), gpu(np.array([0, n], np.int32)), gpu(random_tree(rng, n))
+    q = torch.randn(2, n, 1, 64, device="cuda")
+    want, lse = cache.tree_attention(q[0], lens, off, par, n)
+    odd = q[0].transpose(0, 1).contiguous().transpose(0, 1)   # [n][1][64] of strides (64, 64 n, 1)
+    assert odd.stride(1) == 64 * n
+    out = torch.zeros(1, n, 64, device="cuda").transpose(0, 1)
+    got, lse2 = cache.tree_attention(odd, lens, off, par, n, out=out)
+    assert torch.equal(got, want) and torch.equal(lse, lse2)
+    acc = [torch.zeros(2, 1, 1, 64, device="cuda") for _ in range(2)]
+    sel, e = gpu(np.arange(n, dtype=np.int32)[None]), torch.full((2, n, 1), 3.0, device="cuda")
+    for a, x in zip(acc, (q, q.transpose(1, 2).contiguous().transpose(1, 2))):
+        cache.add_weights(a, x, e, lens, gpu(np.array([n], np.int32)), sel)
+    assert torch.equal(*acc) and bool((acc[0] != 0).any())
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf")])
+def test_a_scale_that_is_not_finite_is_refused(scale):
+    """(It was taken for one next to 0: every row the same weight.)"""
+    import torch
+    from hymt2_b200.device import BackendError
+    from hymt2_b200.kvcache import PagedKV
+    rng = np.random.default_rng(4)
+    kv, pages = make_cache(rng, 1, 1, 64, [60])
+    cache, q = PagedKV(gpu(kv), gpu(pages)), torch.randn(1, 1, 64, device="cuda")
+    one, off = gpu(np.array([50], np.int32)), gpu(np.array([0, 1], np.int32))
+    with pytest.raises(BackendError, match="scale"):
+        cache.tree_attention(q, one, off, gpu(np.array([-1], np.int32)), 1, scale=scale)
+    with pytest.raises(BackendError, match="scale"):
+        cache.add_weights(torch.zeros(1, 1, 1, 64, device="cuda"), q[None], torch.zeros(1, 1, 1, device="cuda"), one, off[1:],
+                          gpu(np.zeros((1, 1), np.int32)), scale=scale)
