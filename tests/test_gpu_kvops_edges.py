@@ -399,14 +399,14 @@ def test_queries_of_one_head():
     lens, off, par = gpu(np.array([50], np.int32)), gpu(np.array([0, n], np.int32)), gpu(random_tree(rng, n))
     q = torch.randn(2, n, 1, 64, device="cuda")
     want, lse = cache.tree_attention(q[0], lens, off, par, n)
-    odd = q[0].transpose(0, 1).contiguous().transpose(0, 1)   # [n][1][64] of strides (64, 64 n, 1)
+    odd = torch.empty(1, n, 64, device="cuda").copy_(q[0].transpose(0, 1)).transpose(0, 1)   # [n][1][64] of strides (64, 64 n, 1)
     assert odd.stride(1) == 64 * n
     out = torch.zeros(1, n, 64, device="cuda").transpose(0, 1)
     got, lse2 = cache.tree_attention(odd, lens, off, par, n, out=out)
     assert torch.equal(got, want) and torch.equal(lse, lse2)
     acc = [torch.zeros(2, 1, 1, 64, device="cuda") for _ in range(2)]
     sel, e = gpu(np.arange(n, dtype=np.int32)[None]), torch.full((2, n, 1), 3.0, device="cuda")
-    for a, x in zip(acc, (q, q.transpose(1, 2).contiguous().transpose(1, 2))):
+    for a, x in zip(acc, (q, torch.empty(2, 1, n, 64, device="cuda").copy_(q.transpose(1, 2)).transpose(1, 2))):
         cache.add_weights(a, x, e, lens, gpu(np.array([n], np.int32)), sel)
     assert torch.equal(*acc) and bool((acc[0] != 0).any())
 
