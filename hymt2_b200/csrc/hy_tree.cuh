@@ -163,6 +163,7 @@ bool tree_run(HyCtx *c, const int *tokens, const int *parent, const int *off, co
         for (int i = 0; i < n; i++) {
             const int k = off[s] + i, p = parent[k];
             REQ(c, i == 0 ? p == -1 : p >= 0 && p < i, "node 0 has parent -1, every other node one below itself");
+            REQ(c, !forced || !forced[s] || p == i - 1, "a forced slot's nodes are a chain");
             pos[k] = i == 0 ? t.pos[s] : pos[off[s] + p] + 1;
             REQ(c, pos[k] < c->ctx, "a position is past the prepared context");
             tok[k] = tokens[k];

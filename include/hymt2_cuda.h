@@ -222,8 +222,8 @@ HYC_API int hyc_serve(void *impl, const int *prompts, const int *prompt_off, int
  * every token is the model's own choice after the one before; path[s]
  * [max_nodes] are their token numbers (-1 behind), next[s] the model's choice
  * after the last of them, which is node 0 of the slot's next tree.  Slots with
- * forced[s] != 0 (forced may be NULL) keep all their nodes, a given chain such
- * as a prompt's last tokens.  The ids are those of one-token steps.
+ * forced[s] != 0 (forced may be NULL) keep all their nodes, which must be a
+ * chain (each the next one's parent), such as a prompt's last tokens.  The ids are those of one-token steps.
  * hyc_tree_evict: every slot with more than budget rows keeps its first
  * `sinks`, last `recent` and, in each layer and KV head, its heaviest other
  * rows, budget in all; positions go on.  All other rows stay as they are, and

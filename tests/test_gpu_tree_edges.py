@@ -131,3 +131,17 @@ def test_the_server_empties_the_slots(backend, synth, model_dir):
         assert np.allclose(dm.tree_state(0, weights=True)[2].sum(-1), dm.hp.heads // dm.hp.kv_heads, rtol=1e-4)
     finally:
         dm.close()
+
+
+def test_forced_nodes_are_a_chain(backend, synth, model_dir):
+    """All of a forced slot's nodes become rows one after the other; two of one position would not be a sequence."""
+    from hymt2_b200.device import BackendError
+    dm = _open(backend, synth, model_dir, slots=2)
+    try:
+        for parents in ([-1, 0, 0], [-1, 0, 1, 1]):
+            with pytest.raises(BackendError, match="chain"):
+                dm.tree_forward({0: ([1] * len(parents), parents)}, 2, forced=[0])
+        assert dm.tree_state(0)[:2] == (0, 0)
+        assert dm.tree_forward({0: ([1, 2, 3], [-1, 0, 1]), 1: ([1, 2, 3], [-1, 0, 0])}, 2, forced=[0])[0][0] == [1, 2, 3]
+    finally:
+        dm.close()
