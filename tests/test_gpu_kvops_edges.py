@@ -426,3 +426,99 @@ def test_a_scale_that_is_not_finite_is_refused(scale):
     with pytest.raises(BackendError, match="scale"):
         cache.add_weights(torch.zeros(1, 1, 1, 64, device="cuda"), q[None], torch.zeros(1, 1, 1, device="cuda"), one, off[1:],
                           gpu(np.zeros((1, 1), np.int32)), scale=scale)
+
+
+# ---------------------------------------------------------------- pages that are not there, lengths out of range
+
+NO_PAGE = (-1, -2 ** 31, 2 ** 31 - 1)
+
+
+def holes(rng, kv, pages, slots):
+    """Page tables with numbers outside the pool in some places, and for the plain form a pool with a page of zeros there."""
+    import torch
+    plain_kv = torch.cat([kv, torch.zeros_like(kv[:, :1])], 1)
+    plain, table = pages.copy(), pages.copy()
+    for s in slots:
+        for i, j in enumerate(rng.choice(pages.shape[1], max(1, pages.shape[1] // 3), replace=False)):
+            plain[s, j] = kv.shape[1]
+            table[s, j] = (*NO_PAGE, kv.shape[1])[i % 4]
+    return plain_kv, plain, table
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("G,n,L", [(4, 5, 60), (4, 5, 700), (8, 13, 60), (8, 13, 700)])
+def test_attention_over_pages_that_are_not_there(G, n, L, bf16):
+    """They read as rows of zeros."""
+    import torch
+    rng = np.random.default_rng(n + L)
+    lens, trees = [L, 30], [random_tree(rng, n), random_tree(rng, n)]
+    kv, pages = make_cache(rng, 1, 2, 64, [L + n, 30 + n])
+    plain_kv, plain, table = holes(rng, kv, pages, (0, 1))
+    q = torch.from_numpy(rng.standard_normal((2 * n, 2 * G, 64)).astype(np.float32)).to(torch.bfloat16 if bf16 else torch.float32)
+    out, lse = run_tree(kv, table, 0, lens, trees, gpu(q), n)
+    want, wlse, tol, tlse = plain_tree(plain_kv, plain, 0, lens, trees, q.double().numpy(), G, 64 ** -0.5)
+    if bf16:
+        tol = tol + np.abs(want) * 2.0 ** -8
+    assert (np.abs(out - want) <= tol).all() and (np.abs(lse - wlse) <= tlse).all()
+
+
+@pytest.mark.parametrize("G,n", [(4, 5), (8, 13)])
+def test_lengths_out_of_range(G, n):
+    """Below 0 they count as 0, past the page table as all of its rows; nodes' rows past it do not exist."""
+    import torch
+    from hymt2_b200.kvcache import PagedKV
+    rng = np.random.default_rng(n)
+    kv, pages = make_cache(rng, 2, 2, 64, [160] * 4)
+    cap = pages.shape[1] * PAGE
+    cache, big = PagedKV(gpu(kv), gpu(pages)), np.iinfo(np.int32)
+    off, par = gpu(np.arange(5, dtype=np.int32) * n), gpu(np.concatenate([random_tree(rng, n) for _ in range(4)]))
+    q = torch.randn(2, 4 * n, 2 * G, 64, device="cuda")
+    wild, tame = (gpu(np.array(x, np.int32)) for x in ([-1, big.min, cap + 1, big.max], [0, 0, cap, cap]))
+    got, want = (cache.tree_attention(q[0], x, off, par, n) for x in (wild, tame))
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and bool(torch.isfinite(got[0]).all())
+    ref = plain_tree(kv, pages, 0, [0, 0, cap, cap], np.split(par.cpu().numpy(), 4), q[0].cpu().double().numpy(), G, 64 ** -0.5)
+    assert (np.abs(got[0].cpu().numpy() - ref[0]) <= ref[2]).all() and (np.abs(got[1].cpu().numpy() - ref[1]) <= ref[3]).all()
+    acc, e = [torch.ones(2, 4, 2, cap, device="cuda") for _ in range(2)], torch.full((2, 4 * n, 2 * G), 4.0, device="cuda")
+    sel, nq = gpu(np.arange(4 * n, dtype=np.int32).reshape(4, n)), gpu(np.array([n, big.max, n, -3], np.int32))
+    for a, x in zip(acc, (wild, tame)):
+        cache.add_weights(a, q, e, x, nq, sel)
+    assert torch.equal(*acc) and bool((acc[0][:, 3] == 1).all()) and bool((acc[0][:, 2] > 1).all())
+    assert bool((acc[0][:, :2, :, n:] == 1).all())
+    kept = [cache.evict(PagedKV(torch.zeros_like(cache.kv), cache.pages), x, acc[0], 20, 2, 5) for x in (wild, tame)]
+    assert all(torch.equal(a, b) for a, b in zip(*kept)) and kept[0][0].tolist() == [0, 0, 20, 20]
+
+
+def test_moves_over_pages_that_are_not_there():
+    """Commit and eviction: such rows move as zeros, and nothing is written in their place."""
+    import torch
+    from hymt2_b200.kvcache import PagedKV
+    rng = np.random.default_rng(6)
+    kv, pages = make_cache(rng, 2, 2, 64, [96])
+    par, n = np.array([-1, 0, 0, 2, 2, 4], np.int32), 6
+    tok, nxt = np.array([9, 1, 2, 3, 4, 5], np.int32), np.array([2, 0, 4, 0, 5, 0], np.int32)   # the path 0, 2, 4, 5
+    zero = torch.zeros(2, 2, 2, 64, dtype=torch.bfloat16)
+    row = lambda t, r: t[:, int(pages[0, r // PAGE]), :, r % PAGE]
+    for no in NO_PAGE + (kv.shape[1],):
+        for L, hole in ((29, 2), (29, 1), (13, 0), (91, 5)):
+            table, d = pages.copy(), gpu(kv)
+            table[0, hole] = no
+            PagedKV(d, gpu(table)).tree_commit(gpu(np.array([L], np.int32)), gpu(np.array([0, n], np.int32)), gpu(par), gpu(tok), gpu(nxt), n)
+            want = kv.clone()
+            for j, i in enumerate((0, 2, 4, 5)):
+                if i != j and (L + j) // PAGE != hole and L + j < 96:
+                    src = zero if L + i >= 96 or (L + i) // PAGE == hole else row(want, L + i).clone()
+                    row(want, L + j)[:] = src
+            assert torch.equal(d.cpu(), want), (no, L, hole)
+    acc = gpu(rng.random((2, 1, 2, 96)).astype(np.float32))
+    for no in NO_PAGE + (kv.shape[1],):
+        table = pages.copy()
+        table[0, 1] = no
+        dst, dtable = torch.full_like(kv, 7.0).cuda(), np.array([[3, no, 5]], np.int32)
+        _, kept, _ = PagedKV(gpu(kv), gpu(table)).evict(PagedKV(dst, gpu(dtable)), gpu(np.array([90], np.int32)), acc, 40, 3, 9)
+        kept, want = kept.cpu().numpy(), torch.full_like(kv, 7.0)
+        for l in range(2):
+            for h in range(2):
+                for j, r in enumerate(kept[l, 0, h]):
+                    if j // PAGE != 1:
+                        want[l, int(dtable[0, j // PAGE]), :, j % PAGE, h] = 0 if r // PAGE == 1 else kv[l, int(pages[0, r // PAGE]), :, r % PAGE, h]
+        assert torch.equal(dst.cpu(), want), no
