@@ -26,6 +26,7 @@ from .device import BackendError, load_library
 
 PAGE_ROWS = 16
 TREE_MAX = 64  # nodes of one tree
+_INT = torch.int32
 
 # The raw handle of a device's current stream without a Stream object around it, and whether it is being captured, where
 # torch has those calls.
@@ -50,6 +51,7 @@ class PagedKV:
         self.kv, self.pages, self.device, self._dev = kv, pages, kv.device, kv.get_device()
         self.layers, self.npages, _, _, self.kv_heads, self.hdim = kv.shape
         self.slots, self.page_max = pages.shape
+        self._one, self._offs = (self.slots,), (self.slots + 1,)  # shapes of lens and offsets
         self._view = abi.KVView(kv.data_ptr(), pages.data_ptr(), self.layers, self.npages, self.kv_heads, self.hdim,
                                 self.slots, self.page_max)
         self._ref = C.byref(self._view)
@@ -61,7 +63,7 @@ class PagedKV:
         self._none = kv.data_ptr()  # in place of an empty array: the library wants pointers, and reads nothing through these
 
     def _ints(self, name: str, t: torch.Tensor, shape: tuple) -> int:
-        if t.dtype is not torch.int32 or t.shape != shape or t.get_device() != self._dev or not t.is_contiguous():
+        if t.dtype is not _INT or t.shape != shape or t.get_device() != self._dev or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous int32 {list(shape)} on {self.device}")
         return t.data_ptr()
 
@@ -143,7 +145,7 @@ class PagedKV:
             lse = q.new_empty(nt, heads, dtype=torch.float32) if bf16 else q.new_empty(nt, heads)
         else:
             self._floats("lse", lse, (nt, heads))
-        ln, of = self._ints("lens", lens, (self.slots,)), self._ints("offsets", offsets, (self.slots + 1,))
+        ln, of = self._ints("lens", lens, self._one), self._ints("offsets", offsets, self._offs)
         pa = self._ints("parent", parent, (nt,))
         if nt == 0:
             return out, lse
@@ -161,8 +163,8 @@ class PagedKV:
 
         The path runs from node 0 to the first child whose token is next_tokens of the node before, and so on; its
         rows move up to rows lens[s] .. in every layer.  Slots with forced[s] != 0 take all their nodes."""
-        nt, one = (tokens.shape[0],), (self.slots,)
-        args = (self._ints("lens", lens, one), self._ints("offsets", offsets, (self.slots + 1,)),
+        nt, one = (tokens.shape[0],), self._one
+        args = (self._ints("lens", lens, one), self._ints("offsets", offsets, self._offs),
                 self._ints("parent", parent, nt) or self._none, self._ints("tokens", tokens, nt) or self._none,
                 self._ints("next_tokens", next_tokens, nt) or self._none,
                 None if forced is None else self._ints("forced", forced, one))
