@@ -63,7 +63,9 @@ int lg2(int G) { return G == 1 ? 0 : G == 2 ? 1 : G == 4 ? 2 : 3; }
 
 // Rows (nodes x heads of a group) up to which a tree takes the narrow form
 // (its own limit: four 8-row columns of registers; at 20 rows over 256 short
-// slots it took 53 us where the wide form took 67), and its most CTAs an SM.
+// slots it took 53 us where the wide form took 67; over one slot of 16000 rows
+// it takes 37 us for 32 rows where the wide form takes 28 for 36), and its most
+// CTAs an SM.
 constexpr int kNarrowRows = 32, kNarrowCtas = 3;
 
 bool group_ok(int heads, int kvh, int &G) {

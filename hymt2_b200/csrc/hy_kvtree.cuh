@@ -67,7 +67,7 @@ __device__ __forceinline__ float4 ld_row4(const __nv_bfloat16 *p) {
 // the same share whatever the lengths are.  Starting a column costs about as
 // much as tree_lead tiles, which stand before it in the count and hold no work
 // (without them CTAs with three short columns ended last: 74 -> 61 us at 32
-// slots of 300 to 3000 rows; in the narrow form, where several CTAs share an
+// slots of 300 to 3000 rows, the one case that three was chosen by; in the narrow form, where several CTAs share an
 // SM, one or two places took 49.5 us against 47.5 at 256 slots).  A column that ends up in several ranges leaves
 // (max, sum, out) pieces which tree_merge joins.
 template <int TK>
@@ -306,12 +306,18 @@ __device__ __noinline__ void tree_redo(const TreeArgs &a, int slot, int kvh, int
 // under it, as the same one divides out at the end.
 //
 // On a B200, in calls one after the other: 30 nodes over 32 slots of 300 to
-// 3000 rows, fp32 (120 rows a tile, 127 MB, 38 GFLOP in three terms) 61 us: the
+// 3000 rows, fp32 (120 rows a tile, 127 MB, 38 GFLOP in three terms) 64 us: the
 // products take 1.9 us a tile at the tensor cores' full rate, 22 us in all, the
-// rest is the change of column (about 6 us).  64 nodes over 12 slots of 11500 to
-// 16500 rows, bf16: 150 us, 1.3 us a tile, of which the products are 0.95 and
-// the waits between them the rest; each K and V tile is read by two CTAs at one
+// rest is the start, two or three changes of column a CTA (about 6 us each) and
+// the join.  64 nodes over 12 slots of 11500 to 16500 rows, bf16: 174 us, of
+// which this kernel is 152 by itself: 71 tiles a CTA, 2.1 us each, where the
+// products of a tile take 1.1.  A tile's softmax overlaps only the next Q . K^T,
+// so the tensor cores wait for it; each K and V tile is read by two CTAs at one
 // time (rows 0-127 and 128-255 of the tree), once from memory.
+//
+// Infinities and NaN: rows whose sum or output is not finite are done again by
+// tree_redo.  The look for them is one pass over a segment's outputs (no
+// difference in any of these times).
 constexpr int kTtK = 128;       // cached rows of a tile
 constexpr int kTtThreads = 384, kTtSoft = 256;
 // Registers of a softmax thread and of the others: 256 * 216 + 128 * 72 = 384 * 168, what the block is launched with.
@@ -772,7 +778,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
 // 256 slots of about 120 rows and 5 nodes).  The terms of fp32 queries and
 // probabilities and the lagging maximum are those of the wide form.
 //
-// 256 slots of 70 to 176 rows x 5 nodes, fp32 (81 MB): 46 us, bound by
+// 256 slots of 70 to 176 rows x 5 nodes, fp32 (81 MB): 47 us, bound by
 // instruction issue and its latencies (38 % of the slots with three CTAs an SM;
 // a tile takes a CTA 3.5 us, 2.2 of them in the products); one node over 55
 // rows: 8 us of kernel time.

@@ -89,8 +89,10 @@ __device__ __noinline__ float weights_redo(const WeightArgs &a, int layer, int s
 // On a B200, in calls one after the other: 3 fp32 queries over 32 layers x
 // 4096 rows, 4 KV heads (139 MB) 32 us, 4.3 TB/s, bound by K's bytes after 6 us
 // until the first queries are there; 31 bf16 queries over 16 slots of about
-// 4500 rows, 4 layers (316 MB) 64 us, 4.9 TB/s, bound by the exponentials and
-// sums of 124 columns a row (2.6 us a tile and group of warps).
+// 4500 rows, 4 layers (316 MB) 76 us, 4.2 TB/s (64 us in short runs, before the
+// power limit), 124 columns a row: the exponentials alone would take 33 us, and
+// most stalls are waits for tensor memory, 16 columns at a time.  A row whose
+// sum is not a number is summed again by weights_redo.
 // S^T = K . Q^T on the tensor cores: the cached rows are the 128 lanes of a
 // tile, the (query, head) pairs its columns, so a thread sums its row's
 // probabilities by itself.  K comes by TMA straight into the K-major operand

@@ -1,10 +1,12 @@
 """Greedy decoding with drafted token trees over a bounded KV cache.
 
-The reference generates one token per step (src/model.c:943-954).  A batch-1
-step is bound by reading the weights, so verifying a few guesses in the same
-pass costs little more than one token: `generate` feeds every slot a tree of
-guesses (DeviceModel.tree_forward), keeps the path the model agrees with, and
-returns the ids of the plain greedy loop.  With a budget, the cache of every
+The reference generates one token per step (src/model.c:943-954).  `generate`
+feeds every slot a tree of guesses in one pass (DeviceModel.tree_forward), keeps
+the path the model agrees with, and returns the ids of the plain greedy loop (up
+to near ties: passes of other sizes sum in another order).  Whether that is
+faster goes by the tree and the guesses: on the 32-layer STQ1_0 model a plain
+token takes 0.81 ms, a pass of one node 1.76, of 16 nodes 8.9, of 32 to 64 nodes
+3.3, so a pass of 32 or more should yield over four tokens.  With a budget, the cache of every
 slot is cut back to its heaviest rows as it grows (DeviceModel.tree_evict).
 
     python -m hymt2_b200.draft MODEL.gguf --budget 512

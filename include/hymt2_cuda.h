@@ -223,7 +223,9 @@ HYC_API int hyc_serve(void *impl, const int *prompts, const int *prompt_off, int
  * [max_nodes] are their token numbers (-1 behind), next[s] the model's choice
  * after the last of them, which is node 0 of the slot's next tree.  Slots with
  * forced[s] != 0 (forced may be NULL) keep all their nodes, which must be a
- * chain (each the next one's parent), such as a prompt's last tokens.  The ids are those of one-token steps.
+ * chain (each the next one's parent), such as a prompt's last tokens.  The ids
+ * are those of one-token steps up to near ties (passes of other sizes sum in
+ * another order).
  * hyc_tree_evict: every slot with more than budget rows keeps its first
  * `sinks`, last `recent` and, in each layer and KV head, its heaviest other
  * rows, budget in all; positions go on.  All other rows stay as they are, and
