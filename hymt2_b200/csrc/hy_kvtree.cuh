@@ -216,6 +216,23 @@ __device__ __forceinline__ float ex2_part(float x) {
     return f < FLT_MIN ? FLT_MIN : f;
 }
 
+// The factor of a part whose maximum is x in a join whose maximum is M (both may be +inf).
+__device__ __forceinline__ float join_part(float x, float M) {
+    const float f = ex2_part(x - M);
+    return x == M ? 1.f : f;
+}
+
+// Query rows (of the narrow form) to be done again: those with odd outputs, and
+// those whose nodes see a drafted row that was left out of the product.
+__device__ __noinline__ unsigned tree_again(const int8_t *s_up, int rows, int lg, unsigned odd, unsigned long long bad) {
+    unsigned again = 0;
+    for (int row = 0; row < rows; row++) {
+        const unsigned long long see = tree_mask(s_up, row >> lg);
+        if (see && (((odd >> row) & 1) || (see & bad))) again |= 1u << row;
+    }
+    return again;
+}
+
 // One (node, head) row over the rows r0 .. r1 - 1 that its node sees (mask: of
 // the drafted ones), by a whole warp in plain fp32 arithmetic, in place of a
 // row whose sum or output is not finite or which sees a V that is not.  The
@@ -227,7 +244,7 @@ __device__ __forceinline__ float ex2_part(float x) {
 template <typename T, int HD>
 __device__ __noinline__ void tree_redo(const TreeArgs &a, int slot, int kvh, int L, unsigned long long mask, int r0, int r1, int tok,
                                        int head, float sl2, float2 *ml, float *po, int step) {
-    constexpr int D = HD / 32, B = 4;  // dims of a lane; rows in flight
+    constexpr int D = HD / 32, B = 8;  // dims of a lane; rows at a time, all of one page
     const int lane = threadIdx.x & 31, d0 = lane * D;
     float q[D], o[D], m = -INFINITY, l = 0.f;
     bool nan = false;
@@ -238,32 +255,48 @@ __device__ __noinline__ void tree_redo(const TreeArgs &a, int slot, int kvh, int
         o[d] = 0.f;
     }
     const uint16_t *base = a.v.kv + a.layer * a.v.layer_stride + kvh * HD + d0;
-    for (int r = r0; r < r1; r += B) {
-        float k[B][D], v[B][D];
+    for (int r = r0; r < r1; r += B) {  // r0 is a multiple of a tile
+        const int pg = a.v.page(slot, r);
+        const uint16_t *row = base + a.v.row(0, max(pg, 0), r);
+        uint32_t k[B][D / 2], v[B][D / 2];  // pairs of dims
+#pragma unroll
+        for (int i = 0; i < B; i++)
+#pragma unroll
+            for (int d = 0; d < D / 2; d++) {
+                const bool on = pg >= 0 && r + i < r1;
+                k[i][d] = on ? *(const uint32_t *)(row + i * a.v.kvd + 2 * d) : 0u;
+                v[i][d] = on ? *(const uint32_t *)(row + (kPageRows + i) * a.v.kvd + 2 * d) : 0u;
+            }
+        float x[B], mn = m;
 #pragma unroll
         for (int i = 0; i < B; i++) {
-            const int pg = r + i < r1 ? a.v.page(slot, r + i) : -1;
-            const uint16_t *row = base + a.v.row(0, max(pg, 0), r + i);
+            x[i] = 0.f;
 #pragma unroll
-            for (int d = 0; d < D; d++) {
-                k[i][d] = pg < 0 ? 0.f : bf16_bits_to_f32(row[d]);
-                v[i][d] = pg < 0 ? 0.f : bf16_bits_to_f32(row[kPageRows * a.v.kvd + d]);
-            }
+            for (int d = 0; d < D; d++) x[i] = fmaf(q[d], __uint_as_float(d & 1 ? k[i][d / 2] & 0xffff0000u : k[i][d / 2] << 16), x[i]);
         }
 #pragma unroll
+        for (int w = 16; w > 0; w >>= 1)
+#pragma unroll
+            for (int i = 0; i < B; i++) x[i] += __shfl_xor_sync(0xffffffffu, x[i], w);
+#pragma unroll
         for (int i = 0; i < B; i++) {
-            if (r + i >= r1 || (r + i >= L && !((mask >> (r + i - L)) & 1))) continue;
-            float x = 0.f;
+            const bool see = r + i < r1 && (r + i < L || ((mask >> (r + i - L)) & 1));
+            x[i] = see ? x[i] * sl2 : -INFINITY;
+            nan |= x[i] != x[i];
+            mn = fmaxf(mn, x[i]);
+        }
+        const float f = m == mn ? 1.f : m == -INFINITY ? 0.f : ex2_part(m - mn);
+        m = mn;
+        l *= f;
 #pragma unroll
-            for (int d = 0; d < D; d++) x = fmaf(q[d], k[i][d], x);
-            x = warp_sum(x) * sl2;
-            if (x == -INFINITY) continue;
-            nan |= x != x;
-            const float mn = fmaxf(m, x), f = m == mn ? 1.f : m == -INFINITY ? 0.f : ex2_part(m - mn), p = ex2_part(x - mn);
-            m = mn;
-            l = fmaf(l, f, p);
+        for (int d = 0; d < D; d++) o[d] *= f;
 #pragma unroll
-            for (int d = 0; d < D; d++) o[d] = fmaf(p, v[i][d], o[d] * f);
+        for (int i = 0; i < B; i++) {
+            if (x[i] == -INFINITY) continue;
+            const float p = ex2_part(x[i] - m);
+            l += p;
+#pragma unroll
+            for (int d = 0; d < D; d++) o[d] = fmaf(p, __uint_as_float(d & 1 ? v[i][d / 2] & 0xffff0000u : v[i][d / 2] << 16), o[d]);
         }
     }
     if (m == INFINITY && !nan) l = 1.f;  // lse = +inf
@@ -742,10 +775,10 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attn_tc(const __grid_const
                         for (int d = 0; d < W; d += 8) st_row8(po + d * 128, o + d, 1.f, true);
                     }
                 }
-                for (unsigned who = __ballot_sync(0xffffffffu, redo && h == 0); who; who &= who - 1) {  // rare
+                // rare: the two halves' warps, which agree on the rows, take every other one
+                for (unsigned who = __ballot_sync(0xffffffffu, redo) & (h ? 0xaaaaaaaau : 0x55555555u); who; who &= who - 1) {
                     const int row = (warp & 3) * 32 + __ffs(who) - 1, nd = node0 + (row >> a.lg);
-                    unsigned long long see = tree_mask(s_up, nd);
-                    tree_redo<T, HD>(a, cur.slot, cur.kvh, L, see, cur.a * kTtK, min(t1 * kTtK, end), cur.t0 + nd,
+                    tree_redo<T, HD>(a, cur.slot, cur.kvh, L, tree_mask(s_up, nd), cur.a * kTtK, min(t1 * kTtK, end), cur.t0 + nd,
                                      cur.kvh * a.G + (row & (a.G - 1)), sl2, whole ? nullptr : a.part_ml + (size_t)piece * 128 + row,
                                      a.part_o + (size_t)piece * 128 * HD + row * 8, 1024);
                 }
@@ -823,7 +856,7 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
     __shared__ int s_scan[kTnWarps], s_start[4];
     __shared__ int8_t s_up[kTreeMax];
     __shared__ float s_mx[kTnWarps][NT * 8];
-    __shared__ unsigned s_redo;  // rows with outputs that are not finite
+    __shared__ unsigned s_odd;  // rows with outputs that are not finite
     __shared__ unsigned long long s_bad, s_mask[NT * 8];  // s_mask: what a query row's node sees of its tree
     uint8_t *bk = dsm, *bv = dsm + kTnK * ROW;
     uint2 *qf = (uint2 *)(bv + kTnK * ROW);    // Q fragments [term][16 dims][8 rows][lane]
@@ -841,7 +874,7 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
     }
     if (th == 0) {  // first used after the barriers of the first tile
         s_bad = 0;
-        s_redo = 0;
+        s_odd = 0;
     }
     const auto step = [&](TreeWalk<kTnK> &w) { return a.whole ? w.next_whole(a) : w.next(a, 0); };
     const int cap = a.v.page_max * kPageRows;
@@ -1083,7 +1116,9 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
             __syncthreads();  // P and V have been read
             copy(1);
         }
-        // the rows' sums: a warp's lanes, then the four warps
+        // the rows' sums: a warp's lanes, then the four warps; and which outputs
+        // are not finite (with a sum that is not, all are not)
+        unsigned odd = 0;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -1091,19 +1126,15 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
 #pragma unroll
                 for (int w = 4; w < 32; w <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], w);
                 if (g == 0) s_mx[warp][nt * 8 + 2 * tq + j] = l[nt][j];
-                float odd = 0.f;  // not 0: an output is not finite (with a sum that is not, all are not)
+                float x = 0.f;
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) odd = fmaf(o[mt][nt][j], 0.f, fmaf(o[mt][nt][2 + j], 0.f, odd));
-                if (odd != 0.f) atomicOr(&s_redo, 1u << (nt * 8 + 2 * tq + j));
+                for (int mt = 0; mt < MT; mt++) x = fmaf(o[mt][nt][j], 0.f, fmaf(o[mt][nt][2 + j], 0.f, x));
+                odd |= (x != 0.f ? 1u : 0u) << (nt * 8 + j);
             }
+        if (odd) atomicOr(&s_odd, odd << (2 * tq));
         __syncthreads();
-        const unsigned odd_rows = s_redo;
-        const unsigned long long bad = s_bad;
-        // whether a row is done again: it is one of those, or its node sees a drafted row that was left out above
-        const auto redo = [&](int row) {
-            const unsigned long long see = tree_mask(s_up, row >> a.lg);
-            return see && (((odd_rows >> row) & 1) || (see & bad));
-        };
+        unsigned again = 0;  // rare
+        if (s_odd || s_bad) again = tree_again(s_up, rows, a.lg, s_odd, s_bad);
         const bool whole = wc.s_a == 0 && wc.s_b == wc.T;
         const size_t piece = (size_t)2 * range + (wc.s_g != wc.g0);
 #pragma unroll
@@ -1111,7 +1142,7 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int row = nt * 8 + 2 * tq + j;
-                if (row >= rows || ((odd_rows || bad) && redo(row))) continue;
+                if (row >= rows || ((again >> row) & 1)) continue;
                 const int tok = wc.t0 + (row >> a.lg), head = wc.s_kvh * a.G + (row & (a.G - 1));
                 const float L = (s_mx[0][row] + s_mx[1][row]) + (s_mx[2][row] + s_mx[3][row]);
                 if (L == 0.f)  // a node that saw nothing: 0 times a cached row is not 0 where that is not finite
@@ -1137,19 +1168,18 @@ __global__ void __launch_bounds__(kTnThreads, 3) tree_attn_mma(const __grid_cons
                     if (g == 0 && warp == 0) a.part_ml[piece * (NT * 8) + row] = make_float2(m[nt][j], L);
                 }
             }
-        if (odd_rows || bad)  // rare
-            for (int row = warp; row < rows; row += kTnWarps) {
-                if (!redo(row)) continue;
-                const size_t at = piece * (NT * 8) + row;
-                tree_redo<T, HD>(a, wc.s_slot, wc.s_kvh, wc.L, tree_mask(s_up, row >> a.lg), wc.s_a * kTnK, min(wc.s_b * kTnK, end),
-                                 wc.t0 + (row >> a.lg), wc.s_kvh * a.G + (row & (a.G - 1)), sl2, whole ? nullptr : a.part_ml + at,
-                                 a.part_o + at * HD, 8);
-            }
+        for (int row = warp; again >> row; row += kTnWarps) {
+            if (!((again >> row) & 1)) continue;
+            const size_t at = piece * (NT * 8) + row;
+            tree_redo<T, HD>(a, wc.s_slot, wc.s_kvh, wc.L, tree_mask(s_up, row >> a.lg), wc.s_a * kTnK, min(wc.s_b * kTnK, end),
+                             wc.t0 + (row >> a.lg), wc.s_kvh * a.G + (row & (a.G - 1)), sl2, whole ? nullptr : a.part_ml + at,
+                             a.part_o + at * HD, 8);
+        }
         if (th == 0 && wc.s_a == 0 && !whole) a.roots[range] = make_int4(wc.s_slot, wc.s_kvh, wc.s_c, s_start[3]);
         __syncthreads();
         if (th == 0) {
             s_bad = 0;
-            s_redo = 0;
+            s_odd = 0;
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -1255,14 +1285,14 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constan
 #pragma unroll
                 for (int i = 0; i < B; i++)
                     if (ml[i].y != 0.f) mn = fmaxf(mn, ml[i].x);
-                const float old = M == mn ? 1.f : M == -INFINITY ? 0.f : ex2_part(M - mn);
+                const float old = M == -INFINITY ? 0.f : join_part(M, mn);
                 M = mn;
                 S *= old;
 #pragma unroll
                 for (int d = 0; d < D; d++) o[d] *= old;
 #pragma unroll
                 for (int i = 0; i < B; i++) {
-                    const float f = ml[i].y == 0.f ? 0.f : ml[i].x == M ? 1.f : ex2_part(ml[i].x - M);  // 0: nothing seen in this piece
+                    const float e = join_part(ml[i].x, M), f = ml[i].y == 0.f ? 0.f : e;  // 0: nothing seen in this piece
                     S = fmaf(ml[i].y, f, S);
 #pragma unroll
                     for (int d = 0; d < D; d++) o[d] = fmaf(v[i][d], f, o[d]);
@@ -1283,7 +1313,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge(const __grid_constan
 #pragma unroll
                 for (int d = 0; d < D; d++) o[d] = 0.f;
                 for (int i = 0; i < wpr; i++) {
-                    const float l = s_l[warp + i], f = l == 0.f ? 0.f : s_m[warp + i] == M ? 1.f : ex2_part(s_m[warp + i] - M);
+                    const float l = s_l[warp + i], e = join_part(s_m[warp + i], M), f = l == 0.f ? 0.f : e;
                     S = fmaf(l, f, S);
 #pragma unroll
                     for (int d = 0; d < D; d++) o[d] = fmaf(s_part[warp + i][d0 + d], f, o[d]);
